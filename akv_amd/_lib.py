@@ -83,6 +83,29 @@ _SIGNATURES = {
         [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int32, c_int32,
          c_int32, c_int32, _P, _P, _P, ctypes.c_float, _P, c_int32, c_int64, c_int64, c_int64, _P, _P],
     ),
+    "akv_tree_attention_workspace_bytes": (
+        c_int64,
+        [c_int64, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64],
+    ),
+    "akv_tree_attention": (
+        c_int32,
+        [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int32, c_int64, c_int32,
+         c_int32, c_int32, c_int32, _P, _P, c_int32, _P, c_int64, c_int64, c_int32, _P, c_int64, c_int32, _P,
+         _P, ctypes.c_float, _P, c_int32, c_int64, c_int64, c_int64, c_int64, _P, c_int64, _P, _P],
+    ),
+    "akv_qk_norm_rope": (
+        c_int32,
+        [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, c_int32, c_int64, c_int32, c_int32,
+         c_int32, c_int32, c_int32, _P, _P, c_int32, ctypes.c_float, _P, c_int32, _P, c_int32, c_int64,
+         c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int32, _P, _P, c_int64, c_int64, c_int64,
+         c_int64, c_int64, _P],
+    ),
+    "akv_step_maps": (
+        c_int32,
+        [_P, _P, c_int64, c_int64, _P, c_int32, _P, _P, c_int32, c_int32, _P, _P, c_int32, c_int64, _P,
+         c_int32, _P, c_int32, _P, c_int64, c_int64, c_int32, _P, _P, c_int64, c_int32, c_int64, _P, c_int64,
+         c_int32, _P, _P, _P],
+    ),
     "akv_context_attention": (
         c_int32,
         [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64, _P, _P, c_int64, c_int64,

@@ -6,12 +6,18 @@ layer's compacted rows from ``compact_rows`` / ``ContextDecodeRegistry.fill``,
 or a sliding-window layer's from ``fill_window``), normalised with per-head
 sink logits exactly as the reference's ``o * sigmoid(lse - sink)``
 (``akv/system/sglang/srt/layers/attention/context_backend.py:254-272``).
+``tree_attention`` is its form for several drafted tokens per request, the
+step that verifies a tree of them (speculative decoding, which the reference
+rejects: ``akv/system/sglang/srt/context_system/capabilities.py:72-73``).
 """
 
 import torch
 
 from . import _lib
 from .ops import _on_device, current_stream_handle
+
+_INDEX = {torch.int32: _lib.AKV_I32, torch.int64: _lib.AKV_I64}
+_TREE_DTYPES = {torch.bfloat16: _lib.AKV_BF16, torch.float16: _lib.AKV_F16, torch.float32: _lib.AKV_F32}
 
 
 def workspace_bytes(n_requests, kv_heads, head_dim, max_len):
@@ -61,4 +67,100 @@ def decode_attention(q, k_buffer, v_buffer, kv_indptr, kv_indices, out, *, scale
             current_stream_handle(q.device),
         )
     _lib.check(rc, "akv_decode_attention")
+    return out
+
+
+def tree_workspace_bytes(n_tokens, n_requests, q_heads, kv_heads, head_dim, max_len, max_new):
+    """Device bytes ``tree_attention`` needs for these sizes and bounds."""
+    need = _lib.calls().akv_tree_attention_workspace_bytes(n_tokens, n_requests, q_heads, kv_heads, head_dim, max_len,
+                                                           max_new)
+    if need < 0:
+        raise ValueError("tree attention takes head dims that are multiples of 8 up to 128 and whole q groups")
+    return need
+
+
+def tree_attention(q, k_buffer, v_buffer, qo_indptr, kv_indptr, kv_indices, out, *, scale, max_len, max_new,
+                   page_size=1, tree_mask=None, key_starts=None, sinks=None, workspace=None, status=None):
+    """Attention of each request's drafted tokens over the cache and each other.
+
+    ``q`` / ``out``: ``[N, q_heads, D]`` (bf16 or fp16 q; q's dtype or f32
+    out), request b's tokens ``qo_indptr[b]:qo_indptr[b + 1]``, n of them;
+    ``k_buffer`` / ``v_buffer``: one layer's ``[slots, kv_heads, D]`` pool,
+    which holds the drafted tokens' own rows already.  Request b's
+    ``kv_indptr[b + 1] - kv_indptr[b]`` keys end in those n; they lie at the
+    slots ``kv_indices[kv_indptr[b]:]`` (1-D, ``context_decode_indices``), or on
+    the pages of row b of a 2-D block table (``context_step_maps``), with
+    ``page_size`` slots each.  Token i sees the request's earlier keys from
+    rank ``key_starts[i]`` on (None: all), and of the drafted tokens those whose
+    bit is set in its ``tree_mask`` row (int64 words ``[N, words]``; None: a
+    chain, each token itself and those before it).  A token that sees no key
+    gets 0; a key at a slot outside the pool is seen by none.  ``sinks``: f32
+    ``[q_heads]``.  ``max_len`` (keys a request's tokens reach: its keys, or
+    window + n + 1) and ``max_new`` (its tokens) are host bounds that size the
+    launch and the workspace; the results do not depend on them.  Rows of
+    ``out`` behind the last token stay as they are.  Head dims: multiples of 8
+    up to 128.  ``status``: as for ``decode_attention``.
+    """
+    if q.dtype not in (torch.bfloat16, torch.float16) or q.ndim != 3 or q.stride(2) != 1:
+        raise ValueError("q must be bf16 or fp16 [tokens, q_heads, head_dim] with unit dim stride")
+    device, dtype = q.device, q.dtype
+    n, hq, d = q.shape
+    if k_buffer.ndim != 3 or v_buffer.shape != k_buffer.shape or k_buffer.shape[2] != d or k_buffer.dtype != dtype \
+            or v_buffer.dtype != dtype or k_buffer.stride(2) != 1 or v_buffer.stride(2) != 1:
+        raise ValueError("K/V must be matching [slots, kv_heads, head_dim] buffers of q's dtype and head_dim")
+    if out.shape != q.shape or out.dtype not in (dtype, torch.float32) or out.stride(2) != 1:
+        raise ValueError("out must be shaped like q, of its dtype or f32")
+    if out.data_ptr() == q.data_ptr() and n:
+        raise ValueError("out must not be q")
+    if qo_indptr.dtype not in _INDEX or kv_indptr.dtype != qo_indptr.dtype or qo_indptr.ndim != 1 \
+            or kv_indptr.shape != qo_indptr.shape or not qo_indptr.is_contiguous() or not kv_indptr.is_contiguous():
+        raise ValueError("qo_indptr and kv_indptr must be contiguous [requests + 1] of one int32/int64 dtype")
+    n_requests = qo_indptr.shape[0] - 1
+    if kv_indices.dtype != torch.int32 or kv_indices.ndim not in (1, 2) or (kv_indices.numel() and
+                                                                            kv_indices.stride(-1) != 1):
+        raise ValueError("kv_indices must be int32: a list of slots or a block table [requests, pages]")
+    if kv_indices.ndim == 2:
+        width = kv_indices.shape[1]
+        stride = kv_indices.stride(0) if n_requests > 1 else max(1, width)
+        if kv_indices.shape[0] != n_requests or stride < max(1, width):
+            raise ValueError("the block table needs a row per request, without overlap")
+    else:
+        if page_size != 1:
+            raise ValueError("pages need a block table")
+        width, stride = kv_indices.shape[0], 0
+    if tree_mask is not None and (tree_mask.dtype != torch.int64 or tree_mask.ndim != 2 or tree_mask.shape[0] != n
+                                  or (tree_mask.numel() and tree_mask.stride(1) != 1) or tree_mask.device != device):
+        raise ValueError("tree_mask must be int64 words [tokens, words] on q's device")
+    if key_starts is not None and (key_starts.dtype != torch.int32 or key_starts.shape != (n,)
+                                   or not key_starts.is_contiguous() or key_starts.device != device):
+        raise ValueError("key_starts must be contiguous int32 [tokens] on q's device")
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (hq,) or not sinks.is_contiguous()
+                              or sinks.device != device):
+        raise ValueError("sinks must be f32 [q_heads] on q's device")
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1 or status.device != device):
+        raise ValueError("status must be an int32 device word on q's device")
+    if device.type != "cuda" or not (k_buffer.device == v_buffer.device == out.device == qo_indptr.device
+                                     == kv_indptr.device == kv_indices.device == device):
+        raise ValueError("tree attention's tensors must be on one GPU")
+    if n == 0 or n_requests <= 0:
+        return out
+    hk = k_buffer.shape[1]
+    lib = _lib.calls()
+    if workspace is None:
+        need = lib.akv_tree_attention_workspace_bytes(n, n_requests, hq, hk, d, int(max_len), int(max_new))
+        workspace = torch.empty(max(16, need), dtype=torch.uint8, device=device)
+    elif workspace.device != device or not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous, on q's device")
+    with _on_device(device):
+        rc = lib.akv_tree_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), k_buffer.data_ptr(), v_buffer.data_ptr(), k_buffer.stride(0),
+            k_buffer.stride(1), v_buffer.stride(0), v_buffer.stride(1), k_buffer.shape[0], _TREE_DTYPES[dtype], n,
+            n_requests, hq, hk, d, qo_indptr.data_ptr(), kv_indptr.data_ptr(), _INDEX[qo_indptr.dtype],
+            kv_indices.data_ptr(), stride, width, int(page_size), _lib.ptr(tree_mask),
+            0 if tree_mask is None else tree_mask.stride(0), 0 if tree_mask is None else tree_mask.shape[1],
+            _lib.ptr(key_starts), _lib.ptr(sinks), float(scale), out.data_ptr(), _TREE_DTYPES[out.dtype],
+            out.stride(0), out.stride(1), int(max_len), int(max_new), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _lib.ptr(status), current_stream_handle(device),
+        )
+    _lib.check(rc, "akv_tree_attention")
     return out

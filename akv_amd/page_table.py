@@ -8,7 +8,9 @@ Mirrors the reference's decode-index path:
 * ``kv_indptr[1:] = cumsum(seq_lens)`` (``akv/system/sglang.patch:2266-2268``)
   -> ``akv_build_indptr``;
 * ``ReqToTokenPool.write`` through side rows (``sglang.patch:4230-4235``)
-  -> ``akv_write_row_slots``.
+  -> ``akv_write_row_slots``;
+* the new tokens' side of a step (slots, positions, block tables, tree masks),
+  which the reference builds on the host -> ``akv_step_maps``.
 
 The reference's decode registry (``context_backend.py:666-809``) calls these
 with its own int64 rows ``(raw_ids_ptr, positions_ptr, prompt_len, active,
@@ -160,3 +162,91 @@ def write_req_to_token_pool(req_to_token, req_pool_indices, prefix_tensors, pre_
             len_t, loc_p, loc_t, len(req_pool_indices), current_stream_handle(device),
         )
     _lib.check(rc, "akv_write_extend_rows")
+
+
+def context_step_maps(registry, table, rows, seq_lens, new_lens, qo_indptr, kv_indptr, slot_map, positions, *,
+                      block_tables=None, page_size=1, parents=None, tree_mask=None, window=None, window_mask=None,
+                      window_starts=None, status=None):
+    """The metadata of a step's new tokens from request lengths, in one launch.
+
+    Request b has ``seq_lens[b]`` ranks, the last ``new_lens[b]`` of them new
+    (decoded or drafted tokens, or a prefill chunk), whose slots and positions
+    follow from its registry row as in ``context_decode_indices``.  Writes
+
+    * ``qo_indptr`` / ``kv_indptr`` ``[B + 1]``: cumulative sums of both;
+    * ``slot_map`` / ``positions`` ``[N]``: each new token's slot and position;
+      -1 and 0 behind the last one, so a padded batch stores nothing there;
+    * ``block_tables`` int32 ``[B, pages]``: the page of every ``page_size``-th
+      rank, -1 behind the request's last;
+    * ``tree_mask`` int64 ``[N, words]``: bit a of token i's row when new token
+      a is i or one of its ancestors.  ``parents`` int32 ``[N]`` names each
+      token's parent by its number among the request's new tokens (an earlier
+      one; anything else: none); without it a request's tokens are a chain.  A
+      token's position is its root's plus its depth;
+    * for layers with a sliding ``window`` (a key is visible when
+      ``q_pos - k_pos <= window``): ``window_mask``, the ancestors inside it,
+      and ``window_starts`` int32 ``[N]``, the first earlier key inside it.
+
+    ``rows`` may be int32 or int64; ``seq_lens`` and ``new_lens`` share either,
+    as do the indptrs; a mask has a word per 64 new tokens of a request.
+    ``status``: as for ``context_decode_indices``.
+    """
+    if registry.dtype != torch.int64 or registry.ndim != 2 or registry.shape[1] != 6 or not registry.is_contiguous():
+        raise ValueError("registry must be contiguous int64 [rows, 6]")
+    if table.dtype != torch.int32 or table.ndim != 2 or table.stride(1) != 1:
+        raise ValueError("the request table must be int32 [rows, width] with unit column stride")
+    batch = seq_lens.numel()
+    if new_lens.dtype != seq_lens.dtype or new_lens.numel() != batch or rows.numel() != batch:
+        raise ValueError("rows, seq_lens and new_lens must have one entry per request, the lengths one dtype")
+    if qo_indptr.dtype != kv_indptr.dtype or qo_indptr.numel() != batch + 1 or kv_indptr.numel() != batch + 1:
+        raise ValueError("qo_indptr and kv_indptr must be [requests + 1] of one dtype")
+    rows_p, rows_t = _idx(rows, "rows")
+    seq_p, len_t = _idx(seq_lens, "seq_lens")
+    new_p, _ = _idx(new_lens, "new_lens")
+    qo_p, ind_t = _idx(qo_indptr, "qo_indptr")
+    kv_p, _ = _idx(kv_indptr, "kv_indptr")
+    slot_p, slot_t = _idx(slot_map, "slot_map")
+    pos_p, pos_t = _idx(positions, "positions")
+    n = slot_map.numel()
+    if positions.numel() != n:
+        raise ValueError("slot_map and positions must have one entry per token")
+    device = slot_map.device
+    tensors = [registry, table, rows, seq_lens, new_lens, qo_indptr, kv_indptr, positions]
+    block_p, block_stride, block_width = None, 0, 0
+    if block_tables is not None:
+        if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.shape[0] != batch \
+                or (block_tables.numel() and block_tables.stride(1) != 1) \
+                or (batch > 1 and block_tables.stride(0) < block_tables.shape[1]):
+            raise ValueError("block_tables must be int32 [requests, pages] with unit column stride, without overlap")
+        block_p, block_stride, block_width = block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1]
+        tensors.append(block_tables)
+    if parents is not None:
+        if parents.dtype != torch.int32 or parents.numel() != n or not parents.is_contiguous():
+            raise ValueError("parents must be contiguous int32 with one entry per token")
+        tensors.append(parents)
+    if (window_mask is not None or window_starts is not None) and window is None:
+        raise ValueError("window_mask and window_starts need a window")
+    masks = []
+    for mask in (tree_mask, window_mask):
+        if mask is None:
+            masks.append((None, 0, 0))
+            continue
+        if mask.dtype != torch.int64 or mask.ndim != 2 or mask.shape[0] != n \
+                or (mask.numel() and mask.stride(1) != 1) or (n > 1 and mask.stride(0) < mask.shape[1]):
+            raise ValueError("masks must be int64 words [tokens, words] with unit word stride, without overlap")
+        masks.append((mask.data_ptr(), mask.stride(0), mask.shape[1]))
+        tensors.append(mask)
+    if window_starts is not None:
+        if window_starts.dtype != torch.int32 or window_starts.numel() != n or not window_starts.is_contiguous():
+            raise ValueError("window_starts must be contiguous int32 with one entry per token")
+        tensors.append(window_starts)
+    if device.type != "cuda" or any(t.device != device for t in tensors):
+        raise ValueError("step maps' tensors must be on one GPU")
+    with _on_device(device):
+        rc = _lib.calls().akv_step_maps(
+            registry.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], rows_p, rows_t, seq_p, new_p,
+            len_t, batch, qo_p, kv_p, ind_t, n, slot_p, slot_t, pos_p, pos_t, block_p, block_stride, block_width,
+            int(page_size), _lib.ptr(parents), *masks[0], 0 if window is None else int(window), *masks[1],
+            _lib.ptr(window_starts), _status_ptr(status, device), current_stream_handle(device),
+        )
+    _lib.check(rc, "akv_step_maps")

@@ -740,6 +740,128 @@ int akv_gather_slots(int32_t slot_dtype, const int64_t* sources,
                      int64_t total, int64_t wide_count, void* out_wide,
                      int32_t* out_narrow, void* stream);
 
+/*
+ * Metadata of a forward's new tokens (one launch): request b has
+ * L = seq_lens[b] ranks, the last n = new_lens[b] of them new (n is clamped to
+ * [0, L]); rank i's slot and position follow from its registry row as in
+ * akv_decode_indices.  Written, with P = page_size and W = window:
+ *   qo_indptr, kv_indptr [B + 1]  cumulative sums of n and L
+ *   slot_map[qo + i]       slot(L - n + i); -1 behind the last token
+ *   positions[qo + i]      position(L - n) + depth(i); 0 behind the last token
+ *   block_tables[b][j]     slot(j P) / P for j P < L, -1 behind (and for ranks
+ *                          without a slot); NULL: none
+ *   tree_mask[qo + i]      bit a: new token a is i or an ancestor of i
+ *   window_mask[qo + i]    bit a: the same, at most W levels up
+ *   window_starts[qo + i]  first rank of [0, L - n) whose position is at least
+ *                          positions[qo + i] - W (positions ascend)
+ * parents[qo + i] is a new token of the request before i, anything else none
+ * (depth 0); without parents token i follows i - 1.  Masks are rows of
+ * *_words 64-bit words, *_stride words apart; tokens past 64 words have no
+ * bits.  n_tokens is the capacity of the token vectors; seq_lens and new_lens
+ * share lens_dtype, the indptrs indptr_dtype.  table_width bounds the table's
+ * rows (a rank past it has no slot); side rows are not bounded.  status as in
+ * akv_decode_indices.
+ *
+ * The reading side's counterpart of the reference is
+ * akv/system/sglang/kernels/ops/attention/context_page_table.py:7-76; the
+ * reference builds the new tokens' side on the host.
+ */
+int akv_step_maps(const int64_t* registry, const int32_t* table,
+                  int64_t row_stride, int64_t table_width, const void* rows,
+                  int32_t rows_dtype, const void* seq_lens,
+                  const void* new_lens, int32_t lens_dtype, int32_t n_requests,
+                  void* qo_indptr, void* kv_indptr, int32_t indptr_dtype,
+                  int64_t n_tokens, void* slot_map, int32_t slots_dtype,
+                  void* positions, int32_t positions_dtype,
+                  int32_t* block_tables, int64_t block_stride,
+                  int64_t block_width, int32_t page_size,
+                  const int32_t* parents, uint64_t* tree_mask,
+                  int64_t tree_stride, int32_t tree_words, int64_t window,
+                  uint64_t* window_mask, int64_t window_stride,
+                  int32_t window_words, int32_t* window_starts,
+                  const int32_t* status, void* stream);
+
+/*
+ * Per-head RMS norms of q and k, the rotation, and the new K/V rows written
+ * to the pool.  For every token t and head row x of D = head_dim values:
+ * y = x / sqrt(mean(x^2) + eps) * weight in fp32, its first rotary_dim values
+ * rotated by row positions[t] of cos_sin (cos | sin; pairs i, i + R/2 with
+ * is_neox, 2i, 2i + 1 otherwise), rounded once to `dtype`.  q rows go to
+ * q_out (which may be q), k rows to k_out (which may be k; NULL: nowhere) and,
+ * with pools, to k_pool[slots[t]]; v rows are copied to v_pool[slots[t]].  A
+ * slot outside [0, pool_slots) writes no pool row.  A position outside
+ * [0, rope_rows) gives NaN rows and no K pool row.  A NULL weight is 1.
+ * Strides are in elements, the last dimension's is 1; slots are distinct.
+ *
+ * No counterpart in the reference, whose engine's model code norms and rotates
+ * before the pool write; the table and pair styles are those of
+ * akv/system/sglang/kernels/ops/attention/context_reposition.py:82-102.
+ */
+int akv_qk_norm_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                     const void* k, int64_t k_stride_t, int64_t k_stride_h,
+                     const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                     int32_t dtype, int64_t n_tokens, int32_t q_heads,
+                     int32_t kv_heads, int32_t head_dim, int32_t rotary_dim,
+                     int32_t is_neox, const void* q_weight,
+                     const void* k_weight, int32_t weight_dtype, float eps,
+                     const void* positions, int32_t positions_dtype,
+                     const void* cos_sin, int32_t cos_sin_dtype,
+                     int64_t rope_stride, int64_t rope_rows, void* q_out,
+                     int64_t qo_stride_t, int64_t qo_stride_h, void* k_out,
+                     int64_t ko_stride_t, int64_t ko_stride_h,
+                     const void* slots, int32_t slots_dtype, void* k_pool,
+                     void* v_pool, int64_t pool_slots, int64_t kp_stride_slot,
+                     int64_t kp_stride_head, int64_t vp_stride_slot,
+                     int64_t vp_stride_head, void* stream);
+
+/*
+ * Attention of drafted tokens over a cache.  Request b's tokens are
+ * q[qo_indptr[b] .. qo_indptr[b + 1]), n of them; its kv_indptr[b + 1] -
+ * kv_indptr[b] keys end in the tokens' own n.  Token i sees an earlier key of
+ * rank j when j >= key_starts[token] (NULL: always), and the request's new
+ * token a when bit a of its tree_mask row is set (NULL: a <= i).  GQA, scaled
+ * scores, sinks in the denominator as in akv_decode_attention; a token that
+ * sees no key gets 0.  q, K and V are bf16 or fp16, the output q's type or
+ * f32; head_dim a multiple of 8 up to 128, any number of q heads per KV head.
+ *
+ * Slots: kv_indices[kv_indptr[b] + j] of a flat list of table_width entries
+ * (table_stride 0, page_size 1), or, with table_stride > 0, the block table
+ * row kv_indices + b * table_stride of table_width pages:
+ * page(j / page_size) * page_size + j % page_size.  A key whose slot lies
+ * outside [0, pool_slots), or whose entry outside the list, is seen by no
+ * token.  max_len (keys a request's tokens reach) and max_new (its tokens) are
+ * host bounds that only size the launch: results do not depend on them.
+ * n_tokens is the capacity of q and out; rows behind qo_indptr[B] stay as they
+ * are.  workspace: akv_tree_attention_workspace_bytes with the same arguments,
+ * 16-byte aligned, any contents; calls that share one must not overlap.
+ * status as in akv_decode_attention.
+ *
+ * The reference rejects speculative decoding
+ * (akv/system/sglang/srt/context_system/capabilities.py:72-73); the sinks are
+ * those of akv/system/sglang/srt/layers/attention/context_backend.py:254-272.
+ */
+int64_t akv_tree_attention_workspace_bytes(int64_t n_tokens, int32_t n_requests,
+                                           int32_t q_heads, int32_t kv_heads,
+                                           int32_t head_dim, int64_t max_len,
+                                           int64_t max_new);
+int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                       const void* k_buffer, const void* v_buffer,
+                       int64_t k_stride_slot, int64_t k_stride_head,
+                       int64_t v_stride_slot, int64_t v_stride_head,
+                       int64_t pool_slots, int32_t dtype, int64_t n_tokens,
+                       int32_t n_requests, int32_t q_heads, int32_t kv_heads,
+                       int32_t head_dim, const void* qo_indptr,
+                       const void* kv_indptr, int32_t indptr_dtype,
+                       const int32_t* kv_indices, int64_t table_stride,
+                       int64_t table_width, int32_t page_size,
+                       const uint64_t* tree_mask, int64_t mask_stride,
+                       int32_t mask_words, const int32_t* key_starts,
+                       const float* sinks, float scale, void* out,
+                       int32_t out_dtype, int64_t out_stride_t,
+                       int64_t out_stride_h, int64_t max_len, int64_t max_new,
+                       void* workspace, int64_t workspace_bytes,
+                       const int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

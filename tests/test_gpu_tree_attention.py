@@ -1,0 +1,272 @@
+"""Tree attention on the GPU against the 64-bit oracle, at the sizes, layouts
+and masks where it can go wrong."""
+
+import numpy as np
+import pytest
+import torch
+
+from akv_amd import attention
+from oracle import drafts
+from tests.drafts import Cache, attention_tolerance, f64
+
+pytestmark = pytest.mark.gpu
+
+
+def _run(c, *, mask, starts=None, sinks=None, out_dtype=None, scale=None, max_len=None, max_new=None, out=None,
+         k=None, v=None, workspace=None, indptr=torch.int32, q=None):
+    scale = c.q.shape[2] ** -0.5 if scale is None else scale
+    if out is None:
+        out = torch.full(c.q.shape, 7.0, dtype=out_dtype or c.q.dtype, device=c.device)
+    attention.tree_attention(
+        c.q if q is None else q, c.k.to(c.device) if k is None else k, c.v.to(c.device) if v is None else v,
+        c.qo.to(indptr), c.kv.to(indptr), c.indices, out, scale=scale, max_len=c.max_len if max_len is None else max_len,
+        max_new=c.max_new if max_new is None else max_new, page_size=c.page, tree_mask=mask,
+        key_starts=None if starts is None else torch.tensor(starts, dtype=torch.int32, device=c.device), sinks=sinks,
+        workspace=workspace)
+    return out
+
+
+def _check(c, out, requests, *, sinks=None, scale=None):
+    scale = c.q.shape[2] ** -0.5 if scale is None else scale
+    want, size, spread = drafts.tree_attention(f64(c.q), f64(c.k), f64(c.v), requests, scale,
+                                               None if sinks is None else f64(sinks))
+    got = f64(out)
+    tol = attention_tolerance(c.q.dtype, out.dtype, c.max_len, want, size, spread, np.abs(f64(c.v)).max(initial=0.0))
+    here = slice(0, c.total)
+    off = np.abs(got - want)[here] - tol[here]
+    assert not np.isnan(got[here]).any()
+    assert (off <= 0).all(), f"{(off > 0).sum()} values off, worst by {off.max():.3g}"
+    assert (got[c.total:] == 7.0).all(), "rows behind the last token were written"
+
+
+SHAPES = [
+    # q heads, kv heads, head_dim, dtype, page, old, new
+    (8, 1, 64, torch.bfloat16, 1, [0], [1]),
+    (8, 1, 64, torch.bfloat16, 1, [1], [1]),
+    (2, 2, 64, torch.bfloat16, 1, [63, 64, 65, 0, 255, 256, 257], [1, 2, 3, 4, 5, 16, 17]),
+    (16, 2, 64, torch.bfloat16, 1, [700, 0, 40, 300], [8, 5, 0, 33]),
+    (16, 2, 64, torch.bfloat16, 16, [700, 3, 40, 300], [8, 5, 0, 33]),
+    (16, 2, 64, torch.float16, 5, [511, 513, 1], [64, 65, 70]),
+    (14, 2, 64, torch.bfloat16, 1, [1000, 129], [9, 100]),
+    (3, 1, 128, torch.bfloat16, 1, [130, 127, 128, 0], [7, 11, 1, 40]),
+    (16, 4, 128, torch.float16, 16, [1500, 10], [8, 32]),
+    (12, 1, 128, torch.bfloat16, 1, [31, 33], [65, 130]),
+    (6, 2, 96, torch.bfloat16, 1, [200, 90], [6, 21]),
+    (4, 2, 80, torch.float16, 3, [200, 90], [6, 21]),
+    (5, 1, 40, torch.bfloat16, 1, [77], [19]),
+    (2, 1, 8, torch.float16, 1, [77, 5], [3, 64]),
+]
+
+
+@pytest.mark.parametrize("kind", ["chain", "tree", "any"])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_matches_oracle(device, shape, kind):
+    hq, hk, d, dtype, page, old, new = SHAPES[shape]
+    print(f"tree attention shape {shape} {SHAPES[shape]} {kind}", flush=True)
+    c = Cache(device, 100 + shape, old, new, q_heads=hq, kv_heads=hk, head_dim=d, dtype=dtype, page=page,
+              capacity=sum(new) + shape % 3)
+    seen, mask = c.masks(kind)
+    sinks = torch.randn(hq, generator=torch.Generator().manual_seed(shape)).to(device) if shape % 2 else None
+    out = _run(c, mask=mask, sinks=sinks, out_dtype=torch.float32 if kind == "any" else None,
+               indptr=torch.int64 if kind == "tree" else torch.int32)
+    _check(c, out, c.visible(seen), sinks=sinks)
+
+
+@pytest.mark.parametrize("d,page", [(64, 1), (64, 16), (128, 1), (96, 4)])
+def test_first_keys_of_a_window(device, d, page):
+    """Windows that begin anywhere, behind every key, and below zero."""
+    old, new = [900, 40, 0, 500], [6, 12, 3, 20]
+    c = Cache(device, 7 + d, old, new, q_heads=4, kv_heads=2, head_dim=d, dtype=torch.bfloat16, page=page)
+    rng = np.random.default_rng(d)
+    starts = np.concatenate([rng.integers(max(0, o - 130), o + 1, n) for o, n in zip(old, new)])
+    starts[:3] = [old[0], 0, old[0] - 1]
+    passed = starts.copy()
+    passed[3], starts[3] = -50, 0
+    passed[4], starts[4] = 5000, old[0]  # past the earlier keys: none of them
+    for kind in ("tree", "any"):
+        print(f"tree attention windows d={d} page={page} {kind}", flush=True)
+        seen, mask = c.masks(kind)
+        out = _run(c, mask=mask, starts=passed, max_len=160)
+        _check(c, out, c.visible(seen, starts))
+
+
+def test_narrow_window_of_a_long_request(device):
+    """Only the window's keys count, wherever the chunks begin."""
+    old, new = [5000, 3000], [16, 7]
+    c = Cache(device, 5, old, new, q_heads=8, kv_heads=2, head_dim=64, dtype=torch.bfloat16)
+    seen, mask = c.masks("tree")
+    starts = np.concatenate([np.full(n, o - 128) for o, n in zip(old, new)]) + np.arange(23) % 9
+    sinks = torch.linspace(-3, 3, 8, device=device)
+    out = _run(c, mask=mask, starts=starts, sinks=sinks, max_len=128 + 17)
+    _check(c, out, c.visible(seen, starts), sinks=sinks)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_long_requests_in_many_chunks(device, d):
+    old, new = [6000, 1, 2500], [3, 9, 16]
+    c = Cache(device, 11 + d, old, new, q_heads=8, kv_heads=2, head_dim=d, dtype=torch.bfloat16)
+    seen, mask = c.masks("tree")
+    out = _run(c, mask=mask, out_dtype=torch.float32)
+    _check(c, out, c.visible(seen))
+
+
+def test_bounds_only_size_the_launch(device):
+    """Bounds below and far above what the batch holds give the same rows."""
+    c = Cache(device, 21, [1200, 30, 700], [20, 3, 9], q_heads=8, kv_heads=2, head_dim=64, dtype=torch.bfloat16)
+    seen, mask = c.masks("tree")
+    for max_len, max_new in ((c.max_len, c.max_new), (1, 1), (0, 0), (100000, 400), (300, 64)):
+        print(f"tree attention bounds {max_len} {max_new}", flush=True)
+        _check(c, _run(c, mask=mask, max_len=max_len, max_new=max_new), c.visible(seen))
+
+
+@pytest.mark.parametrize("page", [1, 16])
+def test_holes_are_not_read(device, page):
+    """Slots outside the pool, and lists shorter than the lengths say."""
+    c = Cache(device, 31, [400, 90], [5, 9], q_heads=4, kv_heads=2, head_dim=64, dtype=torch.bfloat16, page=page,
+              holes=6)
+    seen, mask = c.masks("tree")
+    _check(c, _run(c, mask=mask), c.visible(seen))
+    # the last request's entries end early
+    if page == 1:
+        cut = 40
+        c.indices = c.indices[: -1 - cut].contiguous()
+        c.slots[1][-cut:] = -1
+    else:
+        keep = 3
+        c.indices = c.indices[:, :keep].contiguous()
+        for s in c.slots:
+            s[keep * page:] = -1
+    _check(c, _run(c, mask=mask), c.visible(seen))
+
+
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.float16), (96, torch.bfloat16)])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan"), "lowest"])
+def test_what_a_token_does_not_see_cannot_reach_it(device, d, dtype, value):
+    """Infinities, NaN and the type's lowest value in keys and values that are
+    hidden from some tokens; those that see them are left out here."""
+    value = torch.finfo(dtype).min if value == "lowest" else value
+    old, new = [130, 70], [12, 40]
+    c = Cache(device, 41 + d, old, new, q_heads=4, kv_heads=2, head_dim=d, dtype=dtype)
+    seen, mask = c.masks("any")
+    starts = np.concatenate([np.full(n, 20) + np.arange(n) % 7 for n in new])
+    # a drafted token's rows, and earlier keys below some or all starts
+    bad = {0: [3, 21, 23, 130 + 4, 130 + 7], 1: [0, 24, 70 + 2, 70 + 33]}
+    for b, ranks in bad.items():
+        for r in ranks:
+            c.v[c.slots[b][r], :, (5 * r) % d] = value
+            if r % 2:
+                c.k[c.slots[b][r], :, (3 * r) % d] = value
+    out = f64(_run(c, mask=mask, starts=starts))
+    clean = Cache(device, 41 + d, old, new, q_heads=4, kv_heads=2, head_dim=d, dtype=dtype)
+    requests = c.visible(seen, starts)
+    want, size, spread = drafts.tree_attention(f64(c.q), f64(clean.k), f64(clean.v), requests, d ** -0.5)
+    tol = attention_tolerance(dtype, dtype, c.max_len, want, size, spread, np.abs(f64(clean.v)).max())
+    checked = 0
+    for b, (first, _, keys) in enumerate(requests):
+        for i in range(len(keys)):
+            if not keys[i][bad[b]].any():
+                checked += 1
+                assert (np.abs(out[first + i] - want[first + i]) <= tol[first + i]).all(), (b, i)
+    assert checked >= 4
+    # a token that sees a NaN or infinite value (its key untouched) has it in that dim
+    if value != torch.finfo(dtype).min:
+        hit = 0
+        for b, (first, _, keys) in enumerate(requests):
+            for r in bad[b]:
+                for i in np.flatnonzero(keys[:, r]):
+                    if r % 2 == 0 and not any(keys[i][o] for o in bad[b] if o % 2 and o != r):
+                        hit += 1
+                        assert not np.isfinite(out[first + i, :, (5 * r) % d]).any(), (b, i, r)
+        assert hit
+
+
+def test_nan_queries_stay_in_their_rows(device):
+    c = Cache(device, 51, [300], [9], q_heads=8, kv_heads=2, head_dim=64, dtype=torch.bfloat16)
+    seen, mask = c.masks("tree")
+    clean = f64(_run(c, mask=mask))
+    c.q[4, 3] = float("nan")
+    out = f64(_run(c, mask=mask))
+    assert np.isnan(out[4, 3]).all()
+    out[4, 3] = clean[4, 3]
+    np.testing.assert_array_equal(out, clean)
+
+
+@pytest.mark.parametrize("scores", ["rising", "falling", "far"])
+def test_scores_far_apart(device, scores):
+    """Maxima that keep moving, by little and by more than fp32's range."""
+    c = Cache(device, 61, [900], [10], q_heads=4, kv_heads=1, head_dim=64, dtype=torch.bfloat16)
+    ramp = torch.linspace(-1, 1, 910) if scores != "far" else torch.where(torch.arange(910) % 300 == 299, 40.0, -1.0)
+    c.k[:] = 0.01 * c.k
+    c.k[torch.from_numpy(c.slots[0]), 0, 0] = ((-ramp if scores == "falling" else ramp) * 30).to(torch.bfloat16)
+    c.q[:] = 0.01 * c.q
+    c.q[:, :, 0] = 2.0
+    seen, mask = c.masks("tree")
+    _check(c, _run(c, mask=mask, scale=1.0, out_dtype=torch.float32), c.visible(seen), scale=1.0)
+
+
+def test_strides(device):
+    """q, K, V and out as views: padded heads, a pool of interleaved K and V, a
+    wider table."""
+    c = Cache(device, 71, [200, 60], [7, 4], q_heads=4, kv_heads=2, head_dim=64, dtype=torch.bfloat16, page=16)
+    q = torch.zeros((c.total, 4, 80), dtype=torch.bfloat16, device=device)[:, :, 8:72]
+    q.copy_(c.q)
+    both = torch.stack((c.k, c.v), 2).to(device)  # [slots, heads, 2, dim]
+    store = torch.full((c.total, 6, 64), 7.0, dtype=torch.bfloat16, device=device)
+    c.indices = torch.nn.functional.pad(c.indices, (0, 5), value=123456)[:, : c.indices.shape[1]]
+    seen, mask = c.masks("tree")
+    mask = torch.nn.functional.pad(mask, (0, 3), value=-1)[:, : mask.shape[1]]
+    out = _run(c, mask=mask, q=q, k=both[:, :, 0], v=both[:, :, 1], out=store[:, 1:5])
+    _check(c, out, c.visible(seen))
+    assert (store[:, 0] == 7).all() and (store[:, 5] == 7).all()
+
+
+def test_one_workspace_for_changing_batches(device):
+    """Whatever an earlier call left in a workspace does not matter."""
+    shape = dict(q_heads=8, kv_heads=2, head_dim=64, dtype=torch.bfloat16)
+    batches = [Cache(device, 81, [900, 10], [12, 3], **shape), Cache(device, 82, [40], [2], **shape),
+               Cache(device, 83, [300, 2000, 5], [1, 16, 4], **shape)]
+    need = max(attention.tree_workspace_bytes(c.capacity, len(c.new), 8, 2, 64, c.max_len, c.max_new) for c in batches)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device=device)
+    for c in batches:
+        seen, mask = c.masks("tree")
+        _check(c, _run(c, mask=mask, workspace=ws), c.visible(seen))
+
+
+def test_gate_and_empty_batches(device):
+    c = Cache(device, 91, [30], [4], q_heads=4, kv_heads=2, head_dim=64, dtype=torch.bfloat16)
+    out = torch.full(c.q.shape, 7.0, dtype=torch.bfloat16, device=device)
+    closed = torch.tensor([1], dtype=torch.int32, device=device)
+    attention.tree_attention(c.q, c.k.to(device), c.v.to(device), c.qo, c.kv, c.indices, out, scale=0.125, max_len=34,
+                             max_new=4, status=closed)
+    assert (out == 7).all()
+    none = Cache(device, 92, [30, 0], [0, 0], q_heads=4, kv_heads=2, head_dim=64, dtype=torch.bfloat16, capacity=3)
+    out = _run(none, mask=None)
+    assert (out == 7).all()
+    assert attention.tree_attention(c.q[:0], c.k.to(device), c.v.to(device), c.qo[:1], c.kv[:1], c.indices, c.q[:0],
+                                    scale=0.125, max_len=0, max_new=0).numel() == 0
+
+
+def test_random_batches(device):
+    for seed in range(24):
+        rng = np.random.default_rng(1000 + seed)
+        b = int(rng.integers(1, 7))
+        hi = int(rng.choice([5, 70, 400, 1200]))
+        old, new = rng.integers(0, hi, b), rng.integers(0, int(rng.choice([2, 12, 70])), b)
+        new[0] = max(new[0], 1)
+        hk = int(rng.choice([1, 2, 3]))
+        hq = hk * int(rng.choice([1, 2, 5, 8]))
+        d = int(rng.choice([16, 64, 64, 72, 128]))
+        dtype = torch.bfloat16 if rng.random() < 0.6 else torch.float16
+        page = int(rng.choice([1, 1, 2, 16, 64]))
+        spread = float(rng.choice([1.0, 3.0]))
+        print(f"tree attention random {seed}: {old.tolist()} {new.tolist()} {hq}/{hk}x{d} page {page} {dtype}",
+              flush=True)
+        c = Cache(device, seed, old.tolist(), new.tolist(), q_heads=hq, kv_heads=hk, head_dim=d, dtype=dtype,
+                  page=page, holes=int(rng.integers(0, 3)), spread=spread, capacity=int(sum(new)) + int(rng.integers(0, 4)))
+        seen, mask = c.masks(str(rng.choice(["chain", "tree", "any"])))
+        starts = None
+        if rng.random() < 0.4:
+            starts = np.concatenate([rng.integers(0, o + 1, n) for o, n in zip(old, new)])
+        full = None if starts is None else np.concatenate((starts, np.zeros(c.capacity - c.total, np.int64)))
+        sinks = torch.randn(hq, generator=torch.Generator().manual_seed(seed)).to(device) if seed % 2 else None
+        _check(c, _run(c, mask=mask, starts=full, sinks=sinks), c.visible(seen, starts), sinks=sinks)
