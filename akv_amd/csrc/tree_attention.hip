@@ -12,15 +12,16 @@
 // outside the pool is a hole that no token sees.
 //
 // The n tokens x G heads of a KV head's group are the rows of one product with
-// that head's keys, so K and V are read once for R = 16 SUB rows, and again for
-// every further R.  Workgroup = (chunk of keys, KV head, request, block of R
-// rows) of four waves; all hold the same rows and take the keys in turn, KEYS
-// at a time: K straight into registers in the operand layout, V into the
-// wave's own LDS tile, both asked for one pass ahead.  No barrier until the
-// waves meet at the end.
-//   S^T[KEYS x 16 SUB] = K . Q^T            v_mfma_f32_16x16x32
+// that head's keys, so K and V are read once for a block of 64 SUB rows, and
+// again for every further one.  Workgroup = (chunk of keys, KV head, request,
+// block of rows), four waves, two workgroups per CU.  Tiles of K and V stream
+// into LDS (global_load_lds, two buffers) while the one before is worked on, in
+// 32-key quarters, 16 SUB rows per wave:
+//   S^T[32 x 16 SUB] = K . Q^T              v_mfma_f32_16x16x32
 //   P^T = 2^(scale log2(e) S^T - m)         in the storage type
 //   l += 1^T . P^T,  O^T[D x 16 SUB] += V^T . P^T
+// A block with at most half (a quarter of) its rows has two (four) waves share
+// each group of rows: they take the quarters in turn and meet at the end.
 // P^T leaves the first product in the operand layout of the second; V^T comes
 // through ds_read_b64_tr_b16.  m follows a row's maximum when that exceeds it
 // by more than 2^8.  A second launch merges the chunks and the sink.
@@ -52,9 +53,8 @@ constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;  // log2-domain excess at which a row's maximum moves
 
-// Keys of a wave's pass: 32 K registers and an 8 KiB V tile either way.
-constexpr int keys_of(int d) { return d == 64 ? 64 : 32; }
-constexpr int pass_of(int d) { return kWaves * keys_of(d); }
+// Keys of a tile: 32 KiB of K and V either way.
+constexpr int keys_of(int d) { return d == 64 ? 128 : 64; }
 
 struct TreeArgs {
   const void* q;
@@ -93,9 +93,9 @@ __device__ __forceinline__ int64_t chunk_keys_of(const TreeArgs& a, int64_t span
   const int64_t reach = a.max_len * a.n_requests;
   if (total > reach) total = reach;
   const int64_t work = total * a.kv_heads * a.row_blocks;
-  int64_t most = (work / kTargetGroups + pass_of(D) - 1) / pass_of(D) * pass_of(D);
+  int64_t most = (work / kTargetGroups + keys_of(D) - 1) / keys_of(D) * keys_of(D);
   const int64_t least = (span + a.chunks - 1) / a.chunks;
-  if (most < pass_of(D)) most = pass_of(D);
+  if (most < keys_of(D)) most = keys_of(D);
   if (most < least) most = (least + 63) / 64 * 64;
   const int64_t n = span > 0 ? (span + most - 1) / most : 1;
   return n > 1 ? ((span + n - 1) / n + 63) / 64 * 64 : most;
@@ -103,9 +103,21 @@ __device__ __forceinline__ int64_t chunk_keys_of(const TreeArgs& a, int64_t span
 
 static __device__ __attribute__((aligned(16))) const uint32_t zero_row[64] = {};
 
-// 16-byte chunk c of V row r sits at chunk c ^ swz(r) of its LDS row.
+// Chunk swizzles: 16-byte chunk c of row r lies at chunk c ^ swz(r).  K (16-byte
+// operand reads of 16 rows): distinct banks for the rows of a read.  V (8-byte
+// transposed reads): a row's chunk pair stays adjacent, distinct bank groups for
+// 8 consecutive rows.
 template <int D>
-__device__ __forceinline__ int swz(int r) { return D == 64 ? r & 6 : (r & 7) << 1; }
+__device__ __forceinline__ int swz_k(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
+template <int D>
+__device__ __forceinline__ int swz_v(int r) { return D == 64 ? r & 6 : (r & 7) << 1; }
+
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const uint32_t lo = uniform(static_cast<int32_t>(v)), hi = uniform(static_cast<int32_t>(v >> 32));
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
 
 template <typename T>
 struct Vec {
@@ -120,42 +132,119 @@ __device__ __forceinline__ f32x4 product(Vec<_Float16>::x8 a, Vec<_Float16>::x8 
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Whether any of the eight 16-bit values of a word is an infinity or NaN.
+// Whether the 16 bits are an infinity or NaN of type T.
 template <typename T>
-__device__ __forceinline__ bool not_finite(u32x4 w) {
-  constexpr uint32_t e = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
-  bool bad = false;
+__device__ __forceinline__ bool not_finite(short bits) {
+  constexpr short e = __is_same(T, __bf16) ? 0x7f80 : 0x7c00;
+  return (bits & e) == e;
+}
+
+// Four dims of a token's head, normalised; a weight sum of 0: nothing was seen.
+template <typename T>
+__device__ __forceinline__ void store_row(const TreeArgs& a, int64_t token, int head, int d, f32x4 o, float l) {
+  const int64_t at = token * a.o_st + head * a.o_sh + d;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= (w[i] & e) == e || (w[i] >> 16 & e) == e;
-  return bad;
+  for (int i = 0; i < 4; ++i) {
+    const float x = l == 0.f ? 0.f : o[i] / l;
+    if (a.out_f32)
+      static_cast<float*>(a.out)[at + i] = x;
+    else
+      static_cast<T*>(a.out)[at + i] = static_cast<T>(x);
+  }
+}
+
+// v_max3_f32 / v_max_f32 without the canonicalising moves around fmaxf of
+// matrix-core results; a NaN score still reaches the output through exp2.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
 }
 
 // Maximum over the lanes col, col + 16, col + 32, col + 48 of a column.
 __device__ __forceinline__ float column_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  const uint32_t b = __builtin_bit_cast(uint32_t, x);
+  const auto r16 = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  const uint32_t a0 = r16[0], a1 = r16[1];
+  x = max2(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+  const uint32_t c = __builtin_bit_cast(uint32_t, x);
+  const auto r32 = __builtin_amdgcn_permlane32_swap(c, c, false, false);
+  const uint32_t c0 = r32[0], c1 = r32[1];
+  return max2(__builtin_bit_cast(float, c0), __builtin_bit_cast(float, c1));
+}
+
+// Reads from a tile.  In asm, with their wait: the compiler takes every LDS read
+// for one that may meet the rows streaming into the other buffer, and would wait
+// for those first.
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)p));
+}
+
+// Two 16-byte chunks of the K row at either address, 16 rows apart by STRIDE.
+template <int STRIDE>
+__device__ __forceinline__ void read_k(uint32_t a0, uint32_t a1, u32x4 (&lo)[2], u32x4 (&hi)[2]) {
+  asm volatile(
+      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %4 offset:%6\n\tds_read_b128 %3, %5 offset:%6\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(hi[0]), "=&v"(hi[1])
+      : "v"(a0), "v"(a1), "i"(STRIDE)
+      : "memory");
+}
+
+// Four transposed operands: 4 x 16 dims of 32 keys.
+template <int STRIDE>
+__device__ __forceinline__ void read_v(const uint32_t (&at)[4], s16x4 (&lo)[4], s16x4 (&hi)[4]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "i"(STRIDE)
+      : "memory");
+}
+
+__device__ __forceinline__ u32x4 read_16(uint32_t at) {
+  u32x4 w;
+  asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(w) : "v"(at) : "memory");
+  return w;
 }
 
 template <int D>
-struct WaveTile {
-  char rows[kWaves][keys_of(D) * D * 2];
+struct TileLds {
+  char k[keys_of(D) * D * 2];  // key-major, 16-byte chunks swizzled per row (swz_k)
+  char v[keys_of(D) * D * 2];  // key-major, read transposed, swizzled (swz_v)
 };
 
-// D: 64 or 128, the tile's head width (head_dim <= D).  SUB: row subtiles of 16.
-template <typename T, int D, int SUB>
+// D: 64 or 128, the tile's head width; NARROW: head_dim is less.  SUB: a wave's
+// row subtiles of 16.
+template <typename T, int D, int SUB, bool NARROW>
 __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeArgs a) {
   using x4 = typename Vec<T>::x4;
   using x8 = typename Vec<T>::x8;
-  constexpr int kKeys = keys_of(D), kPass = pass_of(D);
-  constexpr int kTiles = kKeys / 16;
+  constexpr int kKeys = keys_of(D);
+  constexpr int kQuarters = kKeys / 32;
   constexpr int kSteps = D / 32;
   constexpr int kDTiles = D / 16;
-  constexpr int kChunks = D / 8;       // 16-byte chunks of a row
-  constexpr int kVRows = 64 / kChunks;  // V rows of one wave-wide load
-  constexpr int R = 16 * SUB;
-  __shared__ __attribute__((aligned(16))) WaveTile<D> tile0;
-  __shared__ float s_m[kWaves][16], s_l[kWaves][16];
-  static_assert(16 * D * 4 <= kKeys * D * 2, "a subtile's results fit a wave's tile");
+  constexpr int kChunks = D / 8;             // 16-byte chunks of a row
+  constexpr int kLoadRows = 64 / kChunks;    // rows of one wave-wide load
+  constexpr int kWaveKeys = kKeys / kWaves;  // keys of a tile that a wave asks for
+  constexpr int kGroupRows = 16 * SUB;       // rows of a wave
+  constexpr int R = kWaves * kGroupRows;     // rows of a block
+  __shared__ __attribute__((aligned(256))) TileLds<D> buffers[2];
+  __shared__ __attribute__((aligned(16))) uint32_t s_dead[2][4];  // keys of the buffers' quarters that no token sees
+  __shared__ float s_m[kWaves][kGroupRows], s_l[kWaves][kGroupRows];
+  __shared__ int32_t s_tok[kWaves][kGroupRows];  // the rows' tokens, for the masked quarters
+  __shared__ int32_t s_odd;                      // V rows held infinities or NaN that some row does not see
+  __shared__ uint64_t s_list[kWaves];            // and the keys that did
+  static_assert(kWaves * kGroupRows * D * 4 <= sizeof(buffers), "the waves' results fit the tiles");
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -169,10 +258,12 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
   if (pair >= static_cast<uint32_t>(a.n_requests) * a.kv_heads) return;
   const int b = a.heads_last ? pair % a.n_requests : pair / a.kv_heads;
   const int g = a.heads_last ? pair / a.n_requests : pair % a.kv_heads;
-  int64_t q0 = load_index(a.qo_indptr, a.indptr64, b), q1 = load_index(a.qo_indptr, a.indptr64, b + 1);
-  const int64_t kv0 = load_index(a.kv_indptr, a.indptr64, b);
-  int64_t len64 = load_index(a.kv_indptr, a.indptr64, b + 1) - kv0;
-  const int64_t total = load_index(a.kv_indptr, a.indptr64, a.n_requests) - load_index(a.kv_indptr, a.indptr64, 0);
+  // in scalar registers: the loop has no vector register to spare
+  int64_t q0 = uniform(load_index(a.qo_indptr, a.indptr64, b)), q1 = uniform(load_index(a.qo_indptr, a.indptr64, b + 1));
+  const int64_t kv0 = uniform(load_index(a.kv_indptr, a.indptr64, b));
+  const int64_t len64 = uniform(load_index(a.kv_indptr, a.indptr64, b + 1)) - kv0;
+  const int64_t total = uniform(load_index(a.kv_indptr, a.indptr64, a.n_requests)) -
+                        uniform(load_index(a.kv_indptr, a.indptr64, 0));
   if (gated(a.gate)) return;
   if (q0 < 0) q0 = 0;
   if (q1 > a.n_tokens) q1 = a.n_tokens;
@@ -195,64 +286,111 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
       lo = min(lo, __shfl_xor(lo, off));
       hi_start = max(hi_start, __shfl_xor(hi_start, off));
     }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    hi_start = __builtin_amdgcn_readfirstlane(hi_start);
+    lo = uniform(lo);
+    hi_start = uniform(hi_start);
   }
   const int span = len - lo;
-  const int64_t chunk_keys = chunk_keys_of<D>(a, span, total);
-  const int used = span > 0 ? static_cast<int>((span + chunk_keys - 1) / chunk_keys) : 1;
+  const int64_t chunk_keys = uniform(chunk_keys_of<D>(a, span, total));
+  const int used = span > 0 ? uniform(static_cast<int32_t>((span + chunk_keys - 1) / chunk_keys)) : 1;
   if (chunk >= used) return;
   const int begin = lo + static_cast<int>(chunk * chunk_keys);
   const int end = static_cast<int>(std::min<int64_t>(begin + chunk_keys, len));
+  const int tiles = (end - begin + kKeys - 1) / kKeys;
   if (chunk == 0 && g == 0 && rb0 == 0)
     for (int i = threadIdx.x; i < n; i += kThreads) a.used[q0 + i] = used;
 
-  const char* kbase = a.k + g * a.k_sh;
-  const char* vbase = a.v + g * a.v_sh;
+  // (an empty pool holds no key: every slot is a hole, and zeros are read)
+  const bool pool = a.pool_slots > 0;
+  const char* kbase = pool ? a.k + g * a.k_sh : reinterpret_cast<const char*>(zero_row);
+  const char* vbase = pool ? a.v + g * a.v_sh : reinterpret_cast<const char*>(zero_row);
+  const int64_t k_ss = pool ? a.k_ss : 0, v_ss = pool ? a.v_ss : 0;
   const int32_t* list = a.kv_indices + (a.paged ? b * a.table_stride : kv0);
   // entries of the list that exist
-  const int64_t width = a.paged ? a.table_width : a.table_width - kv0;
-  // the slot of key j, or -1: past the chunk, or a hole
-  auto slot_at = [&](int j) -> int64_t {
-    if (j >= end) return -1;
-    int64_t at = j, off = 0;
+  const int64_t left = a.paged ? a.table_width : a.table_width - kv0;
+  const int32_t width = static_cast<int32_t>(std::min<int64_t>(std::max<int64_t>(left, 0), 0x7fffffff));
+  const uint32_t dead_at = lds_address(s_dead), tile_at = lds_address(buffers);
+  const int my_key = kWaveKeys * wave + (lane & (kWaveKeys - 1));  // of a tile
+  // the list entry of this lane's key of tile it (past the end: the last key's),
+  // one tile ahead; what it means is worked out when the tile is asked for
+  auto fetch = [&](int it) -> int32_t {
+    const uint32_t j = min(begin + it * kKeys + my_key, end - 1);
+    const int32_t at = a.paged ? j / static_cast<uint32_t>(a.page_size) : j;
+    return width > 0 ? list[min(at, width - 1)] : -1;
+  };
+  // a wave's keys of a tile, straight into LDS: lane l of a load fills bytes
+  // 16 l of a 1 KiB block, chunk position l % kChunks of a row
+  auto stage = [&](int it, int32_t entry) {
+    TileLds<D>& t = buffers[it & 1];
+    const uint32_t key = begin + it * kKeys + my_key, j = min(key, static_cast<uint32_t>(end - 1));
+    uint32_t at = j, off = 0, per = 1;
     if (a.paged) {
-      const uint32_t page = a.page_size;
-      at = static_cast<uint32_t>(j) / page;
-      off = static_cast<uint32_t>(j) - static_cast<uint32_t>(at) * page;
+      per = a.page_size;
+      at = j / per;
+      off = j - at * per;
     }
-    if (at >= width) return -1;
-    const int64_t entry = list[at];
-    const int64_t slot = a.paged ? entry * a.page_size + off : entry;
-    return entry >= 0 && slot < a.pool_slots ? slot : -1;
+    const uint64_t slot64 = static_cast<uint64_t>(static_cast<uint32_t>(entry)) * per + off;
+    const bool there = entry >= 0 && at < static_cast<uint32_t>(width) && slot64 < static_cast<uint64_t>(a.pool_slots);
+    // a hole reads slot 0; the mask keeps it from every row
+    const uint32_t slot = there ? static_cast<uint32_t>(slot64) : 0;
+    const uint32_t dead = static_cast<uint32_t>(
+        __builtin_amdgcn_ballot_w64(!there || key >= static_cast<uint32_t>(end)));
+    if (lane == 0) {
+      if constexpr (kWaveKeys == 32)
+        asm volatile("ds_write_b32 %0, %1" ::"v"(dead_at + 16 * (it & 1) + 4 * wave), "v"(dead) : "memory");
+      else
+        asm volatile("ds_write_b16 %0, %1" ::"v"(dead_at + 16 * (it & 1) + 2 * wave), "v"(dead) : "memory");
+    }
+#pragma unroll
+    for (int u = 0; u < kWaveKeys / kLoadRows; ++u) {
+      const int mine = u * kLoadRows + lane / kChunks, r = kWaveKeys * wave + mine;
+      const uint64_t from = __shfl(slot, mine);
+      const int ck = (lane % kChunks) ^ swz_k<D>(r), cv = (lane % kChunks) ^ swz_v<D>(r);
+      const char* krow = kbase + from * k_ss + 16 * ck;
+      const char* vrow = vbase + from * v_ss + 16 * cv;
+      if (NARROW) {  // dims past head_dim read zeros
+        krow = 8 * ck < a.head_dim ? krow : reinterpret_cast<const char*>(zero_row);
+        vrow = 8 * cv < a.head_dim ? vrow : reinterpret_cast<const char*>(zero_row);
+      }
+      const int place = (kWaveKeys * wave + u * kLoadRows) * D * 2;
+      __builtin_amdgcn_global_load_lds(krow, (lds_void*)(t.k + place), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(vrow, (lds_void*)(t.v + place), 16, 0, 0);
+    }
   };
 
   for (int rb = rb0; rb * R < rows; rb += a.row_blocks) {
-    // this lane's rows: r = R rb + 16 s + col, token r / G, head g G + r % G
+    int32_t entry = tiles > 0 ? fetch(0) : -1;
+    if (threadIdx.x == 0) s_odd = 0;
+    // groups of rows, and the waves that share one
+    int groups = kWaves, sharers = 1;
+    while (groups > 1 && sharers < kQuarters && rows - rb * R <= (groups >> 1) * kGroupRows) {
+      groups >>= 1;
+      sharers <<= 1;
+    }
+    const int row0 = rb * R + (wave & (groups - 1)) * kGroupRows;
+    const int share = uniform(wave / groups);
+    // this lane's rows: r = row0 + 16 s + col, token r / G, head g G + r % G
     // (rows past the last repeat it and are never stored)
-    int tok[SUB];
     x8 qop[SUB][kSteps];
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-      const int r = min(rb * R + 16 * s + col, rows - 1);
-      tok[s] = r / a.group;
-      const T* row = static_cast<const T*>(a.q) + (q0 + tok[s]) * a.q_st +
-                     static_cast<int64_t>(g * a.group + r - tok[s] * a.group) * a.q_sh;
+      const int r = min(row0 + 16 * s + col, rows - 1);
+      const int tok = r / a.group;
+      s_tok[wave][16 * s + col] = tok;
+      const T* row = static_cast<const T*>(a.q) + (q0 + tok) * a.q_st +
+                     static_cast<int64_t>(g * a.group + r - tok * a.group) * a.q_sh;
 #pragma unroll
       for (int st = 0; st < kSteps; ++st) {
         u32x4 w = {0u, 0u, 0u, 0u};
         const int c = 4 * st + quad;
-        if (8 * c < a.head_dim) w = *((const global_u32x4*)row + c);
+        if (!NARROW || 8 * c < a.head_dim) w = *((const global_u32x4*)row + c);
         qop[s][st] = __builtin_bit_cast(x8, w);
       }
     }
-    f32x4 acc[SUB][kDTiles], lacc[SUB];
-    float neg_m[SUB];  // -m; 0 while the row has seen no finite score
-    bool seen[SUB];
+    f32x4 acc[SUB][kDTiles], lacc[SUB];  // l: four equal copies; 0 while the row has seen no key
+    float neg_m[SUB];
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
       neg_m[s] = 0.f;
-      seen[s] = false;
       lacc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int t = 0; t < kDTiles; ++t) acc[s][t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -261,40 +399,14 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = static_cast<T>(1.f);
 
-    u32x4 k[kTiles][kSteps];
-    uint64_t dead = 0;  // keys of the pass in k that no token sees
-    auto ask = [&](int64_t slot, WaveTile<D>& to) {
-      dead = __builtin_amdgcn_ballot_w64(slot < 0);
-#pragma unroll
-      for (int j = 0; j < kTiles; ++j) {
-        const int64_t at = __shfl(slot, 16 * j + col);
-        const char* row = at < 0 ? reinterpret_cast<const char*>(zero_row) : kbase + at * a.k_ss;
-#pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-          const int c = 4 * st + quad;
-          k[j][st] = u32x4{0u, 0u, 0u, 0u};
-          if (8 * c < a.head_dim) k[j][st] = *((const global_u32x4*)row + c);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kKeys / kVRows; ++u) {
-        const int r = u * kVRows + lane / kChunks;
-        int c = (lane % kChunks) ^ swz<D>(r);
-        // dims past head_dim are never stored: any finite or other value will do
-        if (8 * c >= a.head_dim) c = 0;
-        const int64_t at = __shfl(slot, r);
-        const char* row = at < 0 ? reinterpret_cast<const char*>(zero_row) : vbase + at * a.v_ss;
-        __builtin_amdgcn_global_load_lds(row + 16 * c, (lds_void*)(to.rows[wave] + u * kVRows * D * 2), 16, 0, 0);
-      }
-    };
-    // what row s sees of the 64 keys from t0 on, given the keys that are there
-    auto visible = [&](int s, int t0, uint64_t there) -> uint64_t {
-      const int base = t0 - old;
+    // what a token sees of the 32 keys from k0 on
+    auto visible = [&](int tok, int k0) -> uint32_t {
+      const int base = k0 - old;
       uint64_t bits = ~0ull;
-      if (base > -64) {
+      if (base > -32) {
         auto word = [&](int w) -> uint64_t {
-          if (a.mask) return w < a.mask_words ? a.mask[(q0 + tok[s]) * a.mask_stride + w] : 0;
-          const int i = tok[s] - 64 * w;
+          if (a.mask) return w < a.mask_words ? a.mask[(q0 + tok) * a.mask_stride + w] : 0;
+          const int i = tok - 64 * w;
           return i >= 63 ? ~0ull : i < 0 ? 0 : (2ull << i) - 1;
         };
         if (base < 0) {
@@ -302,189 +414,244 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
         } else {
           const int w = base >> 6, by = base & 63;
           bits = word(w) >> by;
-          if (by) bits |= word(w + 1) << (64 - by);
+          if (by > 32) bits |= word(w + 1) << (64 - by);
         }
       }
       if (a.key_starts) {
-        const int hidden = min(max(a.key_starts[q0 + tok[s]], 0), old) - t0;
-        if (hidden >= 64) bits = 0; else if (hidden > 0) bits &= ~0ull << hidden;
+        const int hidden = min(max(a.key_starts[q0 + tok], 0), old) - k0;
+        if (hidden >= 32) bits = 0; else if (hidden > 0) bits &= ~0ull << hidden;
       }
-      return bits & there;
+      return static_cast<uint32_t>(bits);
     };
-    auto step = [&](int t0, WaveTile<D>& cur) {
-      T* vt = reinterpret_cast<T*>(cur.rows[wave]);
-      const bool masked = dead != 0 || t0 + kKeys > old || t0 < hi_start;
-      uint64_t seen_bits[SUB];
-      x8 p[SUB][kTiles / 2];
+    // A weight of 0 does not hide an infinity or NaN from the product.  Where
+    // rows see different keys such values are cleared (by every wave that uses
+    // them) and the block takes note: its rows get them back at the end.
+    auto clear_odd = [&](uint32_t at, uint32_t dead) {
+      bool noted = false;
+#pragma nounroll
+      for (int i = 0; i < kDTiles; ++i) {
+        const uint32_t here = at + 1024 * i + 16 * lane;
+        s16x8 w = __builtin_bit_cast(s16x8, read_16(here));
+        bool odd = false;
 #pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-        f32x4 sc[kTiles];
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) {
-          sc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int st = 0; st < kSteps; ++st) sc[j] = product(__builtin_bit_cast(x8, k[j][st]), qop[s][st], sc[j]);
+        for (int e = 0; e < 8; ++e) {
+          const bool one = not_finite<T>(w[e]);
+          odd |= one;
+          w[e] = one ? 0 : w[e];
         }
-        if (masked) {
-          seen_bits[s] = visible(s, t0, ~dead);
+        if (odd) asm volatile("ds_write_b128 %0, %1" ::"v"(here), "v"(w) : "memory");
+        noted |= odd && !(dead >> ((64 * i + lane) / kChunks) & 1);
+      }
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): cleared before they are read
+      if (__builtin_amdgcn_ballot_w64(noted) && lane == 0)
+        asm volatile("ds_write_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" ::"v"(lds_address(&s_odd)), "v"(1) : "memory");
+    };
+    // this lane's operand addresses in quarter 0: K chunks quad of row col, and
+    // the source of its transposed V reads (row 4 quad + col / 4, dims 4 (col % 4))
+    const uint32_t k_at = col * D * 2 + 16 * (quad ^ swz_k<D>(col));
+    const int vr = 4 * quad + (col >> 2);
+    const uint32_t v_at = kKeys * D * 2 + vr * D * 2 + 16 * ((col >> 1 & 1) ^ swz_v<D>(vr)) + 8 * (col & 1);
+    // 32 keys, from row 32 kk of a tile on; k0: the first one's rank
+    auto quarter = [&](uint32_t at, int k0, uint32_t dead) {
+      const bool masked = dead != 0 || k0 + 32 > old || k0 < hi_start;
+      f32x4 sc[2][SUB];
 #pragma unroll
-          for (int j = 0; j < kTiles; ++j)
+      for (int h = 0; h < kSteps / 2; ++h) {
+        // k-steps 2 h and 2 h + 1: chunks 4 and 8 on (the swizzle is an xor)
+        u32x4 lo[2], hi[2];
+        read_k<16 * D * 2>((at + k_at) ^ (128 * h), (at + k_at) ^ (128 * h + 64), lo, hi);
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+          for (int s = 0; s < SUB; ++s) {
+            sc[0][s] = product(__builtin_bit_cast(x8, lo[st]), qop[s][2 * h + st],
+                               h + st == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[0][s]);
+            sc[1][s] = product(__builtin_bit_cast(x8, hi[st]), qop[s][2 * h + st],
+                               h + st == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[1][s]);
+          }
+      }
+      if (masked) {
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+          const uint32_t seen = visible(s_tok[wave][16 * s + col], k0) & ~dead;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              sc[j][i] = seen_bits[s] >> (16 * j + 4 * quad + i) & 1 ? sc[j][i] : -INFINITY;
+              sc[j][s][i] = seen >> (16 * j + 4 * quad + i) & 1 ? sc[j][s][i] : -INFINITY;
         }
-        float top = -INFINITY;
+      }
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[j][i]);
-        top = column_max(top);
-        const float over = fmaf(top, a.scale_log2, neg_m[s]);  // above m
-        const bool move = seen[s] ? over > kSlack : top > -INFINITY;
+      for (int s = 0; s < SUB; ++s) {
+        const float m0 = max3(sc[0][s][0], sc[0][s][1], sc[0][s][2]);
+        const float m1 = max3(sc[0][s][3], sc[1][s][0], sc[1][s][1]);
+        const float mx = column_max(max3(m0, m1, max2(sc[1][s][2], sc[1][s][3])));
+        const float over = fmaf(mx, a.scale_log2, neg_m[s]);  // above m
+        const bool any = lacc[s][0] != 0.f;
+        const bool move = any ? over > kSlack : mx > -INFINITY;
         if (__builtin_amdgcn_ballot_w64(move)) {
-          const float alpha = move && seen[s] ? __builtin_amdgcn_exp2f(-over) : 1.f;
+          const float alpha = move && any ? __builtin_amdgcn_exp2f(-over) : 1.f;
           lacc[s] *= alpha;
 #pragma unroll
-          for (int t = 0; t < kDTiles; ++t) acc[s][t] *= alpha;
-          neg_m[s] = move ? -(top * a.scale_log2) : neg_m[s];
-          seen[s] |= move;
-        }
-#pragma unroll
-        for (int jj = 0; jj < kTiles / 2; ++jj) {
-          f32x4 e0, e1;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            e0[i] = __builtin_amdgcn_exp2f(fmaf(sc[2 * jj][i], a.scale_log2, neg_m[s]));
-            e1[i] = __builtin_amdgcn_exp2f(fmaf(sc[2 * jj + 1][i], a.scale_log2, neg_m[s]));
-          }
-          const x4 p0 = __builtin_convertvector(e0, x4), p1 = __builtin_convertvector(e1, x4);
-          p[s][jj] = __builtin_shufflevector(p0, p1, 0, 1, 2, 3, 4, 5, 6, 7);
-          lacc[s] = product(ones, p[s][jj], lacc[s]);
+          for (int dt = 0; dt < kDTiles; ++dt) acc[s][dt] *= alpha;
+          neg_m[s] = move ? -(mx * a.scale_log2) : neg_m[s];
         }
       }
-      // transposing read: lane col of group quad receives V[key][16 t + col]
-      // for keys 32 jj + 4 quad + i (i < 4), then 16 keys on
-      auto v_operand = [&](int jj, int t) -> x8 {
-        const int r0 = 32 * jj + 4 * quad + (col >> 2), r1 = r0 + 16;
-        const int c = 2 * t + ((col & 3) >> 1), h = 4 * (col & 1);
-        const s16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vt + r0 * D + 8 * (c ^ swz<D>(r0)) + h));
-        const s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vt + r1 * D + 8 * (c ^ swz<D>(r1)) + h));
-        return __builtin_bit_cast(x8, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
-      };
-      if (masked) {
-        // A weight of 0 does not hide an infinity or NaN: such V rows are added
-        // key by key to the rows that see them, and cleared for the product.
-        constexpr int kShare = 64 / kKeys;  // lanes per key
-        const int key = lane / kShare;
-        lds_u32x4* row = (lds_u32x4*)(vt + key * D);
-        bool bad = false;
+      x8 p[SUB];
 #pragma unroll
-        for (int c = 0; c < kChunks / kShare; ++c) {
-          const int cc = c + lane % kShare * (kChunks / kShare);
-          if (8 * cc < a.head_dim) bad |= not_finite<T>(row[cc ^ swz<D>(key)]);
-        }
-        if (kShare == 2) bad |= __shfl_xor(static_cast<int>(bad), 1) != 0;
-        for (uint64_t rest = __builtin_amdgcn_ballot_w64(bad); rest;) {
-          const int kk = __builtin_ctzll(rest) / kShare;
-          rest &= ~(((1ull << kShare) - 1) << (kk * kShare));
-          const int jj = kk >> 5, mine = kk & 31;
-#pragma unroll
-          for (int t = 0; t < kDTiles; ++t) {
-            x8 v1 = v_operand(jj, t);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (4 * quad + (i & 3) + 16 * (i >> 2) != mine) v1[i] = static_cast<T>(0.f);
-#pragma unroll
-            for (int s = 0; s < SUB; ++s) {
-              const x8 pj = kTiles == 4 && jj ? p[s][kTiles / 2 - 1] : p[s][0];
-              const f32x4 add = product(v1, pj, f32x4{0.f, 0.f, 0.f, 0.f});
-              if (seen_bits[s] >> kk & 1) acc[s][t] += add;
-            }
-          }
-        }
-        if (bad) {
-#pragma unroll
-          for (int c = 0; c < kChunks / kShare; ++c)
-            row[(c + lane % kShare * (kChunks / kShare)) ^ swz<D>(key)] = u32x4{0u, 0u, 0u, 0u};
-        }
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // the clears are in LDS before the reads below
-        asm volatile("" ::: "memory");
-      }
-#pragma unroll
-      for (int jj = 0; jj < kTiles / 2; ++jj)
-#pragma unroll
-        for (int t = 0; t < kDTiles; ++t) {
-          const x8 vop = v_operand(jj, t);
-#pragma unroll
-          for (int s = 0; s < SUB; ++s) acc[s][t] = product(vop, p[s][jj], acc[s][t]);
-        }
-      // this tile's reads are done before its place is filled again
-      __builtin_amdgcn_s_waitcnt(0xc07f);
-      asm volatile("" ::: "memory");
-    };
-    for (int t0 = begin + wave * kKeys; t0 < end; t0 += kPass) {
-      ask(slot_at(t0 + lane % kKeys), tile0);
-      __builtin_amdgcn_s_waitcnt(0);
-      asm volatile("" ::: "memory");
-      step(t0, tile0);
-    }
-
-    // the waves meet, 16 rows at a time: O rows [row][dim] over their V tiles,
-    // four-float groups turned by the row for the banks
-    float* om = reinterpret_cast<float*>(tile0.rows[wave]);
-#pragma unroll
-    for (int s = 0; s < SUB; ++s) {
-      __syncthreads();
-#pragma unroll
-      for (int t = 0; t < kDTiles; ++t)
-        *reinterpret_cast<f32x4*>(om + col * D + ((16 * t + 4 * quad) ^ (col & 7) << 2)) = acc[s][t];
-      if (quad == 0) {
-        s_m[wave][col] = seen[s] ? -neg_m[s] : -INFINITY;
-        s_l[wave][col] = lacc[s][0];
-      }
-      __syncthreads();
-      for (int u = threadIdx.x; u < 16 * (D / 4); u += kThreads) {
-        const int row = u / (D / 4), d = 4 * (u % (D / 4));
-        const int r = rb * R + 16 * s + row;
-        if (r >= rows || d >= a.head_dim) continue;
-        const int token = r / a.group, head = g * a.group + r - token * a.group;
-        float m = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, s_m[w][row]);
-        // a wave without a finite score carries m = -inf, and O = l = 0 or NaN
-        const float base = m == -INFINITY ? 0.f : m;
-        float l = 0.f;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          const float mw = s_m[w][row];
-          const float sw = mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - base);
-          l += s_l[w][row] * sw;
-          o += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(tile0.rows[w]) + row * D +
-                                               (d ^ (row & 7) << 2)) * sw;
-        }
-        if (used > 1) {
-          const int64_t at = (static_cast<int64_t>(chunk) * a.n_tokens + q0 + token) * a.q_heads + head;
-          *reinterpret_cast<f32x4*>(a.part_o + at * D + d) = o;
-          if (d == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{m, l};
-          continue;
-        }
-        if (a.sinks) {
-          const float sink = a.sinks[head] * kLog2e;
-          const float mt = fmaxf(m, sink);
-          const float by = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mt);
-          o *= by;
-          l = l * by + (mt == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - mt));
-        }
-        const int64_t at = (q0 + token) * a.o_st + head * a.o_sh + d;
+      for (int s = 0; s < SUB; ++s) {
+        f32x4 e0, e1;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float x = l == 0.f ? 0.f : o[i] / l;
-          if (a.out_f32)
-            static_cast<float*>(a.out)[at + i] = x;
-          else
-            static_cast<T*>(a.out)[at + i] = static_cast<T>(x);
+          e0[i] = __builtin_amdgcn_exp2f(fmaf(sc[0][s][i], a.scale_log2, neg_m[s]));
+          e1[i] = __builtin_amdgcn_exp2f(fmaf(sc[1][s][i], a.scale_log2, neg_m[s]));
         }
+        p[s] = __builtin_shufflevector(__builtin_convertvector(e0, x4), __builtin_convertvector(e1, x4), 0, 1, 2, 3, 4,
+                                       5, 6, 7);
+        lacc[s] = product(ones, p[s], lacc[s]);
+      }
+      // transposing reads: lane col of group quad receives V[key][16 dt + col]
+      // for keys 4 quad + i (i < 4) of the quarter, then 16 keys on; dt = 4 h + e
+      auto v_operands = [&](int h, x8 (&v)[4]) {
+        uint32_t from[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) from[e] = (at + v_at) ^ (32 * (4 * h + e));
+        s16x4 lo[4], hi[4];
+        read_v<16 * D * 2>(from, lo, hi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = __builtin_bit_cast(x8, __builtin_shufflevector(lo[e], hi[e], 0, 1, 2, 3, 4, 5, 6, 7));
+      };
+      if (masked) clear_odd(at + kKeys * D * 2, dead);
+#pragma unroll
+      for (int h = 0; h < kDTiles / 4; ++h) {
+        x8 v[4];
+        v_operands(h, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int s = 0; s < SUB; ++s) acc[s][4 * h + e] = product(v[e], p[s], acc[s][4 * h + e]);
+      }
+    };
+    if (tiles > 0) {
+      stage(0, entry);
+      if (tiles > 1) entry = fetch(1);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    // tile it from one buffer while tile it + 1 streams into the other
+#pragma nounroll
+    for (int it = 0; it < tiles; ++it) {
+      const int buf = it & 1;
+      if (it + 1 < tiles) {
+        stage(it + 1, entry);
+        if (it + 2 < tiles) entry = fetch(it + 2);
+      }
+      const int t0 = begin + it * kKeys;
+      const uint32_t cur = tile_at + buf * static_cast<uint32_t>(sizeof(TileLds<D>));
+      const u32x4 dead = read_16(dead_at + 16 * buf);
+#pragma nounroll
+      for (int kk = share; kk < kQuarters; kk += sharers) {
+        const int k0 = t0 + 32 * kk;
+        if (k0 >= end) break;
+        const uint32_t word = kk == 0 ? dead[0] : kk == 1 ? dead[1] : kk == 2 ? dead[2] : dead[3];
+        quarter(cur + kk * 64 * D, k0, __builtin_amdgcn_readfirstlane(word));
+      }
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+    }
+
+    // the waves' O rows [row][dim] over the tiles, four-float groups turned by
+    // the row for the banks; the sharers of a group meet there
+    auto result_of = [&](int w) -> float* {
+      return reinterpret_cast<float*>(&buffers[0]) + w * kGroupRows * D;
+    };
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      const int r = 16 * s + col;
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt)
+        *reinterpret_cast<f32x4*>(result_of(wave) + r * D + ((16 * dt + 4 * quad) ^ (col & 7) << 2)) = acc[s][dt];
+      if (quad == 0) {
+        s_m[wave][r] = lacc[s][0] == 0.f ? -INFINITY : -neg_m[s];
+        s_l[wave][r] = lacc[s][0];
+      }
+    }
+    __syncthreads();
+    const int here = min(rows - rb * R, groups * kGroupRows);
+    for (int u = threadIdx.x; u < here * (D / 4); u += kThreads) {
+      const int r = u / (D / 4), d = 4 * (u % (D / 4));
+      if (NARROW && d >= a.head_dim) continue;
+      const int token = (rb * R + r) / a.group, head = g * a.group + rb * R + r - token * a.group;
+      const int group = r / kGroupRows, in = r % kGroupRows;
+      float m = -INFINITY, l = 0.f;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      for (int w = group; w < kWaves; w += groups) m = fmaxf(m, s_m[w][in]);
+      // a wave that has seen no key carries m = -inf, l = 0 and O = 0
+      const float base = m == -INFINITY ? 0.f : m;
+      for (int w = group; w < kWaves; w += groups) {
+        const float by = __builtin_amdgcn_exp2f(s_m[w][in] - base);
+        l += s_l[w][in] * by;
+        o += *reinterpret_cast<const f32x4*>(result_of(w) + in * D + (d ^ (in & 7) << 2)) * by;
+      }
+      if (used > 1) {
+        const int64_t at = (static_cast<int64_t>(chunk) * a.n_tokens + q0 + token) * a.q_heads + head;
+        *reinterpret_cast<f32x4*>(a.part_o + at * D + d) = o;
+        if (d == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{m, l};
+        continue;
+      }
+      if (a.sinks) {
+        const float sink = a.sinks[head] * kLog2e;
+        const float mt = fmaxf(m, sink);
+        const float by = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mt);
+        o *= by;
+        l = l * by + (mt == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - mt));
+      }
+      store_row<T>(a, q0 + token, head, d, o, l);
+    }
+    // values cleared from the products go back, unweighted, to the rows that see
+    // them: whatever their weights, the results are the infinity or NaN
+    if (s_odd) {
+      for (int base = begin; base < end; base += kThreads) {
+        auto v_row = [&](int j) -> const T* {
+          const uint32_t per = a.paged ? a.page_size : 1, at = static_cast<uint32_t>(j) / per;
+          if (static_cast<int64_t>(at) >= width || list[at] < 0) return nullptr;
+          const uint64_t slot = static_cast<uint64_t>(list[at]) * per + (static_cast<uint32_t>(j) - at * per);
+          return slot < static_cast<uint64_t>(a.pool_slots) ? reinterpret_cast<const T*>(vbase + slot * v_ss) : nullptr;
+        };
+        const int mine = base + static_cast<int>(threadIdx.x);
+        const T* row = mine < end ? v_row(mine) : nullptr;
+        bool odd = false;
+        for (int d = 0; row && d < a.head_dim; ++d) odd |= not_finite<T>(__builtin_bit_cast(short, row[d]));
+        const uint64_t odds = __builtin_amdgcn_ballot_w64(odd);
+        if (lane == 0) s_list[wave] = odds;
+        __syncthreads();
+        for (int u = threadIdx.x; u < here * (D / 4); u += kThreads) {
+          const int r = rb * R + u / (D / 4), d = 4 * (u % (D / 4));
+          const int token = r / a.group, head = g * a.group + r - token * a.group;
+          if (NARROW && d >= a.head_dim) continue;
+          for (int w = 0; w < kWaves; ++w)
+            for (uint64_t rest = s_list[w]; rest; rest &= rest - 1) {
+              const int j = base + 64 * w + __builtin_ctzll(rest);
+              if (!(visible(token, j) & 1)) continue;
+              const T* v = v_row(j) + d;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (!not_finite<T>(__builtin_bit_cast(short, v[i]))) continue;
+                const float x = static_cast<float>(v[i]);
+                if (used > 1) {
+                  a.part_o[((static_cast<int64_t>(chunk) * a.n_tokens + q0 + token) * a.q_heads + head) * D + d + i] += x;
+                  continue;
+                }
+                const int64_t at = (q0 + token) * a.o_st + head * a.o_sh + d + i;
+                if (a.out_f32)
+                  static_cast<float*>(a.out)[at] += x;
+                else
+                  static_cast<T*>(a.out)[at] = static_cast<T>(static_cast<float>(static_cast<T*>(a.out)[at]) + x);
+              }
+            }
+        }
+        __syncthreads();
       }
     }
     __syncthreads();
@@ -517,24 +684,17 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a) {
     const int64_t at = c * step + row;
     const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * at);
     const f32x4 oc = *reinterpret_cast<const f32x4*>(a.part_o + at * D + d);
-    const float w = ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - base);
+    const float w = __builtin_amdgcn_exp2f(ml.x - base);
     l += ml.y * w;
     o += oc * w;
   }
-  const int64_t at = token * a.o_st + head * a.o_sh + d;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float x = l == 0.f ? 0.f : o[i] / l;
-    if (a.out_f32)
-      static_cast<float*>(a.out)[at + i] = x;
-    else
-      static_cast<T*>(a.out)[at + i] = static_cast<T>(x);
-  }
+  store_row<T>(a, token, head, d, o, l);
 }
 
 int tile_dim(int32_t head_dim) { return head_dim <= 64 ? 64 : 128; }
 
-// Row subtiles of a workgroup for requests of up to `rows` rows.
+// A wave's row subtiles for requests of up to `rows` rows: as many as the rows
+// fill, since waves that share rows read every key once.
 int subtiles_for(int d, int64_t rows) {
   const int most = d == 64 ? 4 : 2;
   int sub = 1;
@@ -553,7 +713,7 @@ Launch plan(int64_t n_tokens, int64_t n_requests, int64_t kv_heads, int64_t grou
   p.d = tile_dim(head_dim);
   const int64_t rows = std::max<int64_t>(1, std::min(max_new, n_tokens)) * group;
   p.sub = subtiles_for(p.d, rows);
-  const int64_t block = 16 * p.sub, pass = pass_of(p.d);
+  const int64_t block = 16 * kWaves * p.sub, pass = keys_of(p.d);
   p.row_blocks = static_cast<int32_t>(std::min<int64_t>((rows + block - 1) / block, 4096));
   // chunks: as many as give every CU its share of a batch whose requests all
   // have max_len keys, four times as many for a few long ones among short ones
@@ -572,7 +732,10 @@ int64_t partial_bytes(const Launch& p, int64_t n_tokens, int64_t q_heads) {
 
 template <typename T, int D, int SUB>
 void start(const TreeArgs& a, dim3 grid, hipStream_t st) {
-  hipLaunchKernelGGL((tree_attention_kernel<T, D, SUB>), grid, dim3(kThreads), 0, st, a);
+  if (a.head_dim < D)
+    hipLaunchKernelGGL((tree_attention_kernel<T, D, SUB, true>), grid, dim3(kThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((tree_attention_kernel<T, D, SUB, false>), grid, dim3(kThreads), 0, st, a);
 }
 
 template <typename T>
@@ -653,7 +816,7 @@ extern "C" int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_s
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_buffer) |
         reinterpret_cast<uintptr_t>(v_buffer) | reinterpret_cast<uintptr_t>(workspace)) & 15) != 0)
     return fail(AKV_EINVAL, "akv_tree_attention: q, K and V rows and the workspace must be 16-byte aligned");
-  if (n_tokens > 0x7fffffffLL / q_heads || static_cast<int64_t>(n_requests) * kv_heads > 0x7fffffffLL / 4096)
+  if (pool_slots > 0xffffffffLL || n_tokens > 0x7fffffffLL / q_heads || static_cast<int64_t>(n_requests) * kv_heads > 0x7fffffffLL / 4096)
     return fail(AKV_EINVAL, "akv_tree_attention: batch too large");
   const Launch p = plan(n_tokens, n_requests, kv_heads, q_heads / kv_heads, head_dim, max_len, max_new);
   const int64_t need = partial_bytes(p, n_tokens, q_heads);
