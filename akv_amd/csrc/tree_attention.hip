@@ -23,8 +23,8 @@
 // A block with at most half (a quarter of) its rows has two (four) waves share
 // each group of rows: they take the quarters in turn and meet at the end.
 // P^T leaves the first product in the operand layout of the second; V^T comes
-// through ds_read_b64_tr_b16.  m follows a row's maximum when that exceeds it
-// by more than 2^8.  A second launch merges the chunks and the sink.
+// through ds_read_b64_tr_b16.  m is a row's first maximum and moves only when the
+// weights outgrow their types.  A second launch merges the chunks and the sink.
 //
 // Lane layouts (verified on gfx950): v_mfma_f32_16x16x32 -- lane l supplies
 // A[l%16][k(l,i)], B[k(l,i)][l%16] for i < 8 and holds D[4(l/16)+i][l%16];
@@ -51,7 +51,7 @@ typedef __attribute__((address_space(3))) void lds_void;
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.f;  // log2-domain excess at which a row's maximum moves
+constexpr float kHuge = 18446744073709551616.f;  // 2^64: a weight sum above it may have overflowed the product
 
 // Keys of a tile: 32 KiB of K and V either way.
 constexpr int keys_of(int d) { return d == 64 ? 128 : 64; }
@@ -395,6 +395,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
 #pragma unroll
       for (int t = 0; t < kDTiles; ++t) acc[s][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    bool unset = true;  // some row of the wave has seen no key yet
     x8 ones;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = static_cast<T>(1.f);
@@ -481,34 +482,54 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
               sc[j][s][i] = seen >> (16 * j + 4 * quad + i) & 1 ? sc[j][s][i] : -INFINITY;
         }
       }
-#pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-        const float m0 = max3(sc[0][s][0], sc[0][s][1], sc[0][s][2]);
-        const float m1 = max3(sc[0][s][3], sc[1][s][0], sc[1][s][1]);
-        const float mx = column_max(max3(m0, m1, max2(sc[1][s][2], sc[1][s][3])));
-        const float over = fmaf(mx, a.scale_log2, neg_m[s]);  // above m
-        const bool any = lacc[s][0] != 0.f;
-        const bool move = any ? over > kSlack : mx > -INFINITY;
-        if (__builtin_amdgcn_ballot_w64(move)) {
-          const float alpha = move && any ? __builtin_amdgcn_exp2f(-over) : 1.f;
-          lacc[s] *= alpha;
-#pragma unroll
-          for (int dt = 0; dt < kDTiles; ++dt) acc[s][dt] *= alpha;
-          neg_m[s] = move ? -(mx * a.scale_log2) : neg_m[s];
-        }
-      }
+      // A row's m is its maximum over the first quarter it sees a key of, and then
+      // stays put: the sum tells when it should not have.  A sum past kHuge (a
+      // score ~64 above m in the log2 domain, 16 in fp16, whose weight is then
+      // infinite) takes the quarter again with exact maxima.
       x8 p[SUB];
+      float before[SUB];
 #pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-        f32x4 e0, e1;
+      for (int s = 0; s < SUB; ++s) before[s] = lacc[s][0];
+      for (bool exact = unset;; exact = true) {
+        if (exact) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e0[i] = __builtin_amdgcn_exp2f(fmaf(sc[0][s][i], a.scale_log2, neg_m[s]));
-          e1[i] = __builtin_amdgcn_exp2f(fmaf(sc[1][s][i], a.scale_log2, neg_m[s]));
+          for (int s = 0; s < SUB; ++s) {
+            const float m0 = max3(sc[0][s][0], sc[0][s][1], sc[0][s][2]);
+            const float m1 = max3(sc[0][s][3], sc[1][s][0], sc[1][s][1]);
+            const float mx = column_max(max3(m0, m1, max2(sc[1][s][2], sc[1][s][3])));
+            const float over = fmaf(mx, a.scale_log2, neg_m[s]);  // above m
+            const bool any = before[s] != 0.f;
+            const bool move = any ? over > 0.f : mx > -INFINITY;
+            const float alpha = move && any ? __builtin_amdgcn_exp2f(-over) : 1.f;
+            before[s] *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < kDTiles; ++dt) acc[s][dt] *= alpha;
+            neg_m[s] = move ? -(mx * a.scale_log2) : neg_m[s];
+            lacc[s] = f32x4{before[s], before[s], before[s], before[s]};
+          }
         }
-        p[s] = __builtin_shufflevector(__builtin_convertvector(e0, x4), __builtin_convertvector(e1, x4), 0, 1, 2, 3, 4,
-                                       5, 6, 7);
-        lacc[s] = product(ones, p[s], lacc[s]);
+        bool huge = false;
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+          f32x4 e0, e1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            e0[i] = __builtin_amdgcn_exp2f(fmaf(sc[0][s][i], a.scale_log2, neg_m[s]));
+            e1[i] = __builtin_amdgcn_exp2f(fmaf(sc[1][s][i], a.scale_log2, neg_m[s]));
+          }
+          p[s] = __builtin_shufflevector(__builtin_convertvector(e0, x4), __builtin_convertvector(e1, x4), 0, 1, 2, 3,
+                                         4, 5, 6, 7);
+          lacc[s] = product(ones, p[s], lacc[s]);
+        }
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) huge |= lacc[s][0] > kHuge;
+        if (exact || !__builtin_amdgcn_ballot_w64(huge)) break;
+      }
+      if (unset) {
+        bool none = false;
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) none |= lacc[s][0] == 0.f;
+        unset = __builtin_amdgcn_ballot_w64(none) != 0;
       }
       // transposing reads: lane col of group quad receives V[key][16 dt + col]
       // for keys 4 quad + i (i < 4) of the quarter, then 16 keys on; dt = 4 h + e
@@ -658,37 +679,63 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
   }
 }
 
-// Merges a row's chunks and the sink: D / 4 lanes per (token, head).
+// Merges a row's chunks and the sink: a wave per (token, head).  Lane c takes
+// chunk c's maximum and sum; then D / 4 lanes each take the chunks in turn, four
+// dims a lane.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a) {
-  constexpr int kLanes = D / 4;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
-  const int d = 4 * (threadIdx.x % kLanes);
+  constexpr int kLanes = D / 4, kWays = 64 / kLanes, kAhead = 4;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + uniform(static_cast<int32_t>(threadIdx.x >> 6));
   const int64_t token = row / a.q_heads;
   const int head = static_cast<int>(row - token * a.q_heads);
   if (token >= a.n_tokens || token >= load_index(a.qo_indptr, a.indptr64, a.n_requests) ||
-      token < load_index(a.qo_indptr, a.indptr64, 0) || d >= a.head_dim)
+      token < load_index(a.qo_indptr, a.indptr64, 0))
     return;
   if (gated(a.gate)) return;
-  const int used = a.used[token];
+  const int used = uniform(a.used[token]);
   if (used <= 1) return;
   const int64_t step = a.n_tokens * a.q_heads;
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + row;
+  const int d = 4 * (lane % kLanes), way = lane / kLanes;
+  const float* from = a.part_o + row * D + d;
   const float sink = a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
   float m = sink;
-  for (int c = 0; c < used; ++c) m = fmaxf(m, a.part_ml[2 * (c * step + row)]);
+  for (int c = lane; c < used; c += 64) m = fmaxf(m, ml[c * step].x);
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
   const float base = m == -INFINITY ? 0.f : m;
-  float l = a.sinks && m != -INFINITY ? __builtin_amdgcn_exp2f(sink - base) : 0.f;
+  float l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int c = 0; c < used; ++c) {
-    const int64_t at = c * step + row;
-    const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * at);
-    const f32x4 oc = *reinterpret_cast<const f32x4*>(a.part_o + at * D + d);
-    const float w = __builtin_amdgcn_exp2f(ml.x - base);
-    l += ml.y * w;
-    o += oc * w;
+  for (int c0 = 0; c0 < used; c0 += 64) {
+    f32x2 mine = {-INFINITY, 0.f};
+    if (c0 + lane < used) mine = ml[(c0 + lane) * step];
+    const float w = __builtin_amdgcn_exp2f(mine.x - base);
+    l += mine.y * w;
+    const int count = used - c0 < 64 ? used - c0 : 64;
+    for (int c = 0; c < count; c += kWays * kAhead) {
+      f32x4 x[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int at = c + i * kWays + way;
+        x[i] = *reinterpret_cast<const f32x4*>(from + (c0 + (at < count ? at : 0)) * step * D);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int at = c + i * kWays + way;
+        const float by = __shfl(w, at & 63);
+        if (at < count) o += x[i] * by;
+      }
+    }
   }
-  store_row<T>(a, token, head, d, o, l);
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) l += __shfl_xor(l, off);
+#pragma unroll
+  for (int off = kLanes; off < 64; off <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], off);
+  if (a.sinks && m != -INFINITY) l += __builtin_amdgcn_exp2f(sink - base);
+  if (way == 0 && d < a.head_dim) store_row<T>(a, token, head, d, o, l);
 }
 
 int tile_dim(int32_t head_dim) { return head_dim <= 64 ? 64 : 128; }
@@ -754,8 +801,7 @@ int launch(const TreeArgs& a, const Launch& p, hipStream_t st) {
   }
   int rc = check_launch("akv_tree_attention");
   if (rc || a.chunks == 1) return rc;
-  const int64_t rows = a.n_tokens * a.q_heads, per = 256 / (p.d / 4);
-  const dim3 merge(static_cast<unsigned>((rows + per - 1) / per));
+  const dim3 merge(static_cast<unsigned>((a.n_tokens * a.q_heads + 3) / 4));
   if (p.d == 64)
     hipLaunchKernelGGL((tree_combine_kernel<T, 64>), merge, dim3(256), 0, st, a);
   else
