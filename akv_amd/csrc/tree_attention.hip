@@ -45,16 +45,21 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(1))) u32x4 global_u32x4;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHuge = 18446744073709551616.f;  // 2^64: a weight sum above it may have overflowed the product
 
-// Keys of a tile: 32 KiB of K and V either way.
-constexpr int keys_of(int d) { return d == 64 ? 128 : 64; }
+// Keys of a tile and the tiles in LDS: one is worked on while the next stream in.
+constexpr int keys_of(int d) { return d == 64 ? 64 : 32; }
+constexpr int kBuffers = 4;
+
+// Workgroups of a launch that shares the keys out: two per CU.
+constexpr int kGroups = 2 * 256;
+// What a piece costs beside its tiles (indices, the first tiles' latency, its
+// result), and the least a workgroup is given, in tiles of 64 keys.
+constexpr int kPieceCost = 3, kLeastShare = 2;
 
 struct TreeArgs {
   const void* q;
@@ -75,31 +80,14 @@ struct TreeArgs {
   float scale_log2;
   void* out;
   int64_t o_st, o_sh;
-  float* part_o;   // [chunks][tokens][q heads][D]
-  float* part_ml;  // [chunks][tokens][q heads][2]
-  int32_t* used;   // [tokens]: chunks of the token's request
+  float* part_o;   // [2 kGroups][rows of a block][D]
+  float* part_ml;  // [2 kGroups][rows of a block][2]
+  int32_t* owner;  // [tokens][q heads][4]: the workgroups with the row's first (-1: all) and last keys, its row
   int64_t n_tokens, max_len;
   int32_t n_requests, q_heads, kv_heads, group, head_dim, mask_words, page_size;
-  int32_t chunks, row_blocks, heads_last;
-  bool indptr64, out_f32, paged;
+  int32_t row_blocks;  // whole launch: workgroups that share a request's rows
+  bool indptr64, out_f32, paged, whole;
 };
-
-// Workgroups that a batch's keys are shared out over: four per CU.
-constexpr int64_t kTargetGroups = 4 * 256;
-
-// Keys of a chunk for a request that reaches `span` of a batch's `total` keys.
-template <int D>
-__device__ __forceinline__ int64_t chunk_keys_of(const TreeArgs& a, int64_t span, int64_t total) {
-  const int64_t reach = a.max_len * a.n_requests;
-  if (total > reach) total = reach;
-  const int64_t work = total * a.kv_heads * a.row_blocks;
-  int64_t most = (work / kTargetGroups + keys_of(D) - 1) / keys_of(D) * keys_of(D);
-  const int64_t least = (span + a.chunks - 1) / a.chunks;
-  if (most < keys_of(D)) most = keys_of(D);
-  if (most < least) most = (least + 63) / 64 * 64;
-  const int64_t n = span > 0 ? (span + most - 1) / most : 1;
-  return n > 1 ? ((span + n - 1) / n + 63) / 64 * 64 : most;
-}
 
 static __device__ __attribute__((aligned(16))) const uint32_t zero_row[64] = {};
 
@@ -114,8 +102,10 @@ __device__ __forceinline__ int swz_v(int r) { return D == 64 ? r & 6 : (r & 7) <
 
 __device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
 __device__ __forceinline__ int64_t uniform(int64_t v) {
-  const uint32_t lo = uniform(static_cast<int32_t>(v)), hi = uniform(static_cast<int32_t>(v >> 32));
+  const uint32_t lo = uniform(static_cast<uint32_t>(v)), hi = uniform(static_cast<uint32_t>(v >> 32));
   return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
@@ -179,46 +169,30 @@ __device__ __forceinline__ float column_max(float x) {
   return max2(__builtin_bit_cast(float, c0), __builtin_bit_cast(float, c1));
 }
 
-// Reads from a tile.  In asm, with their wait: the compiler takes every LDS read
-// for one that may meet the rows streaming into the other buffer, and would wait
-// for those first.
+// Loads straight into LDS: lane l's bytes go to `to` + 16 l (4 l).  In asm, since
+// the compiler takes every later LDS read for one that may meet them and waits
+// for all of them; here arrive() does the waiting.  (Nothing else in these kernels
+// uses m0.)
+__device__ __forceinline__ void load_16(const void* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
+}
+__device__ __forceinline__ void load_4(const void* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(to) : "memory");
+}
+
+// Waits for this wave's loads but its last N, and for its LDS accesses, then for
+// the other waves.
+template <int N>
+__device__ __forceinline__ void wait_and_meet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)p));
 }
 
-// Two 16-byte chunks of the K row at either address, 16 rows apart by STRIDE.
-template <int STRIDE>
-__device__ __forceinline__ void read_k(uint32_t a0, uint32_t a1, u32x4 (&lo)[2], u32x4 (&hi)[2]) {
-  asm volatile(
-      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %4 offset:%6\n\tds_read_b128 %3, %5 offset:%6\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(hi[0]), "=&v"(hi[1])
-      : "v"(a0), "v"(a1), "i"(STRIDE)
-      : "memory");
-}
-
-// Four transposed operands: 4 x 16 dims of 32 keys.
-template <int STRIDE>
-__device__ __forceinline__ void read_v(const uint32_t (&at)[4], s16x4 (&lo)[4], s16x4 (&hi)[4]) {
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
-      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "i"(STRIDE)
-      : "memory");
-}
-
-__device__ __forceinline__ u32x4 read_16(uint32_t at) {
-  u32x4 w;
-  asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(w) : "v"(at) : "memory");
-  return w;
-}
-
 template <int D>
-struct TileLds {
+struct alignas(16) TileLds {
   char k[keys_of(D) * D * 2];  // key-major, 16-byte chunks swizzled per row (swz_k)
   char v[keys_of(D) * D * 2];  // key-major, read transposed, swizzled (swz_v)
 };
@@ -236,10 +210,14 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
   constexpr int kChunks = D / 8;             // 16-byte chunks of a row
   constexpr int kLoadRows = 64 / kChunks;    // rows of one wave-wide load
   constexpr int kWaveKeys = kKeys / kWaves;  // keys of a tile that a wave asks for
+  constexpr int kLoads = 2 * kWaveKeys / kLoadRows;  // a wave's loads of a tile
+  constexpr int kEntryTiles = 64 / kWaveKeys;  // tiles whose keys of this wave fill a vector register
+  constexpr int kOver = kPieceCost * 64 / kKeys;
   constexpr int kGroupRows = 16 * SUB;       // rows of a wave
   constexpr int R = kWaves * kGroupRows;     // rows of a block
-  __shared__ __attribute__((aligned(256))) TileLds<D> buffers[2];
-  __shared__ __attribute__((aligned(16))) uint32_t s_dead[2][4];  // keys of the buffers' quarters that no token sees
+  __shared__ TileLds<D> buffers[kBuffers];
+  __shared__ int32_t s_entry[kWaves][2][64];  // list entries of the waves' keys, kEntryTiles tiles at a time
+  __shared__ uint32_t s_dead[2 * kEntryTiles][kQuarters];  // the tiles' keys that no token sees
   __shared__ float s_m[kWaves][kGroupRows], s_l[kWaves][kGroupRows];
   __shared__ int32_t s_tok[kWaves][kGroupRows];  // the rows' tokens, for the masked quarters
   __shared__ int32_t s_odd;                      // V rows held infinities or NaN that some row does not see
@@ -249,29 +227,114 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  // block id -> (unit, row block): a unit's row blocks lie 8 apart, on one XCD
-  const uint32_t round = 8 * a.row_blocks;
-  const uint32_t unit = blockIdx.x / round * 8 + blockIdx.x % 8;
-  const int rb0 = blockIdx.x % round / 8;
-  const uint32_t pair = unit / a.chunks;
-  const int chunk = unit - pair * a.chunks;
-  if (pair >= static_cast<uint32_t>(a.n_requests) * a.kv_heads) return;
-  const int b = a.heads_last ? pair % a.n_requests : pair / a.kv_heads;
-  const int g = a.heads_last ? pair / a.n_requests : pair % a.kv_heads;
-  // in scalar registers: the loop has no vector register to spare
+  // One wave's view of the batch.  A request costs its tiles and kPieceCost for
+  // every block of rows; block rb's cost is 0 where the request has no such rows.
+  auto units_of = [&](int64_t len, int32_t rows, int rb) -> int32_t {
+    if (a.key_starts && len > a.max_len) len = a.max_len;  // what a window reaches is not known here
+    const int64_t tiles = len > kKeys ? (len + kKeys - 1) / kKeys : 1;
+    return rb * R < rows ? static_cast<int32_t>(tiles + kOver) : 0;
+  };
+  struct Cost {
+    int32_t units, rows;
+  };
+  auto cost_of = [&](int64_t b, int rb) -> Cost {
+    int64_t q0 = load_index(a.qo_indptr, a.indptr64, b), q1 = load_index(a.qo_indptr, a.indptr64, b + 1);
+    const int64_t len = load_index(a.kv_indptr, a.indptr64, b + 1) - load_index(a.kv_indptr, a.indptr64, b);
+    q0 = q0 < 0 ? 0 : q0;
+    q1 = q1 > a.n_tokens ? a.n_tokens : q1;
+    const int32_t rows = q1 > q0 ? static_cast<int32_t>(q1 - q0) * a.group : 0;
+    return Cost{units_of(len, rows, rb), rows};
+  };
+  int32_t lane_units = 0;  // of request `lane`, for the block of rows last summed
+  auto sum_of = [&](int rb, int32_t* most_rows) -> int64_t {
+    int64_t sum = 0;
+    int32_t most = 0;
+    lane_units = 0;
+    for (int b = lane; b < a.n_requests; b += 64) {
+      const Cost c = cost_of(b, rb);
+      if (b < 64) lane_units = c.units;
+      sum += c.units;
+      most = max(most, c.rows);
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      sum += __shfl_xor(sum, off);
+      most = max(most, __shfl_xor(most, off));
+    }
+    *most_rows = uniform(most);
+    return uniform(sum);
+  };
+
+  if (gated(a.gate)) return;
+  int b, g, rb, blocks = 0;
+  int64_t off = 0, budget = 0;
+  const int group_id = blockIdx.x;
+  if (a.whole) {
+    // a workgroup per request, KV head and row_blocks-th block of rows
+    const int pair = group_id / a.row_blocks;
+    rb = group_id - pair * a.row_blocks;
+    g = pair / a.n_requests;
+    b = pair - g * a.n_requests;
+  } else {
+    // all work on a line: blocks of rows, KV heads, requests (fastest).  The
+    // workgroups take equal stretches of it; a cut falls among a request's tiles.
+    int32_t most_rows;
+    int64_t sum = sum_of(0, &most_rows);
+    blocks = (most_rows + R - 1) / R;
+    int64_t all = sum;
+    const int32_t first_units = lane_units;
+    for (int i = 1; i < blocks; ++i) {
+      int32_t unused;
+      all += sum_of(i, &unused);
+    }
+    all *= a.kv_heads;
+    lane_units = first_units;
+    if (all == 0) return;
+    int64_t groups = all / (kLeastShare * 64 / kKeys);
+    groups = groups < 1 ? 1 : groups < kGroups ? groups : kGroups;
+    if (group_id >= groups) return;
+    int64_t x = all * group_id / groups;
+    budget = all * (group_id + 1) / groups - x;
+    rb = 0;
+    while (x >= sum * a.kv_heads) {
+      int32_t unused;
+      x -= sum * a.kv_heads;
+      sum = sum_of(++rb, &unused);
+    }
+    g = static_cast<int>(x / sum);
+    x -= g * sum;
+    b = 0;
+    for (int b0 = 0; b0 < a.n_requests; b0 += 64) {
+      const int32_t mine = b0 == 0 ? lane_units : b0 + lane < a.n_requests ? cost_of(b0 + lane, rb).units : 0;
+      int64_t until = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int64_t up = __shfl_up(until, o);
+        if (lane >= o) until += up;
+      }
+      const uint64_t past = __builtin_amdgcn_ballot_w64(until > x);
+      if (past) {
+        const int at = __builtin_ctzll(past);
+        b = b0 + at;
+        off = uniform(x - __shfl(until - mine, at));
+        break;
+      }
+      x -= __shfl(until, 63);
+    }
+  }
+
+  for (;;) {
+  // (in scalar registers: the loop has no vector register to spare)
   int64_t q0 = uniform(load_index(a.qo_indptr, a.indptr64, b)), q1 = uniform(load_index(a.qo_indptr, a.indptr64, b + 1));
   const int64_t kv0 = uniform(load_index(a.kv_indptr, a.indptr64, b));
   const int64_t len64 = uniform(load_index(a.kv_indptr, a.indptr64, b + 1)) - kv0;
-  const int64_t total = uniform(load_index(a.kv_indptr, a.indptr64, a.n_requests)) -
-                        uniform(load_index(a.kv_indptr, a.indptr64, 0));
-  if (gated(a.gate)) return;
   if (q0 < 0) q0 = 0;
   if (q1 > a.n_tokens) q1 = a.n_tokens;
   const int n = static_cast<int>(q1 > q0 ? q1 - q0 : 0);
   const int rows = n * a.group;
-  if (rb0 * R >= rows) return;
   const int len = static_cast<int>(len64 > 0 ? len64 : 0);
   const int old = len > n ? len - n : 0;
+  if (a.whole && rb * R >= rows) return;
   // the keys that some token of the request sees begin here
   int lo = 0, hi_start = 0;
   if (a.key_starts) {
@@ -282,68 +345,82 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
       hi_start = max(hi_start, s);
     }
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      lo = min(lo, __shfl_xor(lo, off));
-      hi_start = max(hi_start, __shfl_xor(hi_start, off));
+    for (int o = 1; o < 64; o <<= 1) {
+      lo = min(lo, __shfl_xor(lo, o));
+      hi_start = max(hi_start, __shfl_xor(hi_start, o));
     }
     lo = uniform(lo);
     hi_start = uniform(hi_start);
   }
-  const int span = len - lo;
-  const int64_t chunk_keys = uniform(chunk_keys_of<D>(a, span, total));
-  const int used = span > 0 ? uniform(static_cast<int32_t>((span + chunk_keys - 1) / chunk_keys)) : 1;
-  if (chunk >= used) return;
-  const int begin = lo + static_cast<int>(chunk * chunk_keys);
-  const int end = static_cast<int>(std::min<int64_t>(begin + chunk_keys, len));
-  const int tiles = (end - begin + kKeys - 1) / kKeys;
-  if (chunk == 0 && g == 0 && rb0 == 0)
-    for (int i = threadIdx.x; i < n; i += kThreads) a.used[q0 + i] = used;
+  // the piece: units [off, stop) of the request's, the first kPieceCost of them
+  // for no tile, the others for equal parts of its tiles
+  const int units = units_of(len, rows, rb);
+  const int stop = a.whole || budget > units - off ? units : static_cast<int>(off + budget);
+  const bool first = off == 0, last = stop == units;
+  const int all_tiles = (len - lo + kKeys - 1) / kKeys;
+  auto tile_of = [&](int64_t unit) -> int {
+    const int64_t at = unit > kOver ? unit - kOver : 0;
+    return static_cast<int>(units - kOver == all_tiles ? at : at * all_tiles / (units - kOver));
+  };
+  const int begin = lo + uniform(tile_of(off)) * kKeys;
+  const int end = min(lo + uniform(tile_of(stop)) * kKeys, len);
+  const int tiles = end > begin ? (end - begin + kKeys - 1) / kKeys : 0;
 
   // (an empty pool holds no key: every slot is a hole, and zeros are read)
   const bool pool = a.pool_slots > 0;
   const char* kbase = pool ? a.k + g * a.k_sh : reinterpret_cast<const char*>(zero_row);
   const char* vbase = pool ? a.v + g * a.v_sh : reinterpret_cast<const char*>(zero_row);
-  const int64_t k_ss = pool ? a.k_ss : 0, v_ss = pool ? a.v_ss : 0;
+  const uint32_t k_ss = pool ? a.k_ss : 0, v_ss = pool ? a.v_ss : 0;
   const int32_t* list = a.kv_indices + (a.paged ? b * a.table_stride : kv0);
   // entries of the list that exist
   const int64_t left = a.paged ? a.table_width : a.table_width - kv0;
   const int32_t width = static_cast<int32_t>(std::min<int64_t>(std::max<int64_t>(left, 0), 0x7fffffff));
-  const uint32_t dead_at = lds_address(s_dead), tile_at = lds_address(buffers);
-  const int my_key = kWaveKeys * wave + (lane & (kWaveKeys - 1));  // of a tile
-  // the list entry of this lane's key of tile it (past the end: the last key's),
-  // one tile ahead; what it means is worked out when the tile is asked for
-  auto fetch = [&](int it) -> int32_t {
-    const uint32_t j = min(begin + it * kKeys + my_key, end - 1);
+  const int32_t* entries = width > 0 ? list : reinterpret_cast<const int32_t*>(zero_row);
+  const int last_entry = max(width - 1, 0);
+  // The wave's keys of kEntryTiles tiles at a time: lane l has key l % kWaveKeys
+  // of tile l / kWaveKeys.  Their list entries come to LDS kEntryTiles tiles ahead.
+  const int my_key = lane / kWaveKeys * kKeys + kWaveKeys * wave + lane % kWaveKeys;
+  auto fetch = [&](int e) {
+    const uint32_t j = min(begin + e * (kEntryTiles * kKeys) + my_key, end - 1);  // past the end: the last key's
     const int32_t at = a.paged ? j / static_cast<uint32_t>(a.page_size) : j;
-    return width > 0 ? list[min(at, width - 1)] : -1;
+    load_4(entries + min(at, last_entry), uniform(lds_address(s_entry[wave][e & 1])));
+  };
+  uint32_t slots = 0;
+  auto look_up = [&](int e) {
+    const uint32_t key = begin + e * (kEntryTiles * kKeys) + my_key, j = min(key, static_cast<uint32_t>(end - 1));
+    const int32_t entry = s_entry[wave][e & 1][lane];
+    uint64_t slot = static_cast<uint32_t>(entry);
+    uint32_t at = j;
+    if (a.paged) {
+      const uint32_t page = a.page_size;
+      at = j / page;
+      slot = slot * page + (j - at * page);
+    }
+    const bool there = entry >= 0 && at < static_cast<uint32_t>(width) && slot < static_cast<uint64_t>(a.pool_slots);
+    // a hole reads slot 0; the mask keeps it from every row
+    slots = there ? static_cast<uint32_t>(slot) : 0;
+    const uint64_t dead = __builtin_amdgcn_ballot_w64(!there || key >= static_cast<uint32_t>(end));
+    if (lane < kEntryTiles) {
+      const uint32_t mine = static_cast<uint32_t>(dead >> (kWaveKeys * lane));
+      char* to = reinterpret_cast<char*>(s_dead[(e & 1) * kEntryTiles + lane]) + kWaveKeys / 8 * wave;
+      if constexpr (kWaveKeys == 16)
+        *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(mine);
+      else
+        *reinterpret_cast<uint8_t*>(to) = static_cast<uint8_t>(mine);
+    }
   };
   // a wave's keys of a tile, straight into LDS: lane l of a load fills bytes
   // 16 l of a 1 KiB block, chunk position l % kChunks of a row
-  auto stage = [&](int it, int32_t entry) {
-    TileLds<D>& t = buffers[it & 1];
-    const uint32_t key = begin + it * kKeys + my_key, j = min(key, static_cast<uint32_t>(end - 1));
-    uint32_t at = j, off = 0, per = 1;
-    if (a.paged) {
-      per = a.page_size;
-      at = j / per;
-      off = j - at * per;
+  auto stage = [&](int it) {
+    if (it % kEntryTiles == 0) {
+      look_up(it / kEntryTiles);
+      fetch(it / kEntryTiles + 1);
     }
-    const uint64_t slot64 = static_cast<uint64_t>(static_cast<uint32_t>(entry)) * per + off;
-    const bool there = entry >= 0 && at < static_cast<uint32_t>(width) && slot64 < static_cast<uint64_t>(a.pool_slots);
-    // a hole reads slot 0; the mask keeps it from every row
-    const uint32_t slot = there ? static_cast<uint32_t>(slot64) : 0;
-    const uint32_t dead = static_cast<uint32_t>(
-        __builtin_amdgcn_ballot_w64(!there || key >= static_cast<uint32_t>(end)));
-    if (lane == 0) {
-      if constexpr (kWaveKeys == 32)
-        asm volatile("ds_write_b32 %0, %1" ::"v"(dead_at + 16 * (it & 1) + 4 * wave), "v"(dead) : "memory");
-      else
-        asm volatile("ds_write_b16 %0, %1" ::"v"(dead_at + 16 * (it & 1) + 2 * wave), "v"(dead) : "memory");
-    }
+    TileLds<D>& t = buffers[it % kBuffers];
 #pragma unroll
     for (int u = 0; u < kWaveKeys / kLoadRows; ++u) {
       const int mine = u * kLoadRows + lane / kChunks, r = kWaveKeys * wave + mine;
-      const uint64_t from = __shfl(slot, mine);
+      const uint64_t from = __shfl(slots, it % kEntryTiles * kWaveKeys + mine);
       const int ck = (lane % kChunks) ^ swz_k<D>(r), cv = (lane % kChunks) ^ swz_v<D>(r);
       const char* krow = kbase + from * k_ss + 16 * ck;
       const char* vrow = vbase + from * v_ss + 16 * cv;
@@ -352,13 +429,24 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
         vrow = 8 * cv < a.head_dim ? vrow : reinterpret_cast<const char*>(zero_row);
       }
       const int place = (kWaveKeys * wave + u * kLoadRows) * D * 2;
-      __builtin_amdgcn_global_load_lds(krow, (lds_void*)(t.k + place), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(vrow, (lds_void*)(t.v + place), 16, 0, 0);
+      load_16(krow, uniform(lds_address(t.k + place)));
+      load_16(vrow, uniform(lds_address(t.v + place)));
     }
   };
+  // the oldest tile asked for is here, with `newer` tiles asked for behind it
+  // (with list entries among them, a load or two more is waited for)
+  auto arrive = [&](int newer) {
+    static_assert(kBuffers == 4, "the waits");
+    if (newer >= 2)
+      wait_and_meet<2 * kLoads>();
+    else if (newer == 1)
+      wait_and_meet<kLoads>();
+    else
+      wait_and_meet<0>();
+  };
 
-  for (int rb = rb0; rb * R < rows; rb += a.row_blocks) {
-    int32_t entry = tiles > 0 ? fetch(0) : -1;
+  {
+    if (tiles > 0) fetch(0);
     if (threadIdx.x == 0) s_odd = 0;
     // groups of rows, and the waves that share one
     int groups = kWaves, sharers = 1;
@@ -386,12 +474,12 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
         qop[s][st] = __builtin_bit_cast(x8, w);
       }
     }
-    f32x4 acc[SUB][kDTiles], lacc[SUB];  // l: four equal copies; 0 while the row has seen no key
-    float neg_m[SUB];
+    f32x4 acc[SUB][kDTiles];
+    float neg_m[SUB], l[SUB];  // l: 0 while the row has seen no key
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
       neg_m[s] = 0.f;
-      lacc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+      l[s] = 0.f;
 #pragma unroll
       for (int t = 0; t < kDTiles; ++t) acc[s][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -427,12 +515,12 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
     // A weight of 0 does not hide an infinity or NaN from the product.  Where
     // rows see different keys such values are cleared (by every wave that uses
     // them) and the block takes note: its rows get them back at the end.
-    auto clear_odd = [&](uint32_t at, uint32_t dead) {
+    auto clear_odd = [&](char* quarter, uint32_t dead) {
       bool noted = false;
 #pragma nounroll
       for (int i = 0; i < kDTiles; ++i) {
-        const uint32_t here = at + 1024 * i + 16 * lane;
-        s16x8 w = __builtin_bit_cast(s16x8, read_16(here));
+        s16x8* here = reinterpret_cast<s16x8*>(quarter + 1024 * i + 16 * lane);
+        s16x8 w = *here;
         bool odd = false;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -440,37 +528,81 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
           odd |= one;
           w[e] = one ? 0 : w[e];
         }
-        if (odd) asm volatile("ds_write_b128 %0, %1" ::"v"(here), "v"(w) : "memory");
+        if (odd) *here = w;
         noted |= odd && !(dead >> ((64 * i + lane) / kChunks) & 1);
       }
-      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): cleared before they are read
-      if (__builtin_amdgcn_ballot_w64(noted) && lane == 0)
-        asm volatile("ds_write_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" ::"v"(lds_address(&s_odd)), "v"(1) : "memory");
+      if (noted) s_odd = 1;
     };
-    // this lane's operand addresses in quarter 0: K chunks quad of row col, and
-    // the source of its transposed V reads (row 4 quad + col / 4, dims 4 (col % 4))
-    const uint32_t k_at = col * D * 2 + 16 * (quad ^ swz_k<D>(col));
+    // this lane's operands in quarter 0: K chunks 4 st + quad of row col, and the
+    // source of its transposed V reads (row 4 quad + col / 4, dims 16 dt + 4 (col
+    // % 4)); the swizzles are the same in every quarter
+    uint32_t k_at[kSteps], v_at[kDTiles];
     const int vr = 4 * quad + (col >> 2);
-    const uint32_t v_at = kKeys * D * 2 + vr * D * 2 + 16 * ((col >> 1 & 1) ^ swz_v<D>(vr)) + 8 * (col & 1);
-    // 32 keys, from row 32 kk of a tile on; k0: the first one's rank
-    auto quarter = [&](uint32_t at, int k0, uint32_t dead) {
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) k_at[st] = col * D * 2 + 16 * ((4 * st + quad) ^ swz_k<D>(col));
+#pragma unroll
+    for (int dt = 0; dt < kDTiles; ++dt)
+      v_at[dt] = vr * D * 2 + 16 * ((2 * dt + (col >> 1 & 1)) ^ swz_v<D>(vr)) + 8 * (col & 1);
+    // scores of the 32 keys of a quarter: S^T[16 j + 4 quad + i][row 16 s + col]
+    auto scores = [&](const TileLds<D>& t, int kk, f32x4 (&sc)[2][SUB]) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+          const x8 kop = __builtin_bit_cast(x8, *reinterpret_cast<const u32x4*>(t.k + (64 * kk + 32 * j) * D + k_at[st]));
+#pragma unroll
+          for (int s = 0; s < SUB; ++s)
+            sc[j][s] = product(kop, qop[s][st], st == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[j][s]);
+        }
+      }
+    };
+    // O^T += V^T . P^T: lane col of group quad receives V[key][16 dt + col] for
+    // keys 4 quad + i (i < 4) of the quarter, then 16 keys on
+    auto values = [&](const TileLds<D>& t, int kk, const x8 (&p)[SUB]) {
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt) {
+        const s16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(t.v + 64 * kk * D + v_at[dt]));
+        const s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(t.v + (64 * kk + 32) * D + v_at[dt]));
+        const x8 vop = __builtin_bit_cast(x8, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) acc[s][dt] = product(vop, p[s], acc[s][dt]);
+      }
+    };
+    // 32 keys that every row sees, when every row has a maximum; false, with
+    // nothing done, where a sum outgrows kHuge
+    auto quick = [&](const TileLds<D>& t, int kk) -> bool {
+      f32x4 sc[2][SUB];
+      scores(t, kk, sc);
+      x8 p[SUB];
+      float sum[SUB];
+      bool huge = false;
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        f32x4 e0, e1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e0[i] = __builtin_amdgcn_exp2f(fmaf(sc[0][s][i], a.scale_log2, neg_m[s]));
+          e1[i] = __builtin_amdgcn_exp2f(fmaf(sc[1][s][i], a.scale_log2, neg_m[s]));
+        }
+        p[s] = __builtin_shufflevector(__builtin_convertvector(e0, x4), __builtin_convertvector(e1, x4), 0, 1, 2, 3, 4,
+                                       5, 6, 7);
+      }
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        sum[s] = l[s] + product(ones, p[s], f32x4{0.f, 0.f, 0.f, 0.f})[0];
+        huge |= sum[s] > kHuge;
+      }
+      if (__builtin_amdgcn_ballot_w64(huge)) return false;
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) l[s] = sum[s];
+      values(t, kk, p);
+      return true;
+    };
+    // any 32 keys; k0: the first one's rank
+    auto quarter = [&](TileLds<D>& t, int kk, int k0, uint32_t dead) {
       const bool masked = dead != 0 || k0 + 32 > old || k0 < hi_start;
       f32x4 sc[2][SUB];
-#pragma unroll
-      for (int h = 0; h < kSteps / 2; ++h) {
-        // k-steps 2 h and 2 h + 1: chunks 4 and 8 on (the swizzle is an xor)
-        u32x4 lo[2], hi[2];
-        read_k<16 * D * 2>((at + k_at) ^ (128 * h), (at + k_at) ^ (128 * h + 64), lo, hi);
-#pragma unroll
-        for (int st = 0; st < 2; ++st)
-#pragma unroll
-          for (int s = 0; s < SUB; ++s) {
-            sc[0][s] = product(__builtin_bit_cast(x8, lo[st]), qop[s][2 * h + st],
-                               h + st == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[0][s]);
-            sc[1][s] = product(__builtin_bit_cast(x8, hi[st]), qop[s][2 * h + st],
-                               h + st == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[1][s]);
-          }
-      }
+      scores(t, kk, sc);
       if (masked) {
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
@@ -487,9 +619,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
       // score ~64 above m in the log2 domain, 16 in fp16, whose weight is then
       // infinite) takes the quarter again with exact maxima.
       x8 p[SUB];
-      float before[SUB];
-#pragma unroll
-      for (int s = 0; s < SUB; ++s) before[s] = lacc[s][0];
+      float sum[SUB];
       for (bool exact = unset;; exact = true) {
         if (exact) {
 #pragma unroll
@@ -498,14 +628,13 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
             const float m1 = max3(sc[0][s][3], sc[1][s][0], sc[1][s][1]);
             const float mx = column_max(max3(m0, m1, max2(sc[1][s][2], sc[1][s][3])));
             const float over = fmaf(mx, a.scale_log2, neg_m[s]);  // above m
-            const bool any = before[s] != 0.f;
+            const bool any = l[s] != 0.f;
             const bool move = any ? over > 0.f : mx > -INFINITY;
             const float alpha = move && any ? __builtin_amdgcn_exp2f(-over) : 1.f;
-            before[s] *= alpha;
+            l[s] *= alpha;
 #pragma unroll
             for (int dt = 0; dt < kDTiles; ++dt) acc[s][dt] *= alpha;
             neg_m[s] = move ? -(mx * a.scale_log2) : neg_m[s];
-            lacc[s] = f32x4{before[s], before[s], before[s], before[s]};
           }
         }
         bool huge = false;
@@ -519,73 +648,61 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
           }
           p[s] = __builtin_shufflevector(__builtin_convertvector(e0, x4), __builtin_convertvector(e1, x4), 0, 1, 2, 3,
                                          4, 5, 6, 7);
-          lacc[s] = product(ones, p[s], lacc[s]);
+          sum[s] = l[s] + product(ones, p[s], f32x4{0.f, 0.f, 0.f, 0.f})[0];
+          huge |= sum[s] > kHuge;
         }
-#pragma unroll
-        for (int s = 0; s < SUB; ++s) huge |= lacc[s][0] > kHuge;
         if (exact || !__builtin_amdgcn_ballot_w64(huge)) break;
       }
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) l[s] = sum[s];
       if (unset) {
         bool none = false;
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) none |= lacc[s][0] == 0.f;
+        for (int s = 0; s < SUB; ++s) none |= l[s] == 0.f;
         unset = __builtin_amdgcn_ballot_w64(none) != 0;
       }
-      // transposing reads: lane col of group quad receives V[key][16 dt + col]
-      // for keys 4 quad + i (i < 4) of the quarter, then 16 keys on; dt = 4 h + e
-      auto v_operands = [&](int h, x8 (&v)[4]) {
-        uint32_t from[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) from[e] = (at + v_at) ^ (32 * (4 * h + e));
-        s16x4 lo[4], hi[4];
-        read_v<16 * D * 2>(from, lo, hi);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = __builtin_bit_cast(x8, __builtin_shufflevector(lo[e], hi[e], 0, 1, 2, 3, 4, 5, 6, 7));
-      };
-      if (masked) clear_odd(at + kKeys * D * 2, dead);
-#pragma unroll
-      for (int h = 0; h < kDTiles / 4; ++h) {
-        x8 v[4];
-        v_operands(h, v);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int s = 0; s < SUB; ++s) acc[s][4 * h + e] = product(v[e], p[s], acc[s][4 * h + e]);
-      }
+      if (masked) clear_odd(t.v + 64 * kk * D, dead);
+      values(t, kk, p);
     };
-    if (tiles > 0) {
-      stage(0, entry);
-      if (tiles > 1) entry = fetch(1);
-    }
-    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_s_waitcnt(0);  // (one the compiler sees: Q has arrived)
     __syncthreads();
-    // tile it from one buffer while tile it + 1 streams into the other
+#pragma unroll
+    for (int it = 0; it < kBuffers - 1; ++it)
+      if (it < tiles) stage(it);
+    arrive(tiles - 1);
+    // this wave's quarters of a tile
+    uint32_t quarters = 0;
+#pragma unroll
+    for (int kk = 0; kk < kQuarters; ++kk) quarters |= (kk & (sharers - 1)) == share ? 1u << kk : 0;
 #pragma nounroll
     for (int it = 0; it < tiles; ++it) {
-      const int buf = it & 1;
-      if (it + 1 < tiles) {
-        stage(it + 1, entry);
-        if (it + 2 < tiles) entry = fetch(it + 2);
-      }
+      // into the place that was last read before the barrier
+      if (it + kBuffers - 1 < tiles) stage(it + kBuffers - 1);
+      TileLds<D>& t = buffers[it % kBuffers];
       const int t0 = begin + it * kKeys;
-      const uint32_t cur = tile_at + buf * static_cast<uint32_t>(sizeof(TileLds<D>));
-      const u32x4 dead = read_16(dead_at + 16 * buf);
-#pragma nounroll
-      for (int kk = share; kk < kQuarters; kk += sharers) {
-        const int k0 = t0 + 32 * kk;
-        if (k0 >= end) break;
-        const uint32_t word = kk == 0 ? dead[0] : kk == 1 ? dead[1] : kk == 2 ? dead[2] : dead[3];
-        quarter(cur + kk * 64 * D, k0, __builtin_amdgcn_readfirstlane(word));
+      const uint32_t* dead = s_dead[it % (2 * kEntryTiles)];
+      uint32_t holes = dead[0];
+#pragma unroll
+      for (int kk = 1; kk < kQuarters; ++kk) holes |= dead[kk];
+      uint32_t todo = quarters;
+      if (!unset && t0 + kKeys <= old && t0 >= hi_start && uniform(holes) == 0) {
+#pragma unroll
+        for (int kk = 0; kk < kQuarters; ++kk)
+          if (todo >> kk & 1 && quick(t, kk)) todo &= ~(1u << kk);
       }
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
+#pragma nounroll
+      for (; todo; todo &= todo - 1) {
+        const int kk = __builtin_ctz(todo), k0 = t0 + 32 * kk;
+        if (k0 >= end) break;
+        quarter(t, kk, k0, uniform(dead[kk]));
+      }
+      arrive(tiles - 2 - it);
     }
 
     // the waves' O rows [row][dim] over the tiles, four-float groups turned by
     // the row for the banks; the sharers of a group meet there
     auto result_of = [&](int w) -> float* {
-      return reinterpret_cast<float*>(&buffers[0]) + w * kGroupRows * D;
+      return reinterpret_cast<float*>(buffers) + w * kGroupRows * D;
     };
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
@@ -594,31 +711,43 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
       for (int dt = 0; dt < kDTiles; ++dt)
         *reinterpret_cast<f32x4*>(result_of(wave) + r * D + ((16 * dt + 4 * quad) ^ (col & 7) << 2)) = acc[s][dt];
       if (quad == 0) {
-        s_m[wave][r] = lacc[s][0] == 0.f ? -INFINITY : -neg_m[s];
-        s_l[wave][r] = lacc[s][0];
+        s_m[wave][r] = l[s] == 0.f ? -INFINITY : -neg_m[s];
+        s_l[wave][r] = l[s];
       }
     }
     __syncthreads();
     const int here = min(rows - rb * R, groups * kGroupRows);
+    // an unfinished piece: a stretch has at most one that continues an earlier
+    // stretch's, and one that the next continues
+    const int64_t place = 2 * group_id + (first ? 1 : 0);
+    float* part = a.part_o + place * R * D;
+    float* part_ml = a.part_ml + place * R * 2;
     for (int u = threadIdx.x; u < here * (D / 4); u += kThreads) {
       const int r = u / (D / 4), d = 4 * (u % (D / 4));
       if (NARROW && d >= a.head_dim) continue;
       const int token = (rb * R + r) / a.group, head = g * a.group + rb * R + r - token * a.group;
       const int group = r / kGroupRows, in = r % kGroupRows;
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, lt = 0.f;
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
       for (int w = group; w < kWaves; w += groups) m = fmaxf(m, s_m[w][in]);
       // a wave that has seen no key carries m = -inf, l = 0 and O = 0
       const float base = m == -INFINITY ? 0.f : m;
       for (int w = group; w < kWaves; w += groups) {
         const float by = __builtin_amdgcn_exp2f(s_m[w][in] - base);
-        l += s_l[w][in] * by;
+        lt += s_l[w][in] * by;
         o += *reinterpret_cast<const f32x4*>(result_of(w) + in * D + (d ^ (in & 7) << 2)) * by;
       }
-      if (used > 1) {
-        const int64_t at = (static_cast<int64_t>(chunk) * a.n_tokens + q0 + token) * a.q_heads + head;
-        *reinterpret_cast<f32x4*>(a.part_o + at * D + d) = o;
-        if (d == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{m, l};
+      if (!a.whole && d == 0) {
+        int32_t* owner = a.owner + 4 * ((q0 + token) * a.q_heads + head);
+        if (first) {
+          owner[0] = last ? -1 : group_id;
+          owner[2] = r;
+        }
+        if (last) owner[1] = group_id;
+      }
+      if (!(first && last)) {
+        *reinterpret_cast<f32x4*>(part + r * D + d) = o;
+        if (d == 0) *reinterpret_cast<f32x2*>(part_ml + 2 * r) = f32x2{m, lt};
         continue;
       }
       if (a.sinks) {
@@ -626,9 +755,9 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
         const float mt = fmaxf(m, sink);
         const float by = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mt);
         o *= by;
-        l = l * by + (mt == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - mt));
+        lt = lt * by + (mt == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - mt));
       }
-      store_row<T>(a, q0 + token, head, d, o, l);
+      store_row<T>(a, q0 + token, head, d, o, lt);
     }
     // values cleared from the products go back, unweighted, to the rows that see
     // them: whatever their weights, the results are the infinity or NaN
@@ -660,8 +789,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
               for (int i = 0; i < 4; ++i) {
                 if (!not_finite<T>(__builtin_bit_cast(short, v[i]))) continue;
                 const float x = static_cast<float>(v[i]);
-                if (used > 1) {
-                  a.part_o[((static_cast<int64_t>(chunk) * a.n_tokens + q0 + token) * a.q_heads + head) * D + d + i] += x;
+                if (!(first && last)) {
+                  part[(r - rb * R) * D + d + i] += x;
                   continue;
                 }
                 const int64_t at = (q0 + token) * a.o_st + head * a.o_sh + d + i;
@@ -677,104 +806,136 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
     }
     __syncthreads();
   }
-}
-
-// Merges a row's chunks and the sink: a wave per (token, head).  Lane c takes
-// chunk c's maximum and sum; then D / 4 lanes each take the chunks in turn, four
-// dims a lane.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a) {
-  constexpr int kLanes = D / 4, kWays = 64 / kLanes, kAhead = 4;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + uniform(static_cast<int32_t>(threadIdx.x >> 6));
-  const int64_t token = row / a.q_heads;
-  const int head = static_cast<int>(row - token * a.q_heads);
-  if (token >= a.n_tokens || token >= load_index(a.qo_indptr, a.indptr64, a.n_requests) ||
-      token < load_index(a.qo_indptr, a.indptr64, 0))
-    return;
-  if (gated(a.gate)) return;
-  const int used = uniform(a.used[token]);
-  if (used <= 1) return;
-  const int64_t step = a.n_tokens * a.q_heads;
-  const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + row;
-  const int d = 4 * (lane % kLanes), way = lane / kLanes;
-  const float* from = a.part_o + row * D + d;
-  const float sink = a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
-  float m = sink;
-  for (int c = lane; c < used; c += 64) m = fmaxf(m, ml[c * step].x);
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int c0 = 0; c0 < used; c0 += 64) {
-    f32x2 mine = {-INFINITY, 0.f};
-    if (c0 + lane < used) mine = ml[(c0 + lane) * step];
-    const float w = __builtin_amdgcn_exp2f(mine.x - base);
-    l += mine.y * w;
-    const int count = used - c0 < 64 ? used - c0 : 64;
-    for (int c = 0; c < count; c += kWays * kAhead) {
-      f32x4 x[kAhead];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int at = c + i * kWays + way;
-        x[i] = *reinterpret_cast<const f32x4*>(from + (c0 + (at < count ? at : 0)) * step * D);
+    if (a.whole) {
+      rb += a.row_blocks;
+      continue;
+    }
+    budget -= stop - off;
+    if (budget <= 0) return;
+    // the next request on the line
+    off = 0;
+    for (++b;;) {
+      int found = -1;
+      for (int b0 = b; b0 < a.n_requests && found < 0; b0 += 64) {
+        const uint64_t live = __builtin_amdgcn_ballot_w64(b0 + lane < a.n_requests && cost_of(b0 + lane, rb).units > 0);
+        if (live) found = b0 + __builtin_ctzll(live);
       }
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int at = c + i * kWays + way;
-        const float by = __shfl(w, at & 63);
-        if (at < count) o += x[i] * by;
+      if (found >= 0) {
+        b = found;
+        break;
+      }
+      b = 0;
+      if (++g == a.kv_heads) {
+        g = 0;
+        if (++rb >= blocks) return;
       }
     }
   }
+}
+
+// Merges the pieces of rows that a cut went through, and the sink: WAYS x D / 4
+// lanes per (token, head), each way every WAYS-th piece, kAhead of them in flight.
+template <typename T, int D, int WAYS>
+__global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a, const int block_rows) {
+  constexpr int kLanes = D / 4, kAhead = 4;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / (kLanes * WAYS)) + threadIdx.x / (kLanes * WAYS);
+  const int d = 4 * (threadIdx.x % kLanes), way = threadIdx.x / kLanes % WAYS;
+  const int64_t token = row / a.q_heads;
+  const int head = static_cast<int>(row - token * a.q_heads);
+  if (token >= a.n_tokens) return;
+  // one round of loads: whether the row is a token's, and who has its pieces
+  const int64_t begin = load_index(a.qo_indptr, a.indptr64, 0), end = load_index(a.qo_indptr, a.indptr64, a.n_requests);
+  const int32_t* owner = a.owner + 4 * row;
+  const int first = owner[0], last = owner[1], r = owner[2];
+  const float sink = a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
+  if (gated(a.gate) || token < begin || token >= end) return;
+  // (indptrs that descend leave rows without owners)
+  if (first < 0 || last < first || last >= kGroups || r < 0 || r >= block_rows) return;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int w = first + way; w <= last; w += kAhead * WAYS) {
+    f32x2 ml[kAhead];
+    f32x4 x[kAhead];
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) l += __shfl_xor(l, off);
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = w + i * WAYS <= last ? w + i * WAYS : last;
+      const int64_t place = (2ll * at + (at == first ? 1 : 0)) * block_rows + r;
+      ml[i] = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * place);
+      x[i] = *reinterpret_cast<const f32x4*>(a.part_o + place * D + d);
+    }
+    float top = m;
 #pragma unroll
-  for (int off = kLanes; off < 64; off <<= 1)
+    for (int i = 0; i < kAhead; ++i) top = fmaxf(top, ml[i].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    // a piece without a key carries m = -inf, l = 0 and O = 0
+    const float by = __builtin_amdgcn_exp2f(m - base);
+    l *= by;
+    o *= by;
+    m = top;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (w + i * WAYS > last) continue;
+      const float mine = __builtin_amdgcn_exp2f(ml[i].x - base);
+      l += ml[i].y * mine;
+      o += x[i] * mine;
+    }
+  }
+  float top = fmaxf(m, sink);
+#pragma unroll
+  for (int off = kLanes; off < kLanes * WAYS; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+  const float base = top == -INFINITY ? 0.f : top;
+  const float by = __builtin_amdgcn_exp2f(m - base);
+  l *= by;
+  o *= by;
+#pragma unroll
+  for (int off = kLanes; off < kLanes * WAYS; off <<= 1) {
+    l += __shfl_xor(l, off);
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], off);
-  if (a.sinks && m != -INFINITY) l += __builtin_amdgcn_exp2f(sink - base);
+  }
+  if (a.sinks) l += __builtin_amdgcn_exp2f(sink - base);
   if (way == 0 && d < a.head_dim) store_row<T>(a, token, head, d, o, l);
 }
 
 int tile_dim(int32_t head_dim) { return head_dim <= 64 ? 64 : 128; }
 
-// A wave's row subtiles for requests of up to `rows` rows: as many as the rows
-// fill, since waves that share rows read every key once.
+// A wave's row subtiles for requests of up to `rows` rows: a tile has keys for
+// two waves (one at D = 128) to share a group of rows, so the rows are dealt out
+// to two (four) groups before a wave takes more of them.
 int subtiles_for(int d, int64_t rows) {
   const int most = d == 64 ? 4 : 2;
+  const int64_t groups = d == 64 ? 2 : 4;
   int sub = 1;
-  while (sub < most && rows > 16 * sub) sub *= 2;
+  while (sub < most && rows > 16 * groups * sub) sub *= 2;
   return sub;
 }
 
 struct Launch {
   int d, sub;
-  int32_t row_blocks, chunks;
+  bool whole;
+  int32_t row_blocks;
 };
 
-Launch plan(int64_t n_tokens, int64_t n_requests, int64_t kv_heads, int64_t group, int32_t head_dim, int64_t max_len,
-            int64_t max_new) {
+// Keys up to which a request is one workgroup's: a cut would save less than the
+// second launch costs.
+constexpr int64_t kWholeKeys = 256;
+
+Launch plan(int64_t n_tokens, int64_t group, int32_t head_dim, int64_t max_len, int64_t max_new) {
   Launch p;
   p.d = tile_dim(head_dim);
   const int64_t rows = std::max<int64_t>(1, std::min(max_new, n_tokens)) * group;
   p.sub = subtiles_for(p.d, rows);
-  const int64_t block = 16 * kWaves * p.sub, pass = keys_of(p.d);
+  const int64_t block = 16 * kWaves * p.sub;
   p.row_blocks = static_cast<int32_t>(std::min<int64_t>((rows + block - 1) / block, 4096));
-  // chunks: as many as give every CU its share of a batch whose requests all
-  // have max_len keys, four times as many for a few long ones among short ones
-  const int64_t keys = std::max<int64_t>(pass, n_requests * max_len * kv_heads * p.row_blocks / kTargetGroups);
-  int64_t chunks = std::min((max_len + pass - 1) / pass, 4 * ((max_len + keys - 1) / keys));
-  chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, 4096));
-  // odd, so that the first chunks of the pairs go round all XCDs
-  p.chunks = static_cast<int32_t>(chunks > 1 ? chunks | 1 : 1);
+  p.whole = max_len <= kWholeKeys;
   return p;
 }
 
+int64_t owner_bytes(int64_t n_tokens, int64_t q_heads) { return 16 * n_tokens * q_heads; }
+
 int64_t partial_bytes(const Launch& p, int64_t n_tokens, int64_t q_heads) {
-  const int64_t rows = p.chunks > 1 ? p.chunks * n_tokens * q_heads : 0;
-  return rows * (p.d + 2) * 4 + (n_tokens + 3) / 4 * 16;
+  if (p.whole) return 16;
+  return owner_bytes(n_tokens, q_heads) + 2ll * kGroups * (16 * kWaves * p.sub) * (p.d + 2) * 4;
 }
 
 template <typename T, int D, int SUB>
@@ -785,10 +946,24 @@ void start(const TreeArgs& a, dim3 grid, hipStream_t st) {
     hipLaunchKernelGGL((tree_attention_kernel<T, D, SUB, false>), grid, dim3(kThreads), 0, st, a);
 }
 
+// Few rows are cut into many pieces each, and many rows fill the chip: a wave per
+// row up to kFewRows, D / 4 lanes beyond.
+constexpr int64_t kFewRows = 4096;
+
+template <typename T, int D>
+void merge(const TreeArgs& a, const Launch& p, hipStream_t st) {
+  constexpr int kWays = 64 / (D / 4);
+  const int64_t rows = a.n_tokens * a.q_heads, per = rows <= kFewRows ? 4 : 4 * kWays;
+  const dim3 grid(static_cast<unsigned>((rows + per - 1) / per));
+  if (rows <= kFewRows)
+    hipLaunchKernelGGL((tree_combine_kernel<T, D, kWays>), grid, dim3(256), 0, st, a, 16 * kWaves * p.sub);
+  else
+    hipLaunchKernelGGL((tree_combine_kernel<T, D, 1>), grid, dim3(256), 0, st, a, 16 * kWaves * p.sub);
+}
+
 template <typename T>
 int launch(const TreeArgs& a, const Launch& p, hipStream_t st) {
-  const int64_t units = static_cast<int64_t>(a.n_requests) * a.kv_heads * a.chunks;
-  const int64_t blocks = (units + 7) / 8 * 8 * a.row_blocks;
+  const int64_t blocks = p.whole ? static_cast<int64_t>(a.n_requests) * a.kv_heads * a.row_blocks : kGroups;
   if (blocks > 0x7fffffffLL) return fail(AKV_EINVAL, "akv_tree_attention: batch too large");
   const dim3 grid(static_cast<unsigned>(blocks));
   if (p.d == 64) {
@@ -800,12 +975,11 @@ int launch(const TreeArgs& a, const Launch& p, hipStream_t st) {
     else start<T, 128, 2>(a, grid, st);
   }
   int rc = check_launch("akv_tree_attention");
-  if (rc || a.chunks == 1) return rc;
-  const dim3 merge(static_cast<unsigned>((a.n_tokens * a.q_heads + 3) / 4));
+  if (rc || p.whole) return rc;
   if (p.d == 64)
-    hipLaunchKernelGGL((tree_combine_kernel<T, 64>), merge, dim3(256), 0, st, a);
+    merge<T, 64>(a, p, st);
   else
-    hipLaunchKernelGGL((tree_combine_kernel<T, 128>), merge, dim3(256), 0, st, a);
+    merge<T, 128>(a, p, st);
   return check_launch("akv_tree_attention (combine)");
 }
 
@@ -823,8 +997,7 @@ extern "C" int64_t akv_tree_attention_workspace_bytes(int64_t n_tokens, int32_t 
                                                        int64_t max_new) {
   using namespace akv;
   if (!sizes_ok(n_tokens, n_requests, q_heads, kv_heads, head_dim, max_len, max_new)) return -1;
-  return partial_bytes(plan(n_tokens, n_requests, kv_heads, q_heads / kv_heads, head_dim, max_len, max_new), n_tokens,
-                       q_heads);
+  return partial_bytes(plan(n_tokens, q_heads / kv_heads, head_dim, max_len, max_new), n_tokens, q_heads);
 }
 
 extern "C" int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_buffer,
@@ -862,9 +1035,10 @@ extern "C" int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_s
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_buffer) |
         reinterpret_cast<uintptr_t>(v_buffer) | reinterpret_cast<uintptr_t>(workspace)) & 15) != 0)
     return fail(AKV_EINVAL, "akv_tree_attention: q, K and V rows and the workspace must be 16-byte aligned");
-  if (pool_slots > 0xffffffffLL || n_tokens > 0x7fffffffLL / q_heads || static_cast<int64_t>(n_requests) * kv_heads > 0x7fffffffLL / 4096)
+  if (pool_slots > 0xffffffffLL || (k_stride_slot | v_stride_slot) >> 31 || n_tokens > 0x7fffffffLL / q_heads ||
+      static_cast<int64_t>(n_requests) * kv_heads > 0x7fffffffLL / 4096)
     return fail(AKV_EINVAL, "akv_tree_attention: batch too large");
-  const Launch p = plan(n_tokens, n_requests, kv_heads, q_heads / kv_heads, head_dim, max_len, max_new);
+  const Launch p = plan(n_tokens, q_heads / kv_heads, head_dim, max_len, max_new);
   const int64_t need = partial_bytes(p, n_tokens, q_heads);
   if (workspace_bytes < need)
     return fail(AKV_EINVAL, "akv_tree_attention: workspace holds %lld bytes, needs %lld",
@@ -895,9 +1069,9 @@ extern "C" int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_s
   a.out = out;
   a.o_st = out_stride_t;
   a.o_sh = out_stride_h;
-  a.used = static_cast<int32_t*>(workspace);
-  a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + (n_tokens + 3) / 4 * 16);
-  a.part_ml = a.part_o + static_cast<int64_t>(p.chunks) * n_tokens * q_heads * p.d;
+  a.owner = static_cast<int32_t*>(workspace);
+  a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + owner_bytes(n_tokens, q_heads));
+  a.part_ml = a.part_o + 2ll * kGroups * (16 * kWaves * p.sub) * p.d;
   a.n_tokens = n_tokens;
   a.max_len = max_len;
   a.n_requests = n_requests;
@@ -906,9 +1080,8 @@ extern "C" int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_s
   a.group = q_heads / kv_heads;
   a.head_dim = head_dim;
   a.page_size = page_size;
-  a.chunks = p.chunks;
   a.row_blocks = p.row_blocks;
-  a.heads_last = p.chunks < 8;
+  a.whole = p.whole;
   a.indptr64 = indptr_dtype == AKV_I64;
   a.out_f32 = out_dtype == AKV_F32;
   a.paged = table_stride != 0;

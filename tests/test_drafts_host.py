@@ -57,8 +57,8 @@ def test_tree_attention_refuses_its_own_input_as_output():
 
 def test_tree_workspace_sizes():
     assert attention.tree_workspace_bytes(0, 0, 8, 2, 64, 0, 0) >= 0
-    # a request of one chunk needs no partial results
-    assert attention.tree_workspace_bytes(8, 1, 8, 2, 64, 100, 8) == 32
+    # requests of one workgroup need no partial results
+    assert attention.tree_workspace_bytes(8, 1, 8, 2, 64, 100, 8) == 16
     assert attention.tree_workspace_bytes(8, 1, 8, 2, 64, 20000, 8) > 8 * 8 * 66 * 4
     for sizes in ((8, 1, 8, 2, 60, 100, 8), (8, 1, 8, 2, 136, 100, 8), (8, 1, 8, 3, 64, 100, 8), (-1, 1, 8, 2, 64, 9, 8),
                   (8, 1, 8, 2, 64, -1, 8), (8, 1, 8, 2, 64, 9, -1), (8, 1, 8, 0, 64, 9, 8)):
@@ -124,7 +124,9 @@ def _call(name, **change):
     ("akv_tree_attention", dict(q_stride_h=60), "16-byte aligned"),
     ("akv_tree_attention", dict(v_buffer=_FAKE + 8), "16-byte aligned"),
     ("akv_tree_attention", dict(workspace=_FAKE + 4), "16-byte aligned"),
-    ("akv_tree_attention", dict(workspace_bytes=16), "workspace holds 16 bytes"),
+    ("akv_tree_attention", dict(workspace_bytes=15), "workspace holds 15 bytes"),
+    ("akv_tree_attention", dict(workspace_bytes=1 << 20, max_len=5000), "workspace holds 1048576 bytes"),
+    ("akv_tree_attention", dict(k_stride_slot=1 << 31), "batch too large"),
     ("akv_tree_attention", dict(n_tokens=1 << 40), "batch too large"),
     ("akv_qk_norm_rope", dict(dtype=9), "dtypes must be"),
     ("akv_qk_norm_rope", dict(weight_dtype=9), "dtypes must be"),
