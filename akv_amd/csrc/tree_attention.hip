@@ -35,6 +35,11 @@
 
 #include "common.h"
 
+extern "C" __device__ long long __ockl_wfred_add_i64(long long);
+extern "C" __device__ int __ockl_wfred_max_i32(int);
+extern "C" __device__ int __ockl_wfred_min_i32(int);
+extern "C" __device__ long long __ockl_wfscan_add_i64(long long, bool);
+
 namespace akv {
 namespace {
 
@@ -56,10 +61,12 @@ constexpr int keys_of(int d) { return d == 64 ? 64 : 32; }
 constexpr int kBuffers = 4;
 
 // Workgroups of a launch that shares the keys out: two per CU.
-constexpr int kGroups = 2 * 256;
+constexpr int kGroupsShift = 9, kGroups = 1 << kGroupsShift;
 // What a piece costs beside its tiles (indices, the first tiles' latency, its
 // result), and the least a workgroup is given, in tiles of 64 keys.
 constexpr int kPieceCost = 3, kLeastShare = 2;
+
+constexpr int kWordsKept = 2;  // mask words of a row in LDS: trees of up to 128 tokens
 
 struct TreeArgs {
   const void* q;
@@ -86,7 +93,7 @@ struct TreeArgs {
   int64_t n_tokens, max_len;
   int32_t n_requests, q_heads, kv_heads, group, head_dim, mask_words, page_size;
   int32_t row_blocks;  // whole launch: workgroups that share a request's rows
-  bool indptr64, out_f32, paged, whole;
+  bool indptr64, out_f32, out_vectors, paged, whole;
 };
 
 static __device__ __attribute__((aligned(16))) const uint32_t zero_row[64] = {};
@@ -129,19 +136,31 @@ __device__ __forceinline__ bool not_finite(short bits) {
   return (bits & e) == e;
 }
 
-// Four dims of a token's head, normalised; a weight sum of 0: nothing was seen.
+// Four dims of an output row.
 template <typename T>
-__device__ __forceinline__ void store_row(const TreeArgs& a, int64_t token, int head, int d, f32x4 o, float l) {
-  const int64_t at = token * a.o_st + head * a.o_sh + d;
+__device__ __forceinline__ void store_four(const TreeArgs& a, int64_t at, f32x4 x) {
+  if (a.out_f32) {
+    float* to = static_cast<float*>(a.out) + at;
+    if (a.out_vectors) {
+      *reinterpret_cast<f32x4*>(to) = x;
+      return;
+    }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float x = l == 0.f ? 0.f : o[i] / l;
-    if (a.out_f32)
-      static_cast<float*>(a.out)[at + i] = x;
-    else
-      static_cast<T*>(a.out)[at + i] = static_cast<T>(x);
+    for (int i = 0; i < 4; ++i) to[i] = x[i];
+  } else {
+    T* to = static_cast<T*>(a.out) + at;
+    const typename Vec<T>::x4 y = __builtin_convertvector(x, typename Vec<T>::x4);
+    if (a.out_vectors) {
+      *reinterpret_cast<typename Vec<T>::x4*>(to) = y;
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = y[i];
   }
 }
+
+// 1 / l; a weight sum of 0 (nothing was seen) gives rows of 0.
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 // v_max3_f32 / v_max_f32 without the canonicalising moves around fmaxf of
 // matrix-core results; a NaN score still reaches the output through exp2.
@@ -167,6 +186,13 @@ __device__ __forceinline__ float column_max(float x) {
   const auto r32 = __builtin_amdgcn_permlane32_swap(c, c, false, false);
   const uint32_t c0 = r32[0], c1 = r32[1];
   return max2(__builtin_bit_cast(float, c0), __builtin_bit_cast(float, c1));
+}
+
+// The same value, of which the compiler knows nothing: what is derived from it
+// is not computed ahead of the loops before it, and holds no register there.
+__device__ __forceinline__ int32_t here_only(int32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 // Loads straight into LDS: lane l's bytes go to `to` + 16 l (4 l).  In asm, since
@@ -219,7 +245,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
   __shared__ int32_t s_entry[kWaves][2][64];  // list entries of the waves' keys, kEntryTiles tiles at a time
   __shared__ uint32_t s_dead[2 * kEntryTiles][kQuarters];  // the tiles' keys that no token sees
   __shared__ float s_m[kWaves][kGroupRows], s_l[kWaves][kGroupRows];
-  __shared__ int32_t s_tok[kWaves][kGroupRows];  // the rows' tokens, for the masked quarters
+  __shared__ int64_t s_out[R];  // where the rows go
+  // for the masked quarters: the rows' tokens, first keys and first mask words
+  __shared__ uint64_t s_words[kWaves][kGroupRows][kWordsKept];
+  __shared__ int32_t s_tok[kWaves][kGroupRows], s_start[kWaves][kGroupRows];
   __shared__ int32_t s_odd;                      // V rows held infinities or NaN that some row does not see
   __shared__ uint64_t s_list[kWaves];            // and the keys that did
   static_assert(kWaves * kGroupRows * D * 4 <= sizeof(buffers), "the waves' results fit the tiles");
@@ -256,13 +285,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
       sum += c.units;
       most = max(most, c.rows);
     }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      sum += __shfl_xor(sum, off);
-      most = max(most, __shfl_xor(most, off));
-    }
-    *most_rows = uniform(most);
-    return uniform(sum);
+    *most_rows = uniform(__ockl_wfred_max_i32(most));
+    return uniform(static_cast<int64_t>(__ockl_wfred_add_i64(sum)));
   };
 
   if (gated(a.gate)) return;
@@ -290,28 +314,24 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
     all *= a.kv_heads;
     lane_units = first_units;
     if (all == 0) return;
-    int64_t groups = all / (kLeastShare * 64 / kKeys);
-    groups = groups < 1 ? 1 : groups < kGroups ? groups : kGroups;
-    if (group_id >= groups) return;
-    int64_t x = all * group_id / groups;
-    budget = all * (group_id + 1) / groups - x;
+    // 2^k stretches: all of the workgroups, or as many as get their least share
+    int k = kGroupsShift;
+    while (k > 0 && (static_cast<int64_t>(kLeastShare * 64 / kKeys) << k) > all) --k;
+    if (group_id >> k) return;
+    auto cut = [&](int64_t i) { return (all >> k) * i + (((all & ((1 << k) - 1)) * i) >> k); };  // all * i / 2^k
+    int64_t x = cut(group_id);
+    budget = cut(group_id + 1) - x;
     rb = 0;
     while (x >= sum * a.kv_heads) {
       int32_t unused;
       x -= sum * a.kv_heads;
       sum = sum_of(++rb, &unused);
     }
-    g = static_cast<int>(x / sum);
-    x -= g * sum;
+    for (g = 0; x >= sum; ++g) x -= sum;
     b = 0;
     for (int b0 = 0; b0 < a.n_requests; b0 += 64) {
       const int32_t mine = b0 == 0 ? lane_units : b0 + lane < a.n_requests ? cost_of(b0 + lane, rb).units : 0;
-      int64_t until = mine;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int64_t up = __shfl_up(until, o);
-        if (lane >= o) until += up;
-      }
+      const int64_t until = __ockl_wfscan_add_i64(mine, true);
       const uint64_t past = __builtin_amdgcn_ballot_w64(until > x);
       if (past) {
         const int at = __builtin_ctzll(past);
@@ -344,13 +364,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
       lo = min(lo, s);
       hi_start = max(hi_start, s);
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      lo = min(lo, __shfl_xor(lo, o));
-      hi_start = max(hi_start, __shfl_xor(hi_start, o));
-    }
-    lo = uniform(lo);
-    hi_start = uniform(hi_start);
+    lo = uniform(__ockl_wfred_min_i32(lo));
+    hi_start = uniform(__ockl_wfred_max_i32(hi_start));
   }
   // the piece: units [off, stop) of the request's, the first kPieceCost of them
   // for no tile, the others for equal parts of its tiles
@@ -463,7 +478,6 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
     for (int s = 0; s < SUB; ++s) {
       const int r = min(row0 + 16 * s + col, rows - 1);
       const int tok = r / a.group;
-      s_tok[wave][16 * s + col] = tok;
       const T* row = static_cast<const T*>(a.q) + (q0 + tok) * a.q_st +
                      static_cast<int64_t>(g * a.group + r - tok * a.group) * a.q_sh;
 #pragma unroll
@@ -488,16 +502,19 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = static_cast<T>(1.f);
 
-    // what a token sees of the 32 keys from k0 on
-    auto visible = [&](int tok, int k0) -> uint32_t {
+    // word w of a token's mask row
+    auto mask_word = [&](int tok, int w) -> uint64_t {
+      if (a.mask) return w < a.mask_words ? a.mask[(q0 + tok) * a.mask_stride + w] : 0;
+      const int i = tok - 64 * w;
+      return i >= 63 ? ~0ull : i < 0 ? 0 : (2ull << i) - 1;
+    };
+    auto start_of = [&](int tok) -> int { return a.key_starts ? min(max(a.key_starts[q0 + tok], 0), old) : 0; };
+    // what a row sees of the 32 keys from k0 on: those from `start` on, and the
+    // drafted ones by its words
+    auto visible = [&](int k0, int start, auto word) -> uint32_t {
       const int base = k0 - old;
       uint64_t bits = ~0ull;
       if (base > -32) {
-        auto word = [&](int w) -> uint64_t {
-          if (a.mask) return w < a.mask_words ? a.mask[(q0 + tok) * a.mask_stride + w] : 0;
-          const int i = tok - 64 * w;
-          return i >= 63 ? ~0ull : i < 0 ? 0 : (2ull << i) - 1;
-        };
         if (base < 0) {
           bits = word(0) << -base | ((1ull << -base) - 1);
         } else {
@@ -506,12 +523,17 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
           if (by > 32) bits |= word(w + 1) << (64 - by);
         }
       }
-      if (a.key_starts) {
-        const int hidden = min(max(a.key_starts[q0 + tok], 0), old) - k0;
-        if (hidden >= 32) bits = 0; else if (hidden > 0) bits &= ~0ull << hidden;
-      }
+      const int hidden = start - k0;
+      if (hidden >= 32) bits = 0; else if (hidden > 0) bits &= ~0ull << hidden;
       return static_cast<uint32_t>(bits);
     };
+    if (lane < kGroupRows) {
+      const int tok = min(row0 + lane, rows - 1) / a.group;
+      s_tok[wave][lane] = tok;
+      s_start[wave][lane] = start_of(tok);
+#pragma unroll
+      for (int w = 0; w < kWordsKept; ++w) s_words[wave][lane][w] = mask_word(tok, w);
+    }
     // A weight of 0 does not hide an infinity or NaN from the product.  Where
     // rows see different keys such values are cleared (by every wave that uses
     // them) and the block takes note: its rows get them back at the end.
@@ -606,7 +628,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
       if (masked) {
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
-          const uint32_t seen = visible(s_tok[wave][16 * s + col], k0) & ~dead;
+          const int in = 16 * s + col;
+          const uint32_t seen = ~dead & visible(k0, s_start[wave][in], [&](int w) -> uint64_t {
+            return w < kWordsKept ? s_words[wave][in][w] : mask_word(s_tok[wave][in], w);
+          });
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -722,42 +747,56 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
     const int64_t place = 2 * group_id + (first ? 1 : 0);
     float* part = a.part_o + place * R * D;
     float* part_ml = a.part_ml + place * R * 2;
-    for (int u = threadIdx.x; u < here * (D / 4); u += kThreads) {
-      const int r = u / (D / 4), d = 4 * (u % (D / 4));
-      if (NARROW && d >= a.head_dim) continue;
-      const int token = (rb * R + r) / a.group, head = g * a.group + rb * R + r - token * a.group;
-      const int group = r / kGroupRows, in = r % kGroupRows;
+    // a thread per row: the sharers' factors, with the sink and the sum when the
+    // piece is all of it
+    const int mine = here_only(threadIdx.x);
+    if (mine < here) {
+      const int r = rb * R + mine, token = r / a.group, head = g * a.group + r - token * a.group;
+      const int64_t row = q0 + token;
+      const int group = mine / kGroupRows, in = mine % kGroupRows;
       float m = -INFINITY, lt = 0.f;
-      f32x4 o = {0.f, 0.f, 0.f, 0.f};
       for (int w = group; w < kWaves; w += groups) m = fmaxf(m, s_m[w][in]);
       // a wave that has seen no key carries m = -inf, l = 0 and O = 0
-      const float base = m == -INFINITY ? 0.f : m;
-      for (int w = group; w < kWaves; w += groups) {
-        const float by = __builtin_amdgcn_exp2f(s_m[w][in] - base);
-        lt += s_l[w][in] * by;
-        o += *reinterpret_cast<const f32x4*>(result_of(w) + in * D + (d ^ (in & 7) << 2)) * by;
+      float base = m == -INFINITY ? 0.f : m;
+      for (int w = group; w < kWaves; w += groups) lt += s_l[w][in] * __builtin_amdgcn_exp2f(s_m[w][in] - base);
+      float scale = 1.f;
+      if (first && last) {
+        if (a.sinks) {
+          const float sink = a.sinks[head] * kLog2e, top = fmaxf(m, sink);
+          const float by = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+          lt = lt * by + (top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - top));
+          scale = by;
+        }
+        scale *= inverse(lt);
+        s_out[mine] = row * a.o_st + head * a.o_sh;
+      } else {
+        *reinterpret_cast<f32x2*>(part_ml + 2 * mine) = f32x2{m, lt};
       }
-      if (!a.whole && d == 0) {
-        int32_t* owner = a.owner + 4 * ((q0 + token) * a.q_heads + head);
+      for (int w = group; w < kWaves; w += groups) s_m[w][in] = __builtin_amdgcn_exp2f(s_m[w][in] - base) * scale;
+      if (!a.whole) {
+        int32_t* owner = a.owner + 4 * (row * a.q_heads + head);
         if (first) {
           owner[0] = last ? -1 : group_id;
-          owner[2] = r;
+          owner[2] = mine;
         }
         if (last) owner[1] = group_id;
       }
-      if (!(first && last)) {
-        *reinterpret_cast<f32x4*>(part + r * D + d) = o;
-        if (d == 0) *reinterpret_cast<f32x2*>(part_ml + 2 * r) = f32x2{m, lt};
-        continue;
+    }
+    __syncthreads();
+    constexpr int kRowsAtOnce = kThreads / (D / 4);
+    const int d = 4 * (mine % (D / 4));
+    if (!NARROW || d < a.head_dim) {
+#pragma unroll 2
+      for (int r = mine / (D / 4); r < here; r += kRowsAtOnce) {
+        const int group = r / kGroupRows, in = r % kGroupRows;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int w = group; w < kWaves; w += groups)
+          o += *reinterpret_cast<const f32x4*>(result_of(w) + in * D + (d ^ (in & 7) << 2)) * s_m[w][in];
+        if (first && last)
+          store_four<T>(a, s_out[r] + d, o);
+        else
+          *reinterpret_cast<f32x4*>(part + r * D + d) = o;
       }
-      if (a.sinks) {
-        const float sink = a.sinks[head] * kLog2e;
-        const float mt = fmaxf(m, sink);
-        const float by = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mt);
-        o *= by;
-        lt = lt * by + (mt == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - mt));
-      }
-      store_row<T>(a, q0 + token, head, d, o, lt);
     }
     // values cleared from the products go back, unweighted, to the rows that see
     // them: whatever their weights, the results are the infinity or NaN
@@ -769,8 +808,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
           const uint64_t slot = static_cast<uint64_t>(list[at]) * per + (static_cast<uint32_t>(j) - at * per);
           return slot < static_cast<uint64_t>(a.pool_slots) ? reinterpret_cast<const T*>(vbase + slot * v_ss) : nullptr;
         };
-        const int mine = base + static_cast<int>(threadIdx.x);
-        const T* row = mine < end ? v_row(mine) : nullptr;
+        const int key = base + static_cast<int>(threadIdx.x);
+        const T* row = key < end ? v_row(key) : nullptr;
         bool odd = false;
         for (int d = 0; row && d < a.head_dim; ++d) odd |= not_finite<T>(__builtin_bit_cast(short, row[d]));
         const uint64_t odds = __builtin_amdgcn_ballot_w64(odd);
@@ -783,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
           for (int w = 0; w < kWaves; ++w)
             for (uint64_t rest = s_list[w]; rest; rest &= rest - 1) {
               const int j = base + 64 * w + __builtin_ctzll(rest);
-              if (!(visible(token, j) & 1)) continue;
+              if (!(visible(j, start_of(token), [&](int w) { return mask_word(token, w); }) & 1)) continue;
               const T* v = v_row(j) + d;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -894,7 +933,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a, con
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], off);
   }
   if (a.sinks) l += __builtin_amdgcn_exp2f(sink - base);
-  if (way == 0 && d < a.head_dim) store_row<T>(a, token, head, d, o, l);
+  if (way == 0 && d < a.head_dim) store_four<T>(a, token * a.o_st + head * a.o_sh + d, o * inverse(l));
 }
 
 int tile_dim(int32_t head_dim) { return head_dim <= 64 ? 64 : 128; }
@@ -1084,6 +1123,8 @@ extern "C" int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_s
   a.whole = p.whole;
   a.indptr64 = indptr_dtype == AKV_I64;
   a.out_f32 = out_dtype == AKV_F32;
+  a.out_vectors = (out_stride_t | out_stride_h) % 4 == 0 &&
+                  reinterpret_cast<uintptr_t>(out) % (out_dtype == AKV_F32 ? 16 : 8) == 0;
   a.paged = table_stride != 0;
   hipStream_t st = as_stream(stream);
   if (dtype == AKV_F16) return launch<_Float16>(a, p, st);
