@@ -13,10 +13,11 @@
 //
 // The n tokens x G heads of a KV head's group are the rows of one product with
 // that head's keys, so K and V are read once for a block of 64 SUB rows, and
-// again for every further one.  Workgroup = (chunk of keys, KV head, request,
-// block of rows), four waves, two workgroups per CU.  Tiles of K and V stream
-// into LDS (global_load_lds, two buffers) while the one before is worked on, in
-// 32-key quarters, 16 SUB rows per wave:
+// again for every further one.  All the batch's tiles of keys lie on a line, and
+// 512 workgroups of four waves, two per CU, take equal stretches of it; where a
+// cut falls among a request's tiles, a second launch merges the parts.  Tiles of
+// K and V stream into LDS (two places) while the one before is worked on, 32 keys
+// (a quarter of a tile at D = 64) at a time, 16 SUB rows per wave:
 //   S^T[32 x 16 SUB] = K . Q^T              v_mfma_f32_16x16x32
 //   P^T = 2^(scale log2(e) S^T - m)         in the storage type
 //   l += 1^T . P^T,  O^T[D x 16 SUB] += V^T . P^T
@@ -24,7 +25,7 @@
 // each group of rows: they take the quarters in turn and meet at the end.
 // P^T leaves the first product in the operand layout of the second; V^T comes
 // through ds_read_b64_tr_b16.  m is a row's first maximum and moves only when the
-// weights outgrow their types.  A second launch merges the chunks and the sink.
+// weights outgrow their types.
 //
 // Lane layouts (verified on gfx950): v_mfma_f32_16x16x32 -- lane l supplies
 // A[l%16][k(l,i)], B[k(l,i)][l%16] for i < 8 and holds D[4(l/16)+i][l%16];
@@ -56,9 +57,11 @@ constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHuge = 18446744073709551616.f;  // 2^64: a weight sum above it may have overflowed the product
 
-// Keys of a tile and the tiles in LDS: one is worked on while the next stream in.
-constexpr int keys_of(int d) { return d == 64 ? 64 : 32; }
-constexpr int kBuffers = 4;
+// Keys of a tile (32 KiB of K and V), and the tiles in LDS: one is worked on while
+// the next streams in.  (Four places for half the keys, with three tiles on their
+// way, took 2-8% longer: a barrier and the loads' addresses for every 64 keys.)
+constexpr int keys_of(int d) { return d == 64 ? 128 : 64; }
+constexpr int kBuffers = 2;
 
 // Workgroups of a launch that shares the keys out: two per CU.
 constexpr int kGroupsShift = 9, kGroups = 1 << kGroupsShift;
@@ -197,7 +200,7 @@ __device__ __forceinline__ int32_t here_only(int32_t v) {
 
 // Loads straight into LDS: lane l's bytes go to `to` + 16 l (4 l).  In asm, since
 // the compiler takes every later LDS read for one that may meet them and waits
-// for all of them; here arrive() does the waiting.  (Nothing else in these kernels
+// for all of them; arrive() does the waiting.  (Nothing else in these kernels
 // uses m0.)
 __device__ __forceinline__ void load_16(const void* from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
@@ -206,16 +209,12 @@ __device__ __forceinline__ void load_4(const void* from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(to) : "memory");
 }
 
-// Waits for this wave's loads but its last N, and for its LDS accesses, then for
-// the other waves.
-template <int N>
-__device__ __forceinline__ void wait_and_meet() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
-
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)p));
 }
+
+// Waits for this wave's loads and LDS accesses, then for the other waves.
+__device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int D>
 struct alignas(16) TileLds {
@@ -236,9 +235,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
   constexpr int kChunks = D / 8;             // 16-byte chunks of a row
   constexpr int kLoadRows = 64 / kChunks;    // rows of one wave-wide load
   constexpr int kWaveKeys = kKeys / kWaves;  // keys of a tile that a wave asks for
-  constexpr int kLoads = 2 * kWaveKeys / kLoadRows;  // a wave's loads of a tile
   constexpr int kEntryTiles = 64 / kWaveKeys;  // tiles whose keys of this wave fill a vector register
-  constexpr int kOver = kPieceCost * 64 / kKeys;
+  constexpr int kOver = (kPieceCost * 64 + kKeys - 1) / kKeys;
   constexpr int kGroupRows = 16 * SUB;       // rows of a wave
   constexpr int R = kWaves * kGroupRows;     // rows of a block
   __shared__ TileLds<D> buffers[kBuffers];
@@ -316,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
     if (all == 0) return;
     // 2^k stretches: all of the workgroups, or as many as get their least share
     int k = kGroupsShift;
-    while (k > 0 && (static_cast<int64_t>(kLeastShare * 64 / kKeys) << k) > all) --k;
+    while (k > 0 && (static_cast<int64_t>((kLeastShare * 64 + kKeys - 1) / kKeys) << k) > all) --k;
     if (group_id >> k) return;
     auto cut = [&](int64_t i) { return (all >> k) * i + (((all & ((1 << k) - 1)) * i) >> k); };  // all * i / 2^k
     int64_t x = cut(group_id);
@@ -418,10 +416,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
     if (lane < kEntryTiles) {
       const uint32_t mine = static_cast<uint32_t>(dead >> (kWaveKeys * lane));
       char* to = reinterpret_cast<char*>(s_dead[(e & 1) * kEntryTiles + lane]) + kWaveKeys / 8 * wave;
-      if constexpr (kWaveKeys == 16)
-        *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(mine);
+      if constexpr (kWaveKeys == 32)
+        *reinterpret_cast<uint32_t*>(to) = mine;
       else
-        *reinterpret_cast<uint8_t*>(to) = static_cast<uint8_t>(mine);
+        *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(mine);
     }
   };
   // a wave's keys of a tile, straight into LDS: lane l of a load fills bytes
@@ -448,18 +446,6 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
       load_16(vrow, uniform(lds_address(t.v + place)));
     }
   };
-  // the oldest tile asked for is here, with `newer` tiles asked for behind it
-  // (with list entries among them, a load or two more is waited for)
-  auto arrive = [&](int newer) {
-    static_assert(kBuffers == 4, "the waits");
-    if (newer >= 2)
-      wait_and_meet<2 * kLoads>();
-    else if (newer == 1)
-      wait_and_meet<kLoads>();
-    else
-      wait_and_meet<0>();
-  };
-
   {
     if (tiles > 0) fetch(0);
     if (threadIdx.x == 0) s_odd = 0;
@@ -691,10 +677,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
     };
     __builtin_amdgcn_s_waitcnt(0);  // (one the compiler sees: Q has arrived)
     __syncthreads();
-#pragma unroll
-    for (int it = 0; it < kBuffers - 1; ++it)
-      if (it < tiles) stage(it);
-    arrive(tiles - 1);
+    if (tiles > 0) stage(0);
+    arrive();
     // this wave's quarters of a tile
     uint32_t quarters = 0;
 #pragma unroll
@@ -702,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
 #pragma nounroll
     for (int it = 0; it < tiles; ++it) {
       // into the place that was last read before the barrier
-      if (it + kBuffers - 1 < tiles) stage(it + kBuffers - 1);
+      if (it + 1 < tiles) stage(it + 1);
       TileLds<D>& t = buffers[it % kBuffers];
       const int t0 = begin + it * kKeys;
       const uint32_t* dead = s_dead[it % (2 * kEntryTiles)];
@@ -721,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
         if (k0 >= end) break;
         quarter(t, kk, k0, uniform(dead[kk]));
       }
-      arrive(tiles - 2 - it);
+      arrive();
     }
 
     // the waves' O rows [row][dim] over the tiles, four-float groups turned by
@@ -939,7 +923,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a, con
 int tile_dim(int32_t head_dim) { return head_dim <= 64 ? 64 : 128; }
 
 // A wave's row subtiles for requests of up to `rows` rows: a tile has keys for
-// two waves (one at D = 128) to share a group of rows, so the rows are dealt out
+// four waves (two at D = 128) to share a group of rows, so the rows are dealt out
 // to two (four) groups before a wave takes more of them.
 int subtiles_for(int d, int64_t rows) {
   const int most = d == 64 ? 4 : 2;
