@@ -101,66 +101,73 @@ def tree_attention(q, k_buffer, v_buffer, qo_indptr, kv_indptr, kv_indices, out,
     ``out`` behind the last token stay as they are.  Head dims: multiples of 8
     up to 128.  ``status``: as for ``decode_attention``.
     """
-    if q.dtype not in (torch.bfloat16, torch.float16) or q.ndim != 3 or q.stride(2) != 1:
+    # one read of every property: the checks are most of a small call's time
+    dtype, at, q_shape, q_stride = q.dtype, q.get_device(), q.shape, q.stride()
+    if dtype not in (torch.bfloat16, torch.float16) or len(q_shape) != 3 or q_stride[2] != 1:
         raise ValueError("q must be bf16 or fp16 [tokens, q_heads, head_dim] with unit dim stride")
-    device, dtype = q.device, q.dtype
-    n, hq, d = q.shape
-    if k_buffer.ndim != 3 or v_buffer.shape != k_buffer.shape or k_buffer.shape[2] != d or k_buffer.dtype != dtype \
-            or v_buffer.dtype != dtype or k_buffer.stride(2) != 1 or v_buffer.stride(2) != 1:
+    n, hq, d = q_shape
+    pool, k_stride, v_stride = k_buffer.shape, k_buffer.stride(), v_buffer.stride()
+    if len(pool) != 3 or v_buffer.shape != pool or pool[2] != d or k_buffer.dtype != dtype \
+            or v_buffer.dtype != dtype or k_stride[2] != 1 or v_stride[2] != 1:
         raise ValueError("K/V must be matching [slots, kv_heads, head_dim] buffers of q's dtype and head_dim")
-    if out.shape != q.shape or out.dtype not in (dtype, torch.float32) or out.stride(2) != 1:
+    out_dtype, out_stride = out.dtype, out.stride()
+    if out.shape != q_shape or (out_dtype != dtype and out_dtype != torch.float32) or out_stride[2] != 1:
         raise ValueError("out must be shaped like q, of its dtype or f32")
-    if out.data_ptr() == q.data_ptr() and n:
+    q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
+    if out_ptr == q_ptr and n:
         raise ValueError("out must not be q")
-    if qo_indptr.dtype not in _INDEX or kv_indptr.dtype != qo_indptr.dtype or qo_indptr.ndim != 1 \
-            or kv_indptr.shape != qo_indptr.shape or not qo_indptr.is_contiguous() or not kv_indptr.is_contiguous():
+    indptr_t = _INDEX.get(qo_indptr.dtype)
+    n_requests = qo_indptr.numel() - 1
+    if indptr_t is None or kv_indptr.dtype != qo_indptr.dtype or qo_indptr.ndim != 1 or kv_indptr.ndim != 1 \
+            or kv_indptr.numel() != n_requests + 1 or not qo_indptr.is_contiguous() or not kv_indptr.is_contiguous():
         raise ValueError("qo_indptr and kv_indptr must be contiguous [requests + 1] of one int32/int64 dtype")
-    n_requests = qo_indptr.shape[0] - 1
-    if kv_indices.dtype != torch.int32 or kv_indices.ndim not in (1, 2) or (kv_indices.numel() and
-                                                                            kv_indices.stride(-1) != 1):
+    list_shape, list_stride = kv_indices.shape, kv_indices.stride()
+    if kv_indices.dtype != torch.int32 or len(list_shape) not in (1, 2) or (list_stride[-1] != 1 and kv_indices.numel()):
         raise ValueError("kv_indices must be int32: a list of slots or a block table [requests, pages]")
-    if kv_indices.ndim == 2:
-        width = kv_indices.shape[1]
-        stride = kv_indices.stride(0) if n_requests > 1 else max(1, width)
-        if kv_indices.shape[0] != n_requests or stride < max(1, width):
+    width, stride = list_shape[-1], 0
+    if len(list_shape) == 2:
+        stride = list_stride[0] if n_requests > 1 else max(1, width)
+        if list_shape[0] != n_requests or stride < max(1, width):
             raise ValueError("the block table needs a row per request, without overlap")
-    else:
-        if page_size != 1:
-            raise ValueError("pages need a block table")
-        width, stride = kv_indices.shape[0], 0
-    if tree_mask is not None and (tree_mask.dtype != torch.int64 or tree_mask.ndim != 2 or tree_mask.shape[0] != n
-                                  or (tree_mask.numel() and tree_mask.stride(1) != 1) or tree_mask.device != device):
-        raise ValueError("tree_mask must be int64 words [tokens, words] on q's device")
-    if key_starts is not None and (key_starts.dtype != torch.int32 or key_starts.shape != (n,)
-                                   or not key_starts.is_contiguous() or key_starts.device != device):
+    elif page_size != 1:
+        raise ValueError("pages need a block table")
+    mask_args = (None, 0, 0)
+    if tree_mask is not None:
+        mask_shape, mask_stride = tree_mask.shape, tree_mask.stride()
+        if tree_mask.dtype != torch.int64 or len(mask_shape) != 2 or mask_shape[0] != n \
+                or (mask_stride[1] != 1 and tree_mask.numel()) or tree_mask.get_device() != at:
+            raise ValueError("tree_mask must be int64 words [tokens, words] on q's device")
+        mask_args = (tree_mask.data_ptr(), mask_stride[0], mask_shape[1])
+    if key_starts is not None and (key_starts.dtype != torch.int32 or key_starts.ndim != 1 or key_starts.numel() != n
+                                   or not key_starts.is_contiguous() or key_starts.get_device() != at):
         raise ValueError("key_starts must be contiguous int32 [tokens] on q's device")
-    if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (hq,) or not sinks.is_contiguous()
-                              or sinks.device != device):
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.ndim != 1 or sinks.numel() != hq
+                              or not sinks.is_contiguous() or sinks.get_device() != at):
         raise ValueError("sinks must be f32 [q_heads] on q's device")
-    if status is not None and (status.dtype != torch.int32 or status.numel() < 1 or status.device != device):
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1 or status.get_device() != at):
         raise ValueError("status must be an int32 device word on q's device")
-    if device.type != "cuda" or not (k_buffer.device == v_buffer.device == out.device == qo_indptr.device
-                                     == kv_indptr.device == kv_indices.device == device):
+    if at < 0 or not (k_buffer.get_device() == v_buffer.get_device() == out.get_device() == qo_indptr.get_device()
+                      == kv_indptr.get_device() == kv_indices.get_device() == at):
         raise ValueError("tree attention's tensors must be on one GPU")
     if n == 0 or n_requests <= 0:
         return out
-    hk = k_buffer.shape[1]
+    device, hk = q.device, pool[1]
     lib = _lib.calls()
     if workspace is None:
         need = lib.akv_tree_attention_workspace_bytes(n, n_requests, hq, hk, d, int(max_len), int(max_new))
         workspace = torch.empty(max(16, need), dtype=torch.uint8, device=device)
-    elif workspace.device != device or not workspace.is_contiguous():
+    elif workspace.get_device() != at or not workspace.is_contiguous():
         raise ValueError("the workspace must be contiguous, on q's device")
     with _on_device(device):
         rc = lib.akv_tree_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), k_buffer.data_ptr(), v_buffer.data_ptr(), k_buffer.stride(0),
-            k_buffer.stride(1), v_buffer.stride(0), v_buffer.stride(1), k_buffer.shape[0], _TREE_DTYPES[dtype], n,
-            n_requests, hq, hk, d, qo_indptr.data_ptr(), kv_indptr.data_ptr(), _INDEX[qo_indptr.dtype],
-            kv_indices.data_ptr(), stride, width, int(page_size), _lib.ptr(tree_mask),
-            0 if tree_mask is None else tree_mask.stride(0), 0 if tree_mask is None else tree_mask.shape[1],
-            _lib.ptr(key_starts), _lib.ptr(sinks), float(scale), out.data_ptr(), _TREE_DTYPES[out.dtype],
-            out.stride(0), out.stride(1), int(max_len), int(max_new), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _lib.ptr(status), current_stream_handle(device),
+            q_ptr, q_stride[0], q_stride[1], k_buffer.data_ptr(), v_buffer.data_ptr(), k_stride[0], k_stride[1],
+            v_stride[0], v_stride[1], pool[0], _TREE_DTYPES[dtype], n, n_requests, hq, hk, d, qo_indptr.data_ptr(),
+            kv_indptr.data_ptr(), indptr_t, kv_indices.data_ptr(), stride, width, int(page_size), *mask_args,
+            None if key_starts is None else key_starts.data_ptr(), None if sinks is None else sinks.data_ptr(),
+            float(scale), out_ptr, _TREE_DTYPES[out_dtype], out_stride[0], out_stride[1], int(max_len), int(max_new),
+            workspace.data_ptr(), workspace.nbytes, None if status is None else status.data_ptr(),
+            current_stream_handle(device),
         )
-    _lib.check(rc, "akv_tree_attention")
+    if rc:
+        _lib.check(rc, "akv_tree_attention")
     return out

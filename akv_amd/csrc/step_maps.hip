@@ -136,6 +136,7 @@ __device__ __forceinline__ uint64_t bits_of(int64_t lo, int64_t hi, int64_t w) {
 
 __device__ __forceinline__ void token_maps(const MapArgs& a, int b) {
   __shared__ int32_t staged[kStagedParents];
+  __shared__ int64_t keys[kThreads];  // positions from the first key inside a root's window on
   const Request r = request_of(a, b);
   int64_t len0, tok0;
   sums_before(a, b, &len0, &tok0);
@@ -165,9 +166,12 @@ __device__ __forceinline__ void token_maps(const MapArgs& a, int b) {
   };
   const int64_t root = r.pos_of(old);
   int64_t first = 0;  // first key inside the window of a token of depth 0
-  if (a.window_starts && r.raw_ids)
+  if (a.window_starts && r.raw_ids) {
     first = first_at_least([&](int32_t i) -> int64_t { return r.pos_of(i); }, static_cast<int32_t>(old),
                            root - a.window, lane);
+    if (first + tid < old) keys[tid] = r.pos_of(first + tid);
+    __syncthreads();
+  }
   for (int64_t i = begin + tid; i < n; i += static_cast<int64_t>(a.token_blocks) * kThreads) {
     const int64_t t = tok0 + i;
     store_index(a.slot_map, a.slots64, t, r.slot_at(r.raw_of(old + i)));
@@ -213,7 +217,8 @@ __device__ __forceinline__ void token_maps(const MapArgs& a, int b) {
         int64_t hi = first + depth < old ? first + depth : old;
         while (lo < hi) {
           const int64_t mid = (lo + hi) >> 1;
-          if (r.pos_of(mid) < lower) lo = mid + 1; else hi = mid;
+          const int64_t at = mid - first < kThreads ? keys[mid - first] : r.pos_of(mid);
+          if (at < lower) lo = mid + 1; else hi = mid;
         }
       }
       a.window_starts[t] = static_cast<int32_t>(lo);

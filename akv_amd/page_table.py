@@ -191,9 +191,12 @@ def context_step_maps(registry, table, rows, seq_lens, new_lens, qo_indptr, kv_i
     as do the indptrs; a mask has a word per 64 new tokens of a request.
     ``status``: as for ``context_decode_indices``.
     """
+    # one read of every property: the checks are most of the call's time
+    at = slot_map.get_device()
     if registry.dtype != torch.int64 or registry.ndim != 2 or registry.shape[1] != 6 or not registry.is_contiguous():
         raise ValueError("registry must be contiguous int64 [rows, 6]")
-    if table.dtype != torch.int32 or table.ndim != 2 or table.stride(1) != 1:
+    table_shape, table_stride = table.shape, table.stride()
+    if table.dtype != torch.int32 or len(table_shape) != 2 or table_stride[1] != 1:
         raise ValueError("the request table must be int32 [rows, width] with unit column stride")
     batch = seq_lens.numel()
     if new_lens.dtype != seq_lens.dtype or new_lens.numel() != batch or rows.numel() != batch:
@@ -210,43 +213,47 @@ def context_step_maps(registry, table, rows, seq_lens, new_lens, qo_indptr, kv_i
     n = slot_map.numel()
     if positions.numel() != n:
         raise ValueError("slot_map and positions must have one entry per token")
-    device = slot_map.device
-    tensors = [registry, table, rows, seq_lens, new_lens, qo_indptr, kv_indptr, positions]
-    block_p, block_stride, block_width = None, 0, 0
+    one_device = at >= 0 and (at == registry.get_device() == table.get_device() == rows.get_device()
+                              == seq_lens.get_device() == new_lens.get_device() == qo_indptr.get_device()
+                              == kv_indptr.get_device() == positions.get_device())
+    block_args = (None, 0, 0)
     if block_tables is not None:
-        if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.shape[0] != batch \
-                or (block_tables.numel() and block_tables.stride(1) != 1) \
-                or (batch > 1 and block_tables.stride(0) < block_tables.shape[1]):
+        shape, stride = block_tables.shape, block_tables.stride()
+        if block_tables.dtype != torch.int32 or len(shape) != 2 or shape[0] != batch \
+                or (stride[1] != 1 and block_tables.numel()) or (batch > 1 and stride[0] < shape[1]):
             raise ValueError("block_tables must be int32 [requests, pages] with unit column stride, without overlap")
-        block_p, block_stride, block_width = block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1]
-        tensors.append(block_tables)
+        block_args = (block_tables.data_ptr(), stride[0], shape[1])
+        one_device &= block_tables.get_device() == at
     if parents is not None:
         if parents.dtype != torch.int32 or parents.numel() != n or not parents.is_contiguous():
             raise ValueError("parents must be contiguous int32 with one entry per token")
-        tensors.append(parents)
-    if (window_mask is not None or window_starts is not None) and window is None:
+        one_device &= parents.get_device() == at
+    if window is None and (window_mask is not None or window_starts is not None):
         raise ValueError("window_mask and window_starts need a window")
-    masks = []
-    for mask in (tree_mask, window_mask):
+    mask_args = [(None, 0, 0), (None, 0, 0)]
+    for i, mask in enumerate((tree_mask, window_mask)):
         if mask is None:
-            masks.append((None, 0, 0))
             continue
-        if mask.dtype != torch.int64 or mask.ndim != 2 or mask.shape[0] != n \
-                or (mask.numel() and mask.stride(1) != 1) or (n > 1 and mask.stride(0) < mask.shape[1]):
+        shape, stride = mask.shape, mask.stride()
+        if mask.dtype != torch.int64 or len(shape) != 2 or shape[0] != n or (stride[1] != 1 and mask.numel()) \
+                or (n > 1 and stride[0] < shape[1]):
             raise ValueError("masks must be int64 words [tokens, words] with unit word stride, without overlap")
-        masks.append((mask.data_ptr(), mask.stride(0), mask.shape[1]))
-        tensors.append(mask)
+        mask_args[i] = (mask.data_ptr(), stride[0], shape[1])
+        one_device &= mask.get_device() == at
     if window_starts is not None:
         if window_starts.dtype != torch.int32 or window_starts.numel() != n or not window_starts.is_contiguous():
             raise ValueError("window_starts must be contiguous int32 with one entry per token")
-        tensors.append(window_starts)
-    if device.type != "cuda" or any(t.device != device for t in tensors):
+        one_device &= window_starts.get_device() == at
+    if not one_device:
         raise ValueError("step maps' tensors must be on one GPU")
+    device = slot_map.device
     with _on_device(device):
         rc = _lib.calls().akv_step_maps(
-            registry.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], rows_p, rows_t, seq_p, new_p,
-            len_t, batch, qo_p, kv_p, ind_t, n, slot_p, slot_t, pos_p, pos_t, block_p, block_stride, block_width,
-            int(page_size), _lib.ptr(parents), *masks[0], 0 if window is None else int(window), *masks[1],
-            _lib.ptr(window_starts), _status_ptr(status, device), current_stream_handle(device),
+            registry.data_ptr(), table.data_ptr(), table_stride[0], table_shape[1], rows_p, rows_t, seq_p, new_p,
+            len_t, batch, qo_p, kv_p, ind_t, n, slot_p, slot_t, pos_p, pos_t, *block_args, int(page_size),
+            None if parents is None else parents.data_ptr(), *mask_args[0], 0 if window is None else int(window),
+            *mask_args[1], None if window_starts is None else window_starts.data_ptr(), _status_ptr(status, device),
+            current_stream_handle(device),
         )
-    _lib.check(rc, "akv_step_maps")
+    if rc:
+        _lib.check(rc, "akv_step_maps")

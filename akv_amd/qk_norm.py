@@ -35,67 +35,83 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, positions, cos_sin_cache, q_out, *
     are 16-byte aligned, with D and rotary_dim multiples of 16, take the
     vector kernel.
     """
-    device, dtype = q.device, q.dtype
+    # one read of every property: the checks are most of a small call's time
+    dtype, at = q.dtype, q.get_device()
     if dtype not in _KV_DTYPES:
         raise ValueError("q, k and v must be float32, float16 or bfloat16")
-    if q.ndim != 3 or k.ndim != 3 or q.stride(2) != 1 or k.stride(2) != 1:
+    q_shape, k_shape, q_stride, k_stride = q.shape, k.shape, q.stride(), k.stride()
+    if len(q_shape) != 3 or len(k_shape) != 3 or q_stride[2] != 1 or k_stride[2] != 1:
         raise ValueError("q and k must be [tokens, heads, head_dim] with unit dim stride")
-    n, hq, d = q.shape
-    hk = k.shape[1]
-    if k.dtype != dtype or k.device != device or k.shape[0] != n or k.shape[2] != d:
+    n, hq, d = q_shape
+    hk = k_shape[1]
+    if k.dtype != dtype or k.get_device() != at or k_shape[0] != n or k_shape[2] != d:
         raise ValueError("q and k must share tokens, head_dim, dtype and device")
-    if q_out.shape != q.shape or q_out.dtype != dtype or q_out.device != device or q_out.stride(2) != 1:
+    out_stride = q_out.stride()
+    if q_out.shape != q_shape or q_out.dtype != dtype or q_out.get_device() != at or out_stride[2] != 1:
         raise ValueError("q_out must be shaped like q, of its dtype and device")
-    if k_out is not None and (k_out.shape != k.shape or k_out.dtype != dtype or k_out.device != device
-                              or k_out.stride(2) != 1):
-        raise ValueError("k_out must be shaped like k, of its dtype and device")
+    k_out_args = (None, 0, 0)
+    if k_out is not None:
+        stride = k_out.stride()
+        if k_out.shape != k_shape or k_out.dtype != dtype or k_out.get_device() != at or stride[2] != 1:
+            raise ValueError("k_out must be shaped like k, of its dtype and device")
+        k_out_args = (k_out.data_ptr(), stride[0], stride[1])
     weight = q_weight if q_weight is not None else k_weight
+    weight_dtype = torch.float32 if weight is None else weight.dtype
     for w in (q_weight, k_weight):
-        if w is not None and (w.shape != (d,) or w.dtype != weight.dtype or w.dtype not in _KV_DTYPES
-                              or w.device != device or not w.is_contiguous()):
+        if w is not None and (w.dtype != weight_dtype or w.dtype not in _KV_DTYPES or w.get_device() != at
+                              or w.ndim != 1 or w.numel() != d or not w.is_contiguous()):
             raise ValueError("norm weights must be contiguous [head_dim] vectors of one floating-point dtype")
-    if positions.dtype not in _INDEX or positions.shape != (n,) or positions.device != device \
+    positions_t = _INDEX.get(positions.dtype)
+    if positions_t is None or positions.ndim != 1 or positions.numel() != n or positions.get_device() != at \
             or not positions.is_contiguous():
         raise ValueError("positions must be a contiguous int32/int64 [tokens] tensor")
-    rotary_dim = d if rotary_dim is None else rotary_dim
-    if type(rotary_dim) is not int or not 0 < rotary_dim <= d or rotary_dim % 2 or cos_sin_cache.ndim != 2 \
-            or cos_sin_cache.shape[1] != rotary_dim or cos_sin_cache.stride(1) != 1 \
-            or cos_sin_cache.dtype not in _KV_DTYPES or cos_sin_cache.device != device:
+    if rotary_dim is None:
+        rotary_dim = d
+    table_shape, table_stride = cos_sin_cache.shape, cos_sin_cache.stride()
+    table_t = _KV_DTYPES.get(cos_sin_cache.dtype)
+    if type(rotary_dim) is not int or not 0 < rotary_dim <= d or rotary_dim % 2 or len(table_shape) != 2 \
+            or table_shape[1] != rotary_dim or table_stride[1] != 1 or table_t is None \
+            or cos_sin_cache.get_device() != at:
         raise ValueError("the rotation needs a native cos/sin cache matching rotary_dim")
-    if (k_buffer is None) != (v_buffer is None) or (k_buffer is None) != (slot_map is None):
-        raise ValueError("the pool write needs k_buffer, v_buffer and slot_map")
     if k_buffer is None:
+        if v_buffer is not None or slot_map is not None:
+            raise ValueError("the pool write needs k_buffer, v_buffer and slot_map")
         if k_out is None:
             raise ValueError("k needs k_out, the pool, or both")
         pool = (None, _lib.AKV_I32, None, None, 0, 0, 0, 0, 0)
         v_args = (None, 0, 0)
     else:
-        if v is None or v.shape != k.shape or v.dtype != dtype or v.device != device or v.stride(2) != 1:
+        if v_buffer is None or slot_map is None:
+            raise ValueError("the pool write needs k_buffer, v_buffer and slot_map")
+        v_stride = None if v is None else v.stride()
+        if v is None or v.shape != k_shape or v.dtype != dtype or v.get_device() != at or v_stride[2] != 1:
             raise ValueError("v must be shaped like k, of its dtype and device, with unit dim stride")
-        for t in (k_buffer, v_buffer):
-            if t.ndim != 3 or t.shape[1:] != k.shape[1:] or t.shape[0] != k_buffer.shape[0] or t.dtype != dtype \
-                    or t.device != device or t.stride(2) != 1:
-                raise ValueError("the pool must be [slots, kv_heads, head_dim] buffers of k's dtype and device")
-        if slot_map.dtype not in _INDEX or slot_map.shape != (n,) or slot_map.device != device \
+        pool_shape, kp_stride, vp_stride = k_buffer.shape, k_buffer.stride(), v_buffer.stride()
+        if len(pool_shape) != 3 or pool_shape[1] != hk or pool_shape[2] != d or v_buffer.shape != pool_shape \
+                or k_buffer.dtype != dtype or v_buffer.dtype != dtype or k_buffer.get_device() != at \
+                or v_buffer.get_device() != at or kp_stride[2] != 1 or vp_stride[2] != 1:
+            raise ValueError("the pool must be [slots, kv_heads, head_dim] buffers of k's dtype and device")
+        slots_t = _INDEX.get(slot_map.dtype)
+        if slots_t is None or slot_map.ndim != 1 or slot_map.numel() != n or slot_map.get_device() != at \
                 or not slot_map.is_contiguous():
             raise ValueError("slot_map must be a contiguous int32/int64 [tokens] tensor")
-        pool = (slot_map.data_ptr(), _INDEX[slot_map.dtype], k_buffer.data_ptr(), v_buffer.data_ptr(),
-                k_buffer.shape[0], k_buffer.stride(0), k_buffer.stride(1), v_buffer.stride(0), v_buffer.stride(1))
-        v_args = (v.data_ptr(), v.stride(0), v.stride(1))
-    if device.type != "cuda":
+        pool = (slot_map.data_ptr(), slots_t, k_buffer.data_ptr(), v_buffer.data_ptr(), pool_shape[0], kp_stride[0],
+                kp_stride[1], vp_stride[0], vp_stride[1])
+        v_args = (v.data_ptr(), v_stride[0], v_stride[1])
+    if at < 0:
         raise ValueError("q must be on a GPU")
-    k_out_args = (None, 0, 0) if k_out is None else (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
     if n == 0:
         return q_out
-    lib = _lib.calls()
+    device = q.device
     with _on_device(device):
-        rc = lib.akv_qk_norm_rope(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), *v_args,
-            _KV_DTYPES[dtype], n, hq, hk, d, rotary_dim, 1 if is_neox_style else 0, _lib.ptr(q_weight),
-            _lib.ptr(k_weight), _lib.AKV_F32 if weight is None else _KV_DTYPES[weight.dtype], float(eps),
-            positions.data_ptr(), _INDEX[positions.dtype], cos_sin_cache.data_ptr(), _KV_DTYPES[cos_sin_cache.dtype],
-            cos_sin_cache.stride(0), cos_sin_cache.shape[0], q_out.data_ptr(), q_out.stride(0), q_out.stride(1),
-            *k_out_args, *pool, current_stream_handle(device),
+        rc = _lib.calls().akv_qk_norm_rope(
+            q.data_ptr(), q_stride[0], q_stride[1], k.data_ptr(), k_stride[0], k_stride[1], *v_args,
+            _KV_DTYPES[dtype], n, hq, hk, d, rotary_dim, 1 if is_neox_style else 0,
+            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+            _KV_DTYPES[weight_dtype], float(eps), positions.data_ptr(), positions_t, cos_sin_cache.data_ptr(), table_t,
+            table_stride[0], table_shape[0], q_out.data_ptr(), out_stride[0], out_stride[1], *k_out_args, *pool,
+            current_stream_handle(device),
         )
-    _lib.check(rc, "akv_qk_norm_rope")
+    if rc:
+        _lib.check(rc, "akv_qk_norm_rope")
     return q_out
