@@ -97,8 +97,9 @@ def tree_attention(q, k_buffer, v_buffer, qo_indptr, kv_indptr, kv_indices, out,
     gets 0; a key at a slot outside the pool is seen by none.  ``sinks``: f32
     ``[q_heads]``.  ``max_len`` (keys a request's tokens reach: its keys, or
     window + n + 1) and ``max_new`` (its tokens) are host bounds that size the
-    launch and the workspace; the results do not depend on them.  Rows of
-    ``out`` behind the last token stay as they are.  Head dims: multiples of 8
+    launch and the workspace; the results depend on them only in the order of
+    their fp32 sums.  Rows of ``out``, which must not overlap ``q``, behind the
+    last token stay as they are.  Head dims: multiples of 8
     up to 128.  ``status``: as for ``decode_attention``.
     """
     # one read of every property: the checks are most of a small call's time

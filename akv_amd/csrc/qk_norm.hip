@@ -305,8 +305,10 @@ int launch_vector(const NormArgs& args, hipStream_t st) {
   const int at_once = 64 / lanes;
   const int rounds = (a.rows + at_once - 1) / at_once;
   // a token's rows go to one wave (its cos / sin and the weights are loaded
-  // once) unless there are too few tokens to fill the chip with waves
-  a.parts = a.n_tokens >= 4096 ? 1 : rounds;
+  // once) unless there are too few tokens to fill the chip with waves (us with one
+  // wave and with one per round, 64 + 16 heads of 64: 1024 tokens 8.9, 7.2; 2048
+  // 11.5, 12.9; 16384 72.8, 85.6; 32 + 16 heads of 128: 1024 9.5, 8.8; 2048 12.5, 14.8)
+  a.parts = a.n_tokens >= 2048 ? 1 : rounds;
   const int64_t waves = a.n_tokens * a.parts;
   const int64_t blocks = (waves + kThreads / 64 - 1) / (kThreads / 64);
   if (blocks > 0x7fffffffLL) return fail(AKV_EINVAL, "akv_qk_norm_rope: too many tokens");

@@ -70,7 +70,7 @@ struct Request {
     if (!raw_ids) return i;
     return i < active ? raw_ids[i] : prompt + i - active;
   }
-  __device__ __forceinline__ int32_t slot_at(int64_t raw) const { return raw < width ? row[raw] : -1; }
+  __device__ __forceinline__ int32_t slot_at(int64_t raw) const { return raw >= 0 && raw < width ? row[raw] : -1; }
   __device__ __forceinline__ int64_t pos_of(int64_t i) const {
     if (!raw_ids) return i;
     return i < active ? positions[i] : next_pos + i - active;

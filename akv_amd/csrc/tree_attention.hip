@@ -66,8 +66,13 @@ constexpr int kBuffers = 2;
 // Workgroups of a launch that shares the keys out: two per CU.
 constexpr int kGroupsShift = 9, kGroups = 1 << kGroupsShift;
 // What a piece costs beside its tiles (indices, the first tiles' latency, its
-// result), and the least a workgroup is given, in tiles of 64 keys.
+// result), and the least a workgroup is given, in tiles of 64 keys.  (us with a
+// cost of 1, 3 and 6, 64 / 8 heads of 64: 16 requests of 1500 keys 27.4, 26.1, 26.4; 32
+// of 3000 56.5, 56.6, 58.9.  A least share of 4: 4 requests of 2000 19.6 for 21.0,
+// one of 1000 17.7 for 16.3.)
 constexpr int kPieceCost = 3, kLeastShare = 2;
+
+constexpr int64_t kMostKeys = 1 << 30;  // of a request: ranks and tiles stay far inside 32 bits
 
 constexpr int kWordsKept = 2;  // mask words of a row in LDS: trees of up to 128 tokens
 
@@ -264,13 +269,16 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
   struct Cost {
     int32_t units, rows;
   };
+  auto keys_in = [&](int64_t b) -> int64_t {
+    const int64_t len = load_index(a.kv_indptr, a.indptr64, b + 1) - load_index(a.kv_indptr, a.indptr64, b);
+    return len < 0 ? 0 : len < kMostKeys ? len : kMostKeys;
+  };
   auto cost_of = [&](int64_t b, int rb) -> Cost {
     int64_t q0 = load_index(a.qo_indptr, a.indptr64, b), q1 = load_index(a.qo_indptr, a.indptr64, b + 1);
-    const int64_t len = load_index(a.kv_indptr, a.indptr64, b + 1) - load_index(a.kv_indptr, a.indptr64, b);
     q0 = q0 < 0 ? 0 : q0;
     q1 = q1 > a.n_tokens ? a.n_tokens : q1;
     const int32_t rows = q1 > q0 ? static_cast<int32_t>(q1 - q0) * a.group : 0;
-    return Cost{units_of(len, rows, rb), rows};
+    return Cost{units_of(keys_in(b), rows, rb), rows};
   };
   int32_t lane_units = 0;  // of request `lane`, for the block of rows last summed
   auto sum_of = [&](int rb, int32_t* most_rows) -> int64_t {
@@ -342,111 +350,109 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
   }
 
   for (;;) {
-  // (in scalar registers: the loop has no vector register to spare)
-  int64_t q0 = uniform(load_index(a.qo_indptr, a.indptr64, b)), q1 = uniform(load_index(a.qo_indptr, a.indptr64, b + 1));
-  const int64_t kv0 = uniform(load_index(a.kv_indptr, a.indptr64, b));
-  const int64_t len64 = uniform(load_index(a.kv_indptr, a.indptr64, b + 1)) - kv0;
-  if (q0 < 0) q0 = 0;
-  if (q1 > a.n_tokens) q1 = a.n_tokens;
-  const int n = static_cast<int>(q1 > q0 ? q1 - q0 : 0);
-  const int rows = n * a.group;
-  const int len = static_cast<int>(len64 > 0 ? len64 : 0);
-  const int old = len > n ? len - n : 0;
-  if (a.whole && rb * R >= rows) return;
-  // the keys that some token of the request sees begin here
-  int lo = 0, hi_start = 0;
-  if (a.key_starts) {
-    lo = old;
-    for (int i = lane; i < n; i += 64) {
-      const int s = min(max(a.key_starts[q0 + i], 0), old);
-      lo = min(lo, s);
-      hi_start = max(hi_start, s);
-    }
-    lo = uniform(__ockl_wfred_min_i32(lo));
-    hi_start = uniform(__ockl_wfred_max_i32(hi_start));
-  }
-  // the piece: units [off, stop) of the request's, the first kPieceCost of them
-  // for no tile, the others for equal parts of its tiles
-  const int units = units_of(len, rows, rb);
-  const int stop = a.whole || budget > units - off ? units : static_cast<int>(off + budget);
-  const bool first = off == 0, last = stop == units;
-  const int all_tiles = (len - lo + kKeys - 1) / kKeys;
-  auto tile_of = [&](int64_t unit) -> int {
-    const int64_t at = unit > kOver ? unit - kOver : 0;
-    return static_cast<int>(units - kOver == all_tiles ? at : at * all_tiles / (units - kOver));
-  };
-  const int begin = lo + uniform(tile_of(off)) * kKeys;
-  const int end = min(lo + uniform(tile_of(stop)) * kKeys, len);
-  const int tiles = end > begin ? (end - begin + kKeys - 1) / kKeys : 0;
-
-  // (an empty pool holds no key: every slot is a hole, and zeros are read)
-  const bool pool = a.pool_slots > 0;
-  const char* kbase = pool ? a.k + g * a.k_sh : reinterpret_cast<const char*>(zero_row);
-  const char* vbase = pool ? a.v + g * a.v_sh : reinterpret_cast<const char*>(zero_row);
-  const uint32_t k_ss = pool ? a.k_ss : 0, v_ss = pool ? a.v_ss : 0;
-  const int32_t* list = a.kv_indices + (a.paged ? b * a.table_stride : kv0);
-  // entries of the list that exist
-  const int64_t left = a.paged ? a.table_width : a.table_width - kv0;
-  const int32_t width = static_cast<int32_t>(std::min<int64_t>(std::max<int64_t>(left, 0), 0x7fffffff));
-  const int32_t* entries = width > 0 ? list : reinterpret_cast<const int32_t*>(zero_row);
-  const int last_entry = max(width - 1, 0);
-  // The wave's keys of kEntryTiles tiles at a time: lane l has key l % kWaveKeys
-  // of tile l / kWaveKeys.  Their list entries come to LDS kEntryTiles tiles ahead.
-  const int my_key = lane / kWaveKeys * kKeys + kWaveKeys * wave + lane % kWaveKeys;
-  auto fetch = [&](int e) {
-    const uint32_t j = min(begin + e * (kEntryTiles * kKeys) + my_key, end - 1);  // past the end: the last key's
-    const int32_t at = a.paged ? j / static_cast<uint32_t>(a.page_size) : j;
-    load_4(entries + min(at, last_entry), uniform(lds_address(s_entry[wave][e & 1])));
-  };
-  uint32_t slots = 0;
-  auto look_up = [&](int e) {
-    const uint32_t key = begin + e * (kEntryTiles * kKeys) + my_key, j = min(key, static_cast<uint32_t>(end - 1));
-    const int32_t entry = s_entry[wave][e & 1][lane];
-    uint64_t slot = static_cast<uint32_t>(entry);
-    uint32_t at = j;
-    if (a.paged) {
-      const uint32_t page = a.page_size;
-      at = j / page;
-      slot = slot * page + (j - at * page);
-    }
-    const bool there = entry >= 0 && at < static_cast<uint32_t>(width) && slot < static_cast<uint64_t>(a.pool_slots);
-    // a hole reads slot 0; the mask keeps it from every row
-    slots = there ? static_cast<uint32_t>(slot) : 0;
-    const uint64_t dead = __builtin_amdgcn_ballot_w64(!there || key >= static_cast<uint32_t>(end));
-    if (lane < kEntryTiles) {
-      const uint32_t mine = static_cast<uint32_t>(dead >> (kWaveKeys * lane));
-      char* to = reinterpret_cast<char*>(s_dead[(e & 1) * kEntryTiles + lane]) + kWaveKeys / 8 * wave;
-      if constexpr (kWaveKeys == 32)
-        *reinterpret_cast<uint32_t*>(to) = mine;
-      else
-        *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(mine);
-    }
-  };
-  // a wave's keys of a tile, straight into LDS: lane l of a load fills bytes
-  // 16 l of a 1 KiB block, chunk position l % kChunks of a row
-  auto stage = [&](int it) {
-    if (it % kEntryTiles == 0) {
-      look_up(it / kEntryTiles);
-      fetch(it / kEntryTiles + 1);
-    }
-    TileLds<D>& t = buffers[it % kBuffers];
-#pragma unroll
-    for (int u = 0; u < kWaveKeys / kLoadRows; ++u) {
-      const int mine = u * kLoadRows + lane / kChunks, r = kWaveKeys * wave + mine;
-      const uint64_t from = __shfl(slots, it % kEntryTiles * kWaveKeys + mine);
-      const int ck = (lane % kChunks) ^ swz_k<D>(r), cv = (lane % kChunks) ^ swz_v<D>(r);
-      const char* krow = kbase + from * k_ss + 16 * ck;
-      const char* vrow = vbase + from * v_ss + 16 * cv;
-      if (NARROW) {  // dims past head_dim read zeros
-        krow = 8 * ck < a.head_dim ? krow : reinterpret_cast<const char*>(zero_row);
-        vrow = 8 * cv < a.head_dim ? vrow : reinterpret_cast<const char*>(zero_row);
+    // (in scalar registers: the loop has no vector register to spare)
+    int64_t q0 = uniform(load_index(a.qo_indptr, a.indptr64, b)), q1 = uniform(load_index(a.qo_indptr, a.indptr64, b + 1));
+    const int64_t kv0 = uniform(load_index(a.kv_indptr, a.indptr64, b));
+    const int len = static_cast<int>(uniform(keys_in(b)));
+    if (q0 < 0) q0 = 0;
+    if (q1 > a.n_tokens) q1 = a.n_tokens;
+    const int n = static_cast<int>(q1 > q0 ? q1 - q0 : 0);
+    const int rows = n * a.group;
+    const int old = len > n ? len - n : 0;
+    if (a.whole && rb * R >= rows) return;
+    // the keys that some token of the request sees begin here
+    int lo = 0, hi_start = 0;
+    if (a.key_starts) {
+      lo = old;
+      for (int i = lane; i < n; i += 64) {
+        const int s = min(max(a.key_starts[q0 + i], 0), old);
+        lo = min(lo, s);
+        hi_start = max(hi_start, s);
       }
-      const int place = (kWaveKeys * wave + u * kLoadRows) * D * 2;
-      load_16(krow, uniform(lds_address(t.k + place)));
-      load_16(vrow, uniform(lds_address(t.v + place)));
+      lo = uniform(__ockl_wfred_min_i32(lo));
+      hi_start = uniform(__ockl_wfred_max_i32(hi_start));
     }
-  };
-  {
+    // the piece: units [off, stop) of the request's, the first kPieceCost of them
+    // for no tile, the others for equal parts of its tiles
+    const int units = units_of(len, rows, rb);
+    const int stop = a.whole || budget > units - off ? units : static_cast<int>(off + budget);
+    const bool first = off == 0, last = stop == units;
+    const int all_tiles = (len - lo + kKeys - 1) / kKeys;
+    auto tile_of = [&](int64_t unit) -> int {
+      const int64_t at = unit > kOver ? unit - kOver : 0;
+      return static_cast<int>(units - kOver == all_tiles ? at : at * all_tiles / (units - kOver));
+    };
+    const int begin = lo + uniform(tile_of(off)) * kKeys;
+    const int end = min(lo + uniform(tile_of(stop)) * kKeys, len);
+    const int tiles = end > begin ? (end - begin + kKeys - 1) / kKeys : 0;
+
+    // (an empty pool holds no key: every slot is a hole, and zeros are read)
+    const bool pool = a.pool_slots > 0;
+    const char* kbase = pool ? a.k + g * a.k_sh : reinterpret_cast<const char*>(zero_row);
+    const char* vbase = pool ? a.v + g * a.v_sh : reinterpret_cast<const char*>(zero_row);
+    const uint32_t k_ss = pool ? a.k_ss : 0, v_ss = pool ? a.v_ss : 0;
+    const int32_t* list = a.kv_indices + (a.paged ? b * a.table_stride : kv0);
+    // entries of the list that exist
+    const int64_t left = a.paged ? a.table_width : kv0 < 0 ? 0 : a.table_width - kv0;
+    const int32_t width = static_cast<int32_t>(std::min<int64_t>(std::max<int64_t>(left, 0), 0x7fffffff));
+    const int32_t* entries = width > 0 ? list : reinterpret_cast<const int32_t*>(zero_row);
+    const int last_entry = max(width - 1, 0);
+    // The wave's keys of kEntryTiles tiles at a time: lane l has key l % kWaveKeys
+    // of tile l / kWaveKeys.  Their list entries come to LDS kEntryTiles tiles ahead.
+    const int my_key = lane / kWaveKeys * kKeys + kWaveKeys * wave + lane % kWaveKeys;
+    auto fetch = [&](int e) {
+      const uint32_t j = min(begin + e * (kEntryTiles * kKeys) + my_key, end - 1);  // past the end: the last key's
+      const int32_t at = a.paged ? j / static_cast<uint32_t>(a.page_size) : j;
+      load_4(entries + min(at, last_entry), uniform(lds_address(s_entry[wave][e & 1])));
+    };
+    uint32_t slots = 0;
+    auto look_up = [&](int e) {
+      const uint32_t key = begin + e * (kEntryTiles * kKeys) + my_key, j = min(key, static_cast<uint32_t>(end - 1));
+      const int32_t entry = s_entry[wave][e & 1][lane];
+      uint64_t slot = static_cast<uint32_t>(entry);
+      uint32_t at = j;
+      if (a.paged) {
+        const uint32_t page = a.page_size;
+        at = j / page;
+        slot = slot * page + (j - at * page);
+      }
+      const bool there = entry >= 0 && at < static_cast<uint32_t>(width) && slot < static_cast<uint64_t>(a.pool_slots);
+      // a hole reads slot 0; the mask keeps it from every row
+      slots = there ? static_cast<uint32_t>(slot) : 0;
+      const uint64_t dead = __builtin_amdgcn_ballot_w64(!there || key >= static_cast<uint32_t>(end));
+      if (lane < kEntryTiles) {
+        const uint32_t mine = static_cast<uint32_t>(dead >> (kWaveKeys * lane));
+        char* to = reinterpret_cast<char*>(s_dead[(e & 1) * kEntryTiles + lane]) + kWaveKeys / 8 * wave;
+        if constexpr (kWaveKeys == 32)
+          *reinterpret_cast<uint32_t*>(to) = mine;
+        else
+          *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(mine);
+      }
+    };
+    // a wave's keys of a tile, straight into LDS: lane l of a load fills bytes
+    // 16 l of a 1 KiB block, chunk position l % kChunks of a row
+    auto stage = [&](int it) {
+      if (it % kEntryTiles == 0) {
+        look_up(it / kEntryTiles);
+        fetch(it / kEntryTiles + 1);
+      }
+      TileLds<D>& t = buffers[it % kBuffers];
+  #pragma unroll
+      for (int u = 0; u < kWaveKeys / kLoadRows; ++u) {
+        const int mine = u * kLoadRows + lane / kChunks, r = kWaveKeys * wave + mine;
+        const uint64_t from = __shfl(slots, it % kEntryTiles * kWaveKeys + mine);
+        const int ck = (lane % kChunks) ^ swz_k<D>(r), cv = (lane % kChunks) ^ swz_v<D>(r);
+        const char* krow = kbase + from * k_ss + 16 * ck;
+        const char* vrow = vbase + from * v_ss + 16 * cv;
+        if (NARROW) {  // dims past head_dim read zeros
+          krow = 8 * ck < a.head_dim ? krow : reinterpret_cast<const char*>(zero_row);
+          vrow = 8 * cv < a.head_dim ? vrow : reinterpret_cast<const char*>(zero_row);
+        }
+        const int place = (kWaveKeys * wave + u * kLoadRows) * D * 2;
+        load_16(krow, uniform(lds_address(t.k + place)));
+        load_16(vrow, uniform(lds_address(t.v + place)));
+      }
+    };
     if (tiles > 0) fetch(0);
     if (threadIdx.x == 0) s_odd = 0;
     // groups of rows, and the waves that share one
@@ -828,7 +834,6 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
       }
     }
     __syncthreads();
-  }
     if (a.whole) {
       rb += a.row_blocks;
       continue;
@@ -924,7 +929,10 @@ int tile_dim(int32_t head_dim) { return head_dim <= 64 ? 64 : 128; }
 
 // A wave's row subtiles for requests of up to `rows` rows: a tile has keys for
 // four waves (two at D = 128) to share a group of rows, so the rows are dealt out
-// to two (four) groups before a wave takes more of them.
+// to two (four) groups before a wave takes more of them.  (us for 16 requests of
+// 4096 keys, 64 / 8 heads of 64, the waves' rows halved, as here, doubled: 64 rows a
+// KV head 39.1, 38.6, 38.9, 128 rows 47.0, 46.7, 47.0; 32 / 8 heads of 128: 64 rows
+// 60.5, 61.2, 64.1, 128 rows 86.0, 73.6, 72.9.)
 int subtiles_for(int d, int64_t rows) {
   const int most = d == 64 ? 4 : 2;
   const int64_t groups = d == 64 ? 2 : 4;
@@ -939,18 +947,25 @@ struct Launch {
   int32_t row_blocks;
 };
 
-// Keys up to which a request is one workgroup's: a cut would save less than the
-// second launch costs.
-constexpr int64_t kWholeKeys = 256;
+// Where a block of rows is one workgroup's from its first key to its last: the
+// second launch and the pieces cost 6 to 10 us, more than a cut saves on up to four
+// tiles (8 tokens, 64 / 8 heads of 64, one request, us whole and cut: 384 keys
+// 14.3, 15.9; 512: 15.8, 16.0; 768: 18.7, 14.6), or, where the workgroups fill half
+// the chip, on up to 1024 keys (the same with 16 requests of 1024: 21.7, 24.6, of
+// 2048: 32.6, 29.3; 64 requests of 8 to 1024: 27.9, 41.2; with one of 1024 among
+// 63 of 100: 25.0, 29.5; 65 requests of 1024, a round and a bit: 47.9, 45.5).
+constexpr int64_t kWholeTiles = 4, kWholeKeys = 1024, kWholeGroups = 128;
 
-Launch plan(int64_t n_tokens, int64_t group, int32_t head_dim, int64_t max_len, int64_t max_new) {
+Launch plan(int64_t n_tokens, int64_t n_requests, int64_t q_heads, int64_t kv_heads, int32_t head_dim,
+            int64_t max_len, int64_t max_new) {
   Launch p;
   p.d = tile_dim(head_dim);
-  const int64_t rows = std::max<int64_t>(1, std::min(max_new, n_tokens)) * group;
+  const int64_t rows = std::max<int64_t>(1, std::min(max_new, n_tokens)) * (q_heads / kv_heads);
   p.sub = subtiles_for(p.d, rows);
   const int64_t block = 16 * kWaves * p.sub;
   p.row_blocks = static_cast<int32_t>(std::min<int64_t>((rows + block - 1) / block, 4096));
-  p.whole = max_len <= kWholeKeys;
+  p.whole = max_len <= kWholeTiles * keys_of(p.d) ||
+            (max_len <= kWholeKeys && n_requests * kv_heads * p.row_blocks >= kWholeGroups);
   return p;
 }
 
@@ -970,7 +985,9 @@ void start(const TreeArgs& a, dim3 grid, hipStream_t st) {
 }
 
 // Few rows are cut into many pieces each, and many rows fill the chip: a wave per
-// row up to kFewRows, D / 4 lanes beyond.
+// row up to kFewRows, D / 4 lanes beyond (both launches, us by the wave and by the
+// lanes: 512 rows of one request of 8192 keys 22.6, 31.5; 4096 rows 42.8, 44.8; 16384
+// rows of 16 requests of 4096 49.7, 46.8).
 constexpr int64_t kFewRows = 4096;
 
 template <typename T, int D>
@@ -1020,7 +1037,8 @@ extern "C" int64_t akv_tree_attention_workspace_bytes(int64_t n_tokens, int32_t 
                                                        int64_t max_new) {
   using namespace akv;
   if (!sizes_ok(n_tokens, n_requests, q_heads, kv_heads, head_dim, max_len, max_new)) return -1;
-  return partial_bytes(plan(n_tokens, q_heads / kv_heads, head_dim, max_len, max_new), n_tokens, q_heads);
+  return partial_bytes(plan(n_tokens, n_requests, q_heads, kv_heads, head_dim, max_len, max_new), n_tokens,
+                       q_heads);
 }
 
 extern "C" int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_buffer,
@@ -1058,10 +1076,10 @@ extern "C" int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_s
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_buffer) |
         reinterpret_cast<uintptr_t>(v_buffer) | reinterpret_cast<uintptr_t>(workspace)) & 15) != 0)
     return fail(AKV_EINVAL, "akv_tree_attention: q, K and V rows and the workspace must be 16-byte aligned");
-  if (pool_slots > 0xffffffffLL || (k_stride_slot | v_stride_slot) >> 31 || n_tokens > 0x7fffffffLL / q_heads ||
+  if (pool_slots > 0xffffffffLL || (k_stride_slot | v_stride_slot) >> 31 || n_tokens > 0x7f000000LL / q_heads ||
       static_cast<int64_t>(n_requests) * kv_heads > 0x7fffffffLL / 4096)
     return fail(AKV_EINVAL, "akv_tree_attention: batch too large");
-  const Launch p = plan(n_tokens, q_heads / kv_heads, head_dim, max_len, max_new);
+  const Launch p = plan(n_tokens, n_requests, q_heads, kv_heads, head_dim, max_len, max_new);
   const int64_t need = partial_bytes(p, n_tokens, q_heads);
   if (workspace_bytes < need)
     return fail(AKV_EINVAL, "akv_tree_attention: workspace holds %lld bytes, needs %lld",

@@ -753,7 +753,8 @@ int akv_gather_slots(int32_t slot_dtype, const int64_t* sources,
  *   tree_mask[qo + i]      bit a: new token a is i or an ancestor of i
  *   window_mask[qo + i]    bit a: the same, at most W levels up
  *   window_starts[qo + i]  first rank of [0, L - n) whose position is at least
- *                          positions[qo + i] - W (positions ascend)
+ *                          positions[qo + i] - W (positions ascend
+ *                          strictly)
  * parents[qo + i] is a new token of the request before i, anything else none
  * (depth 0); without parents token i follows i - 1.  Masks are rows of
  * *_words 64-bit words, *_stride words apart; tokens past 64 words have no
@@ -830,7 +831,9 @@ int akv_qk_norm_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  * page(j / page_size) * page_size + j % page_size.  A key whose slot lies
  * outside [0, pool_slots), or whose entry outside the list, is seen by no
  * token.  max_len (keys a request's tokens reach) and max_new (its tokens) are
- * host bounds that only size the launch: results do not depend on them.
+ * host bounds that only size the launch: results do not depend on them (but
+ * for the order of their fp32 sums).  A request has up to 2^30 keys; out must
+ * not overlap q.
  * n_tokens is the capacity of q and out; rows behind qo_indptr[B] stay as they
  * are.  workspace: akv_tree_attention_workspace_bytes with the same arguments,
  * 16-byte aligned, any contents; calls that share one must not overlap.
