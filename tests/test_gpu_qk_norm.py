@@ -170,3 +170,15 @@ def test_no_tokens_and_int32_vectors(device):
     empty = _case(device, 10, 0, 4, 2, 64, torch.bfloat16)
     _run(empty)
     assert (empty["pool"][0] == 7).all()
+
+
+@pytest.mark.parametrize("n", [2047, 2048, 2053])
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.float16), (80, torch.float32)])
+def test_around_the_split_of_a_token(device, n, d, dtype):
+    """Token counts on both sides of the rule that gives a token to one wave."""
+    print(f"qk norm {n} tokens of {d} {dtype}", flush=True)
+    c = _case(device, n + d, n, 9, 4, d, dtype)
+    q_out, k_out = torch.empty_like(c["q"]), torch.empty_like(c["k"])
+    qk_norm.qk_norm_rope(c["q"], c["k"], c["v"], *c["w"], c["positions"], c["table"], q_out, k_out=k_out,
+                         slot_map=c["slots"], k_buffer=c["pool"][0], v_buffer=c["pool"][1])
+    _check(c, q_out, k_out)

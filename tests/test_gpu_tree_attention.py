@@ -270,3 +270,135 @@ def test_random_batches(device):
         full = None if starts is None else np.concatenate((starts, np.zeros(c.capacity - c.total, np.int64)))
         sinks = torch.randn(hq, generator=torch.Generator().manual_seed(seed)).to(device) if seed % 2 else None
         _check(c, _run(c, mask=mask, starts=full, sinks=sinks), c.visible(seen, starts), sinks=sinks)
+
+
+@pytest.mark.parametrize("bound", [1, 5000])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_whole_and_shared_out(device, shape, bound):
+    """Every shape as one workgroup per block of rows, and on the line."""
+    hq, hk, d, dtype, page, old, new = SHAPES[shape]
+    print(f"tree attention shape {shape} {SHAPES[shape]} bound {bound}", flush=True)
+    c = Cache(device, 200 + shape, old, new, q_heads=hq, kv_heads=hk, head_dim=d, dtype=dtype, page=page, holes=2)
+    seen, mask = c.masks("any")
+    starts = np.concatenate([c.rng.integers(0, o + 1, n) for o, n in zip(old, new)])
+    sinks = torch.randn(hq, generator=torch.Generator().manual_seed(shape)).to(device) if shape % 2 == 0 else None
+    _check(c, _run(c, mask=mask, max_len=bound, max_new=max(1, c.max_new // 3)), c.visible(seen))
+    _check(c, _run(c, mask=mask, starts=starts, sinks=sinks, max_len=bound), c.visible(seen, starts), sinks=sinks)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bound", [1, 5000])
+def test_trees_of_many_words(device, d, bound):
+    """More drafted tokens than the mask words kept at hand, and words that end
+    before the tokens do."""
+    old, new = [300, 1], [200, 333]
+    c = Cache(device, 300 + d, old, new, q_heads=4, kv_heads=2, head_dim=d, dtype=torch.bfloat16)
+    starts = np.concatenate([c.rng.integers(0, o + 1, n) for o, n in zip(old, new)])
+    for kind in ("chain", "tree", "any"):
+        print(f"tree attention large trees d={d} bound {bound} {kind}", flush=True)
+        seen, mask = c.masks(kind)
+        _check(c, _run(c, mask=mask, starts=starts, max_len=bound), c.visible(seen, starts))
+        if mask is None:
+            continue
+        short = [s.copy() for s in seen]
+        for s in short:
+            s[:, 192:] = False
+        _check(c, _run(c, mask=mask[:, :3], max_len=bound), c.visible(short))
+
+
+@pytest.mark.parametrize("bound", [1, 900, 5000])
+def test_many_requests(device, bound):
+    """More requests than a wave has lanes, empty ones among them."""
+    rng = np.random.default_rng(9)
+    old = [int(rng.integers(0, 900)) if i % 3 else 0 for i in range(150)]
+    new = [0 if i % 7 == 3 or 64 <= i < 130 else int(rng.integers(0, 6)) for i in range(150)]
+    c = Cache(device, 400, old, new, q_heads=6, kv_heads=3, head_dim=64, dtype=torch.float16)
+    seen, mask = c.masks("tree")
+    _check(c, _run(c, mask=mask, max_len=bound), c.visible(seen))
+    c = Cache(device, 401, old, [20 if i == 149 else 0 for i in range(150)], q_heads=24, kv_heads=1, head_dim=64,
+              dtype=torch.bfloat16)  # a block of rows that only the last request has
+    seen, mask = c.masks("tree")
+    _check(c, _run(c, mask=mask, max_len=bound), c.visible(seen))
+
+
+@pytest.mark.parametrize("page", [1, 16])
+def test_slots_past_32_bits(device, page):
+    """A layer whose rows lie 2 MiB apart: offsets beyond 4 GiB in bytes."""
+    c = Cache(device, 500 + page, [2300], [5], q_heads=4, kv_heads=2, head_dim=64, dtype=torch.bfloat16, page=page)
+    stride, n = 1 << 20, c.k.shape[0]
+    store = torch.empty(n * stride, dtype=torch.bfloat16, device=device)
+    k, v = (store.as_strided((n, 2, 64), (stride, 64, 1), at) for at in (0, 4096))
+    k.copy_(c.k), v.copy_(c.v)
+    seen, mask = c.masks("tree")
+    _check(c, _run(c, mask=mask, k=k, v=v), c.visible(seen))
+
+
+@pytest.mark.parametrize("d,out_dtype", [(64, torch.float32), (128, torch.bfloat16), (96, torch.float32)])
+def test_unaligned_outputs(device, d, out_dtype):
+    for old in ([300, 20], [3000, 20]):
+        c = Cache(device, 600 + d, old, [7, 4], q_heads=4, kv_heads=2, head_dim=d, dtype=torch.bfloat16)
+        store = torch.full((c.total, 4, d + 3), 7.0, dtype=out_dtype, device=device)
+        seen, mask = c.masks("tree")
+        out = _run(c, mask=mask, out=store[:, :, 1: d + 1])
+        _check(c, out, c.visible(seen))
+        assert (store[:, :, 0] == 7).all() and (store[:, :, d + 1:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [2, 40])
+def test_maxima_that_jump_behind_the_first_tiles(device, d, dtype, new):
+    """Keys that every token sees, their scores above the first ones' by more
+    than a weight of the storage type can hold, in some rows only."""
+    c = Cache(device, 700 + d, [1400], [new], q_heads=4, kv_heads=1, head_dim=d, dtype=dtype)
+    c.k[:] = 0.01 * c.k
+    c.q[:] = 0.01 * c.q
+    ranks = torch.from_numpy(c.slots[0])
+    jump = torch.zeros(1400 + new)
+    for at, by in ((100, 6.0), (300, 12.0), (301, 13.0), (700, 40.0), (1200, 41.0)):
+        jump[at] = by
+    c.k[ranks, 0, 0] = jump.to(dtype)
+    c.q[::2, 1:3, 0] = 2.0
+    seen, mask = c.masks("tree")
+    for bound in (1, 5000):
+        _check(c, _run(c, mask=mask, scale=1.0, out_dtype=torch.float32, max_len=bound), c.visible(seen), scale=1.0)
+
+
+@pytest.mark.parametrize("bound", [1, 5000])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_odd_values_in_pieces(device, value, bound):
+    """Infinities and NaN of one dim: in the rows that see the key, that dim is
+    not finite and the others are right; the other rows are."""
+    old, new = [2000, 300], [6, 30]
+    c = Cache(device, 800, old, new, q_heads=4, kv_heads=2, head_dim=64, dtype=torch.bfloat16)
+    seen, mask = c.masks("any")
+    starts = np.concatenate([np.linspace(0, o, n).astype(np.int64) for o, n in zip(old, new)])
+    clean = f64(c.v)
+    bad = {0: [1, 130, 777, 1500, 2003], 1: [5, 290, 303]}
+    for b, ranks in bad.items():
+        for r in ranks:
+            c.v[c.slots[b][r], :, r % 64] = value
+    got = f64(_run(c, mask=mask, starts=starts, max_len=bound))
+    requests = c.visible(seen, starts)
+    want, size, spread = drafts.tree_attention(f64(c.q), f64(c.k), clean, requests, 0.125)
+    tol = attention_tolerance(c.q.dtype, c.q.dtype, c.max_len, want, size, spread, 0)
+    hit = np.zeros(want.shape, dtype=bool)
+    for b, (first, _, keys) in enumerate(requests):
+        for r in bad[b]:
+            for i in np.flatnonzero(keys[:, r]):
+                hit[first + i, :, r % 64] = True
+    assert hit.any() and not np.isfinite(got[hit]).any()
+    assert (np.abs(got - want)[~hit] <= tol[~hit]).all()
+
+
+@pytest.mark.parametrize("fill", [0, 1, 170])
+def test_any_workspace_contents(device, fill):
+    c = Cache(device, 900, [2600, 0, 700], [7, 0, 12], q_heads=8, kv_heads=2, head_dim=64, dtype=torch.bfloat16,
+              capacity=25)
+    seen, mask = c.masks("tree")
+    need = attention.tree_workspace_bytes(25, 3, 8, 2, 64, c.max_len, c.max_new)
+    ws = torch.full((need,), fill, dtype=torch.uint8, device=device)
+    first = _run(c, mask=mask, workspace=ws)
+    _check(c, first, c.visible(seen))
+    for _ in range(3):  # sums are in a fixed order
+        assert torch.equal(_run(c, mask=mask, workspace=ws), first)
