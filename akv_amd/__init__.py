@@ -9,6 +9,10 @@ A drop-in for the KV-cache hot path of thu-nics/AKV:
 * ``akv_amd.page_table`` -- decode indices, window lengths, indptr rebuild
   over the reference registry's rows, and the side-row / extend writes of
   request rows;
+* ``akv_amd.page_table.context_step_maps``, ``akv_amd.qk_norm.qk_norm_rope`` and
+  ``akv_amd.attention.tree_attention`` -- the step that verifies drafted
+  tokens: metadata of the new tokens, per-head norms with the rotation and the
+  pool write, attention of token trees (beside ``decode_attention``);
 * ``akv_amd.context_attention.extend_attention_fwd`` -- prefill attention
   over the compacted rows with context positions;
 * ``akv_amd.plan.compile_context_layout`` -- the host event compiler;

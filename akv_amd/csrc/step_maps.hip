@@ -21,7 +21,9 @@
 // One launch.  Grid (token blocks + table blocks, B + 1): the first workgroups
 // of request b share its tokens, the others its block table; row B fills what
 // lies behind the last token.  A table entry is two dependent loads (raw id,
-// row entry), four chains of them in flight per thread.
+// row entry), four chains of them in flight per thread.  Bound by such round trips:
+// one request of 4096 ranks 3.6 us, 32 of 20k with a page per rank, trees of 16 and
+// a window 8.4 us (7.7 MB), 64 of 2k to 64k with pages of 16 7.8 us.
 #include "common.h"
 
 namespace akv {
@@ -29,7 +31,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;
-constexpr int kMaxTokenBlocks = 16, kMaxTableBlocks = 64;
+// Most workgroups of a request, four times as many in batches of up to kSmallBatch
+// (us: one request of 65536 tokens, 16 groups 8.0, 64 4.5; 64 of 2048 tokens, 4.9 and
+// 8.4, most of them idle; a table of one request of 10^6 ranks, 64 groups 11.8, 256
+// 5.5; of 64 requests of 65536, 10.3 and 10.8).
+constexpr int kMaxTokenBlocks = 16, kMaxTableBlocks = 64, kSmallBatch = 16;
 constexpr int kStagedParents = 2048;  // nodes of a tree kept in LDS; later ones read global memory
 
 struct MapArgs {
@@ -336,15 +342,17 @@ extern "C" int akv_step_maps(const int64_t* registry, const int32_t* table, int6
   a.indptr64 = indptr_dtype == AKV_I64;
   a.slots64 = slots_dtype == AKV_I64;
   a.pos64 = positions_dtype == AKV_I64;
+  const int more = n_requests <= kSmallBatch ? 4 : 1;
   unsigned blocks = 0;
   if (a.block_tables) {
     const int64_t want = (block_width + kThreads * kUnroll - 1) / (kThreads * kUnroll);
-    blocks = static_cast<unsigned>(want < kMaxTableBlocks ? want : kMaxTableBlocks);
+    blocks = static_cast<unsigned>(want < more * kMaxTableBlocks ? want : more * kMaxTableBlocks);
   }
   // a thread's tokens follow each other: four of them where a request has most
   const int64_t shares = (n_tokens + kThreads * kUnroll - 1) / (kThreads * kUnroll);
-  a.token_blocks = static_cast<int32_t>(shares < 1 ? 1 : shares < kMaxTokenBlocks ? shares : kMaxTokenBlocks);
-  hipLaunchKernelGGL(step_maps_kernel, dim3(a.token_blocks + blocks, static_cast<unsigned>(n_requests) + 1), dim3(kThreads), 0,
-                     as_stream(stream), a);
+  const int64_t most = more * kMaxTokenBlocks;
+  a.token_blocks = static_cast<int32_t>(shares < 1 ? 1 : shares < most ? shares : most);
+  const dim3 grid(a.token_blocks + blocks, static_cast<unsigned>(n_requests) + 1);
+  hipLaunchKernelGGL(step_maps_kernel, grid, dim3(kThreads), 0, as_stream(stream), a);
   return check_launch("akv_step_maps");
 }

@@ -163,3 +163,34 @@ def test_empty_batch_and_closed_gate(device):
     page_table.context_step_maps(b.registry, b.table, b.rows, b.seq, b.fresh, qo, kv, slots, positions,
                                  status=torch.tensor([2], dtype=torch.int32, device=device))
     assert (qo == 7).all() and (slots == -1).all()
+
+
+@pytest.mark.parametrize("copies", [1, 17])
+def test_long_requests_on_both_sides_of_the_batch_rule(device, copies):
+    """Requests that take every workgroup a request may have (chains, which need
+    no ancestors: positions ascend by one from the root's)."""
+    for old, new, kept, window in (([230000] + [5] * (copies - 1), [70000] + [3] * (copies - 1), [1] + [0] * (copies - 1), 100),
+                                   ([9000] * copies, [1200] * copies, [1] * copies, None)):
+        print(f"step maps {copies} requests of {old[0]} + {new[0]}", flush=True)
+        b = Batch(device, 20 + copies + len(kept), old, new, kept=kept, holes=3)
+        total, longest = sum(new), max(len(s) for s, _ in b.requests)
+        full = lambda *shape, t=torch.int32: torch.full(shape, 77, dtype=t, device=device)  # noqa: E731
+        qo, kv, table = full(copies + 1), full(copies + 1), full(copies, longest + 2)
+        slot_map, positions, starts = full(total, t=torch.int64), full(total, t=torch.int64), full(total)
+        page_table.context_step_maps(b.registry, b.table, b.rows, b.seq, b.fresh, qo, kv, slot_map, positions,
+                                     block_tables=table, window=window, window_starts=starts if window else None)
+        want = dict(slots=[], positions=[], starts=[])
+        for r, ((slots, pos), o, n) in enumerate(zip(b.requests, old, new)):
+            row = np.full(longest + 2, -1)
+            row[: len(slots)] = np.maximum(slots, -1)
+            np.testing.assert_array_equal(table[r].cpu().numpy(), row)
+            at = pos[o] + np.arange(n)
+            want["slots"].append(slots[o:])
+            want["positions"].append(at)
+            want["starts"].append(np.searchsorted(pos[:o], at - (window or 0)))
+        np.testing.assert_array_equal(qo.cpu().numpy(), np.concatenate(([0], np.cumsum(new))))
+        np.testing.assert_array_equal(kv.cpu().numpy(), np.concatenate(([0], np.cumsum(np.add(old, new)))))
+        np.testing.assert_array_equal(slot_map.cpu().numpy(), np.concatenate(want["slots"]))
+        np.testing.assert_array_equal(positions.cpu().numpy(), np.concatenate(want["positions"]))
+        if window:
+            np.testing.assert_array_equal(starts.cpu().numpy(), np.concatenate(want["starts"]))
