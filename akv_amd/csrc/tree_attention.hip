@@ -588,15 +588,22 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
       }
     };
     // O^T += V^T . P^T: lane col of group quad receives V[key][16 dt + col] for
-    // keys 4 quad + i (i < 4) of the quarter, then 16 keys on
-    auto values = [&](const TileLds<D>& t, int kk, const x8 (&p)[SUB]) {
+    // keys 4 quad + i (i < 4) of the quarter, then 16 keys on.  Reads are two
+    // tiles of 16 dims ahead of the products, the first two before the
+    // exponentials; barriers for the compiler's schedule keep them there (1% to 2%).
+    auto v_tile = [&](const TileLds<D>& t, int kk, int dt) -> x8 {
+      const s16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(t.v + 64 * kk * D + v_at[dt]));
+      const s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(t.v + (64 * kk + 32) * D + v_at[dt]));
+      return __builtin_bit_cast(x8, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto values = [&](const TileLds<D>& t, int kk, const x8 (&p)[SUB], x8 v0, x8 v1) {
+      x8 v[2] = {v0, v1};
 #pragma unroll
       for (int dt = 0; dt < kDTiles; ++dt) {
-        const s16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(t.v + 64 * kk * D + v_at[dt]));
-        const s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(t.v + (64 * kk + 32) * D + v_at[dt]));
-        const x8 vop = __builtin_bit_cast(x8, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) acc[s][dt] = product(vop, p[s], acc[s][dt]);
+        for (int s = 0; s < SUB; ++s) acc[s][dt] = product(v[dt & 1], p[s], acc[s][dt]);
+        if (dt + 2 < kDTiles) v[dt & 1] = v_tile(t, kk, dt + 2);
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
     // 32 keys that every row sees, when every row has a maximum; false, with
@@ -604,6 +611,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
     auto quick = [&](const TileLds<D>& t, int kk) -> bool {
       f32x4 sc[2][SUB];
       scores(t, kk, sc);
+      const x8 v0 = v_tile(t, kk, 0), v1 = v_tile(t, kk, 1);
+      __builtin_amdgcn_sched_barrier(0);
       x8 p[SUB];
       float sum[SUB];
       bool huge = false;
@@ -626,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
       if (__builtin_amdgcn_ballot_w64(huge)) return false;
 #pragma unroll
       for (int s = 0; s < SUB; ++s) l[s] = sum[s];
-      values(t, kk, p);
+      values(t, kk, p, v0, v1);
       return true;
     };
     // any 32 keys; k0: the first one's rank
@@ -696,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
         unset = __builtin_amdgcn_ballot_w64(none) != 0;
       }
       if (masked) clear_odd(t.v + 64 * kk * D, dead);
-      values(t, kk, p);
+      values(t, kk, p, v_tile(t, kk, 0), v_tile(t, kk, 1));
     };
     __builtin_amdgcn_s_waitcnt(0);  // (one the compiler sees: Q has arrived)
     __syncthreads();
@@ -879,10 +888,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
 }
 
 // Merges the pieces of rows that a cut went through, and the sink: WAYS x D / 4
-// lanes per (token, head), each way every WAYS-th piece, kAhead of them in flight.
-template <typename T, int D, int WAYS>
+// lanes per (token, head), each way every WAYS-th piece, AHEAD of them in flight.
+template <typename T, int D, int WAYS, int AHEAD>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a, const int block_rows) {
-  constexpr int kLanes = D / 4, kAhead = 4;
+  constexpr int kLanes = D / 4;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / (kLanes * WAYS)) + threadIdx.x / (kLanes * WAYS);
   const int d = 4 * (threadIdx.x % kLanes), way = threadIdx.x / kLanes % WAYS;
   const int64_t token = row / a.q_heads;
@@ -898,11 +907,11 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a, con
   if (first < 0 || last < first || last >= kGroups || r < 0 || r >= block_rows) return;
   float m = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int w = first + way; w <= last; w += kAhead * WAYS) {
-    f32x2 ml[kAhead];
-    f32x4 x[kAhead];
+  for (int w = first + way; w <= last; w += AHEAD * WAYS) {
+    f32x2 ml[AHEAD];
+    f32x4 x[AHEAD];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < AHEAD; ++i) {
       const int at = w + i * WAYS <= last ? w + i * WAYS : last;
       const int64_t place = (2ll * at + (at == first ? 1 : 0)) * block_rows + r;
       ml[i] = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * place);
@@ -910,7 +919,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a, con
     }
     float top = m;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) top = fmaxf(top, ml[i].x);
+    for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, ml[i].x);
     const float base = top == -INFINITY ? 0.f : top;
     // a piece without a key carries m = -inf, l = 0 and O = 0
     const float by = __builtin_amdgcn_exp2f(m - base);
@@ -918,7 +927,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a, con
     o *= by;
     m = top;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < AHEAD; ++i) {
       if (w + i * WAYS > last) continue;
       const float mine = __builtin_amdgcn_exp2f(ml[i].x - base);
       l += ml[i].y * mine;
@@ -1007,18 +1016,28 @@ void start(const TreeArgs& a, dim3 grid, hipStream_t st) {
 // Few rows are cut into many pieces each, and many rows fill the chip: a wave per
 // row up to kFewRows, D / 4 lanes beyond (both launches, us by the wave and by the
 // lanes: 512 rows of one request of 8192 keys 22.6, 31.5; 4096 rows 42.8, 44.8; 16384
-// rows of 16 requests of 4096 49.7, 46.8).
-constexpr int64_t kFewRows = 4096;
+// rows of 16 requests of 4096 49.7, 46.8).  Up to kFewestRows all of a row's pieces
+// are on their way at once, 16 per way, 4 beyond (128 rows of 128 dims over 4096 keys
+// 16.8, 18.3; 512 rows over 8192 21.1, 22.1; 4096 rows 44.2, 41.2).
+constexpr int64_t kFewRows = 4096, kFewestRows = 512;
+
+template <typename T, int D, int WAYS, int AHEAD>
+void merge_by(const TreeArgs& a, const Launch& p, hipStream_t st) {
+  constexpr int kRows = 256 / (D / 4 * WAYS);
+  const dim3 grid(static_cast<unsigned>((a.n_tokens * a.q_heads + kRows - 1) / kRows));
+  hipLaunchKernelGGL((tree_combine_kernel<T, D, WAYS, AHEAD>), grid, dim3(256), 0, st, a, 16 * kWaves * p.sub);
+}
 
 template <typename T, int D>
 void merge(const TreeArgs& a, const Launch& p, hipStream_t st) {
   constexpr int kWays = 64 / (D / 4);
-  const int64_t rows = a.n_tokens * a.q_heads, per = rows <= kFewRows ? 4 : 4 * kWays;
-  const dim3 grid(static_cast<unsigned>((rows + per - 1) / per));
-  if (rows <= kFewRows)
-    hipLaunchKernelGGL((tree_combine_kernel<T, D, kWays>), grid, dim3(256), 0, st, a, 16 * kWaves * p.sub);
+  const int64_t rows = a.n_tokens * a.q_heads;
+  if (rows <= kFewestRows)
+    merge_by<T, D, kWays, 16>(a, p, st);
+  else if (rows <= kFewRows)
+    merge_by<T, D, kWays, 4>(a, p, st);
   else
-    hipLaunchKernelGGL((tree_combine_kernel<T, D, 1>), grid, dim3(256), 0, st, a, 16 * kWaves * p.sub);
+    merge_by<T, D, 1, 4>(a, p, st);
 }
 
 template <typename T>
