@@ -14,7 +14,8 @@
 // lane swaps; a wave takes the rows of one token, 64 / lanes at a time, and
 // keeps that token's cos / sin and both weights in registers.  32768 tokens of 80
 // rows of 64 in bf16: 680 MB in 135 us, 5.0 TB/s, what a large copy reaches; 8191 of
-// 24 rows of 128: 103 MB in 22 us, 4.7 TB/s; one token 3.7 us.
+// 24 rows of 128: 103 MB in 22 us (28 from cold caches, where a copy takes 21); one
+// token 3.7 us.
 #include "common.h"
 
 namespace akv {

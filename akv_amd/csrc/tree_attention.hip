@@ -28,11 +28,11 @@
 // weights outgrow their types.
 //
 // Bound: HBM while a KV head has up to about 128 rows (16 tokens x 8 heads of 64
-// over 32 requests of 20k keys: 1.30 GB in 285-306 us, 4.3-4.6 TB/s; 5 to 32 tokens x
-// 4 heads of 128 over 12 paged requests: 0.50 GB in 126 us, 4.0 TB/s); matrix and
+// over 32 requests of 20k keys: 1.30 GB in 278-306 us, 4.3-4.7 TB/s; 5 to 32 tokens x
+// 4 heads of 128 over 12 paged requests: 0.50 GB in 124 us, 4.0 TB/s); matrix and
 // vector work above (64 tokens over 8 requests of 25k: 203 GFLOP in 255-280 us,
 // 720-800 TFLOP/s); round trips where there is little (8 tokens over 4096 keys: 13
-// us and 6 for the merge; a window's 145 keys x 32 requests: 16 us).
+// us and 4 for the merge; a window's 145 keys x 32 requests: 16 us).
 //
 // Lane layouts (verified on gfx950): v_mfma_f32_16x16x32 -- lane l supplies
 // A[l%16][k(l,i)], B[k(l,i)][l%16] for i < 8 and holds D[4(l/16)+i][l%16];
