@@ -101,8 +101,8 @@ def tree_attention(q, k_buffer, v_buffer, qo_indptr, kv_indptr, kv_indices, out,
     their fp32 sums.  Rows of ``out``, which must not overlap ``q``, behind the
     last token stay as they are.  Head dims: multiples of 8
     up to 128.  Weights are relative to a row's first scores and may grow to
-    2^64 before they are rescaled, so bf16 values that a token sees are taken
-    up to 2^62 in magnitude.  ``status``: as for ``decode_attention``.
+    2^32 before they are rescaled, so bf16 values that a token sees are taken
+    up to 2^94 in magnitude.  ``status``: as for ``decode_attention``.
     """
     # one read of every property: the checks are most of a small call's time
     dtype, at, q_shape, q_stride = q.dtype, q.get_device(), q.shape, q.stride()

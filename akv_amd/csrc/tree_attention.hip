@@ -63,7 +63,9 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kHuge = 18446744073709551616.f;  // 2^64: a weight sum above it may have overflowed the product
+// A weight sum above 2^32 takes exact maxima (the keys alone add up to 2^30).  Values
+// up to 2^94 stay finite in the products.
+constexpr float kHuge = 4294967296.f;
 
 // Keys of a tile (32 KiB of K and V), and the tiles in LDS: one is worked on while
 // the next streams in.  (Four places for half the keys, with three tiles on their
@@ -659,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
       }
       // A row's m is its maximum over the first quarter it sees a key of, and then
       // stays put: the sum tells when it should not have.  A sum past kHuge (a
-      // score ~64 above m in the log2 domain, 16 in fp16, whose weight is then
+      // score ~32 above m in the log2 domain, 16 in fp16, whose weight is then
       // infinite) takes the quarter again with exact maxima.
       x8 p[SUB];
       float sum[SUB];
@@ -672,12 +674,14 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
             const float mx = column_max(max3(m0, m1, max2(sc[1][s][2], sc[1][s][3])));
             const float over = fmaf(mx, a.scale_log2, neg_m[s]);  // above m
             const bool any = l[s] != 0.f;
+            // (a sum near kHuge whose large weights lie behind moves by 2^16)
+            const bool down = l[s] > 0.5f * kHuge && !(over > 16.f);
             const bool move = any ? over > 0.f : mx > -INFINITY;
-            const float alpha = move && any ? __builtin_amdgcn_exp2f(-over) : 1.f;
+            const float alpha = down ? 0x1p-16f : move && any ? __builtin_amdgcn_exp2f(-over) : 1.f;
             l[s] *= alpha;
 #pragma unroll
             for (int dt = 0; dt < kDTiles; ++dt) acc[s][dt] *= alpha;
-            neg_m[s] = move ? -(mx * a.scale_log2) : neg_m[s];
+            neg_m[s] = down ? neg_m[s] - 16.f : move ? -(mx * a.scale_log2) : neg_m[s];
           }
         }
         bool huge = false;

@@ -402,3 +402,36 @@ def test_any_workspace_contents(device, fill):
     _check(c, first, c.visible(seen))
     for _ in range(3):  # sums are in a fixed order
         assert torch.equal(_run(c, mask=mask, workspace=ws), first)
+
+
+@pytest.mark.parametrize("bound", [1, 5000])
+def test_large_values_under_rising_scores(device, bound):
+    """bf16 values of 2^90 and below, weights of up to 2^31 against the first keys'."""
+    c = Cache(device, 950, [1500], [5], q_heads=4, kv_heads=2, head_dim=64, dtype=torch.bfloat16)
+    c.k[:] = 0.01 * c.k
+    c.q[:] = 0.01 * c.q
+    c.q[:, :, 0] = 2.0
+    c.k[torch.from_numpy(c.slots[0]), :, 0] = torch.linspace(0, 10, 1505).to(torch.bfloat16)[:, None]
+    c.v *= 2.0 ** 88
+    seen, mask = c.masks("tree")
+    out = _run(c, mask=mask, scale=1.0, out_dtype=torch.float32, max_len=bound)
+    assert torch.isfinite(out).all()
+    _check(c, out, c.visible(seen), scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bound", [1, 9000])
+def test_sums_that_stay_large(device, bound, dtype):
+    """A few keys whose weights nearly fill the sum's range against the first
+    ones', among thousands that are close to those."""
+    c = Cache(device, 960, [6000], [5], q_heads=4, kv_heads=2, head_dim=64, dtype=dtype)
+    c.k[:] = 0.01 * c.k
+    c.q[:] = 0.01 * c.q
+    c.q[:, :, 0] = 2.0
+    level = torch.zeros(6005)
+    level[64:] = 0.02 * torch.rand(6005 - 64, generator=torch.Generator().manual_seed(1))
+    # log2 weights of 31.7 (beside the sum's limit), of 15.9 (beside fp16's)
+    level[100:104] = (31.7 if dtype == torch.bfloat16 else 15.9) / 2 / np.log2(np.e)
+    c.k[torch.from_numpy(c.slots[0]), :, 0] = level.to(dtype)[:, None]
+    seen, mask = c.masks("tree")
+    _check(c, _run(c, mask=mask, scale=1.0, out_dtype=torch.float32, max_len=bound), c.visible(seen), scale=1.0)
