@@ -435,3 +435,17 @@ def test_sums_that_stay_large(device, bound, dtype):
     c.k[torch.from_numpy(c.slots[0]), :, 0] = level.to(dtype)[:, None]
     seen, mask = c.masks("tree")
     _check(c, _run(c, mask=mask, scale=1.0, out_dtype=torch.float32, max_len=bound), c.visible(seen), scale=1.0)
+
+
+@pytest.mark.parametrize("bound", [1, 5000])
+def test_a_stretch_of_a_larger_batch(device, bound):
+    """Indptrs that begin past zero: the rows and entries before stay out of it."""
+    c = Cache(device, 970, [700, 30], [6, 9], q_heads=8, kv_heads=2, head_dim=64, dtype=torch.bfloat16)
+    seen, mask = c.masks("any")
+    alone = _run(c, mask=mask, max_len=bound)
+    _check(c, alone, c.visible(seen))
+    pad = lambda t, n: torch.cat((torch.full((n, *t.shape[1:]), 5, dtype=t.dtype, device=device), t))  # noqa: E731
+    q, out = pad(c.q, 3), torch.full((c.total + 3, 8, 64), 7.0, dtype=torch.bfloat16, device=device)
+    attention.tree_attention(q, c.k.to(device), c.v.to(device), c.qo + 3, c.kv + 4, pad(c.indices, 4), out, scale=0.125,
+                             max_len=bound, max_new=9, tree_mask=pad(mask, 3))
+    assert (out[:3] == 7).all() and torch.equal(out[3:], alone)
