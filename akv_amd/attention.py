@@ -71,7 +71,8 @@ def decode_attention(q, k_buffer, v_buffer, kv_indptr, kv_indices, out, *, scale
 
 
 def tree_workspace_bytes(n_tokens, n_requests, q_heads, kv_heads, head_dim, max_len, max_new):
-    """Device bytes ``tree_attention`` needs for these sizes and bounds."""
+    """Device bytes ``tree_attention`` needs for every batch of up to these
+    tokens and requests, under bounds of up to these."""
     need = _lib.calls().akv_tree_attention_workspace_bytes(n_tokens, n_requests, q_heads, kv_heads, head_dim, max_len,
                                                            max_new)
     if need < 0:

@@ -986,11 +986,16 @@ struct Launch {
 // 63 of 100: 25.0, 29.5; 65 requests of 1024, a round and a bit: 47.9, 45.5).
 constexpr int64_t kWholeTiles = 4, kWholeKeys = 1024, kWholeGroups = 128;
 
+// Rows of a KV head that a request may have.
+int64_t most_rows(int64_t n_tokens, int64_t q_heads, int64_t kv_heads, int64_t max_new) {
+  return std::max<int64_t>(1, std::min(max_new, n_tokens)) * (q_heads / kv_heads);
+}
+
 Launch plan(int64_t n_tokens, int64_t n_requests, int64_t q_heads, int64_t kv_heads, int32_t head_dim,
             int64_t max_len, int64_t max_new) {
   Launch p;
   p.d = tile_dim(head_dim);
-  const int64_t rows = std::max<int64_t>(1, std::min(max_new, n_tokens)) * (q_heads / kv_heads);
+  const int64_t rows = most_rows(n_tokens, q_heads, kv_heads, max_new);
   p.sub = subtiles_for(p.d, rows);
   auto blocks = [&]() -> int64_t { return (rows + 16 * kWaves * p.sub - 1) / (16 * kWaves * p.sub); };
   p.whole = max_len <= kWholeTiles * keys_of(p.d) ||
@@ -1004,9 +1009,22 @@ Launch plan(int64_t n_tokens, int64_t n_requests, int64_t q_heads, int64_t kv_he
 
 int64_t owner_bytes(int64_t n_tokens, int64_t q_heads) { return 16 * n_tokens * q_heads; }
 
+int64_t cut_bytes(int d, int sub, int64_t n_tokens, int64_t q_heads) {
+  return owner_bytes(n_tokens, q_heads) + 2ll * kGroups * (16 * kWaves * sub) * (d + 2) * 4;
+}
+
+// What a launch needs.
 int64_t partial_bytes(const Launch& p, int64_t n_tokens, int64_t q_heads) {
-  if (p.whole) return 16;
-  return owner_bytes(n_tokens, q_heads) + 2ll * kGroups * (16 * kWaves * p.sub) * (p.d + 2) * 4;
+  return p.whole ? 16 : cut_bytes(p.d, p.sub, n_tokens, q_heads);
+}
+
+// What every batch of up to these sizes and bounds needs: a batch that fills the
+// chip runs whole, but one of fewer requests under the same bounds is cut.
+int64_t largest_bytes(int64_t n_tokens, int64_t q_heads, int64_t kv_heads, int32_t head_dim, int64_t max_len,
+                      int64_t max_new) {
+  const int d = tile_dim(head_dim);
+  if (max_len <= kWholeTiles * keys_of(d)) return 16;
+  return cut_bytes(d, subtiles_for(d, most_rows(n_tokens, q_heads, kv_heads, max_new)), n_tokens, q_heads);
 }
 
 template <typename T, int D, int SUB>
@@ -1080,8 +1098,7 @@ extern "C" int64_t akv_tree_attention_workspace_bytes(int64_t n_tokens, int32_t 
                                                        int64_t max_new) {
   using namespace akv;
   if (!sizes_ok(n_tokens, n_requests, q_heads, kv_heads, head_dim, max_len, max_new)) return -1;
-  return partial_bytes(plan(n_tokens, n_requests, q_heads, kv_heads, head_dim, max_len, max_new), n_tokens,
-                       q_heads);
+  return largest_bytes(n_tokens, q_heads, kv_heads, head_dim, max_len, max_new);
 }
 
 extern "C" int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_buffer,

@@ -835,8 +835,10 @@ int akv_qk_norm_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  * for the order of their fp32 sums).  A request has up to 2^30 keys; out must
  * not overlap q.
  * n_tokens is the capacity of q and out; rows behind qo_indptr[B] stay as they
- * are.  workspace: akv_tree_attention_workspace_bytes with the same arguments,
- * 16-byte aligned, any contents; calls that share one must not overlap.
+ * are.  workspace: akv_tree_attention_workspace_bytes with the same arguments
+ * or with larger n_tokens, n_requests, max_len and max_new (it does not fall as
+ * they grow), 16-byte aligned, any contents; calls that share one must not
+ * overlap.
  * status as in akv_decode_attention.
  *
  * The reference rejects speculative decoding

@@ -238,3 +238,37 @@ def _maps(**change):
 def test_step_maps_refuse(change, message):
     with pytest.raises(ValueError, match=message):
         _maps(**change)
+
+
+def _need(q_heads, kv_heads, head_dim, requests, tokens, max_len, max_new):
+    """What the call itself asks for: it is refused without."""
+    assert _call("akv_tree_attention", q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, n_requests=requests,
+                 n_tokens=tokens, max_len=max_len, max_new=max_new, workspace_bytes=0) == _lib.AKV_EINVAL
+    words = _lib.last_error().split()
+    assert words[-2] == "needs"
+    return int(words[-1])
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,head_dim", [(64, 8, 64), (32, 8, 128), (8, 1, 64), (4, 4, 96)])
+def test_a_workspace_serves_every_smaller_batch(q_heads, kv_heads, head_dim):
+    """On both sides of the launch rules: 128 workgroups, 4 tiles, 1024 keys,
+    rows of one to four subtiles."""
+    lens = (1, 256, 257, 512, 513, 1000, 1024, 1025, 30000)
+    for max_new in (1, 8, 9, 40, 300):
+        before = 0
+        for max_len in lens:
+            sizes = [attention.tree_workspace_bytes(r * t, r, q_heads, kv_heads, head_dim, max_len, max_new)
+                     for r in (1, 2, 15, 16, 17, 127, 128, 129, 600) for t in (max_new,)]
+            assert sizes == sorted(sizes) and sizes[0] >= 16
+            assert sizes[0] >= before
+            before = sizes[0]
+            whole = sizes[-1]
+            for requests in (1, 15, 16, 32, 128, 600):
+                for tokens in (requests, requests * max_new):
+                    for bound in (b for b in lens if b <= max_len):
+                        for new in (1, max_new):
+                            assert _need(q_heads, kv_heads, head_dim, requests, tokens, bound, new) <= whole
+    for max_len in lens:
+        sizes = [attention.tree_workspace_bytes(4000, 16, q_heads, kv_heads, head_dim, max_len, n)
+                 for n in (1, 2, 5, 8, 9, 17, 64, 65, 300)]
+        assert sizes == sorted(sizes)
