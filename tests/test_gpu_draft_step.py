@@ -260,3 +260,86 @@ def test_stored_keys_move_as_the_reposition_moves_them(device):
     tol = 2.0 ** -8 * 1.5 * pair + 2.0 ** -8 * np.abs(want) + 1e-5 * pair
     assert (np.abs(f64(s.k[dst.long()]) - want) <= tol).all()
     assert torch.equal(s.v[dst.long()], s.v[src.long()])
+
+
+class CutStep(Step):
+    """A step whose full layer is cut into pieces and merged: its bound is past
+    what one workgroup takes, as a server's is, however short the requests are."""
+
+    def __init__(self, *args, max_len=5000, **more):
+        super().__init__(*args, max_len=max_len, **more)
+        assert self.workspace.numel() > 16
+
+    def check(self):
+        # errors are counted by the keys that are there
+        bound, self.max_len = self.max_len, max(np.add(self.old, self.new))
+        super().check()
+        self.max_len = bound
+
+
+@pytest.mark.parametrize("d,q_heads,page", [(64, 8, 1), (64, 16, 16), (128, 8, 1)])
+def test_cut_step_in_order(device, d, q_heads, page):
+    s = CutStep(device, 41, [400, 0, 33, 290], [9, 4, 16, 1], page=page, d=d, q_heads=q_heads)
+    s.run()
+    s.check()
+    s.set(42, [5, 700, 64], [16, 2, 7])
+    s.run()
+    s.check()
+
+
+def test_cut_padded_batch(device):
+    s = CutStep(device, 43, [500, 140], [7, 5], capacity=40, requests=6)
+    pool = s.k.clone()
+    s.out.fill_(7)
+    s.run()
+    s.check()
+    assert (s.out[12:] == 7).all()
+    untouched = torch.ones(s.k.shape[0], dtype=torch.bool, device=device)
+    untouched[s.slot_map[:12]] = False
+    assert torch.equal(s.k[untouched], pool[untouched])
+
+
+def test_cut_steps_on_streams_beside_each_other(device):
+    """Each stream with its own workspace: neither's pieces reach the other."""
+    steps = [CutStep(device, 50 + i, [700, 120 + i], [16, 9]) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device) for _ in steps]
+    for _ in range(20):
+        for s, stream in zip(steps, streams):
+            with torch.cuda.stream(stream):
+                s.run()
+    torch.cuda.synchronize()
+    for s in steps:
+        s.check()
+
+
+def test_cut_captured_steps_share_a_workspace(device):
+    """Two graphs over one workspace, replayed in turn for batches that leave
+    other pieces and owners in it, with eager work of the same between them."""
+    s = CutStep(device, 60, [400, 60, 7], [8, 3, 16], capacity=48, requests=5)
+    eager = CutStep(device, 60, [400, 60, 7], [8, 3, 16], capacity=48, requests=5)
+    eager.workspace = s.workspace
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(side):
+        s.run()
+    torch.cuda.current_stream(device).wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            s.run()
+        graphs.append(graph)
+    batches = [([400, 60, 7], [8, 3, 16]), ([900], [16]), ([0, 1, 2, 3, 4], [1, 2, 3, 4, 5]), ([30, 0, 500], [0, 16, 6])]
+    for i, (old, new) in enumerate(batches * 2):
+        print(f"cut captured step, replay {i}", flush=True)
+        for t in (s, eager):
+            t.set(70 + i, old, new)
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        s.check()
+        eager.k.copy_(s.k), eager.v.copy_(s.v)
+        eager.run()
+        torch.cuda.synchronize()
+        total = sum(new)
+        assert torch.equal(s.out[:total], eager.out[:total]) and torch.equal(s.win[:total], eager.win[:total])

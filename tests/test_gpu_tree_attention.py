@@ -449,3 +449,15 @@ def test_a_stretch_of_a_larger_batch(device, bound):
     attention.tree_attention(q, c.k.to(device), c.v.to(device), c.qo + 3, c.kv + 4, pad(c.indices, 4), out, scale=0.125,
                              max_len=bound, max_new=9, tree_mask=pad(mask, 3))
     assert (out[:3] == 7).all() and torch.equal(out[3:], alone)
+
+
+def test_one_workspace_while_a_batch_drains(device):
+    """Sized once for the full batch, which runs whole; its last requests are cut."""
+    shape = dict(q_heads=16, kv_heads=4, head_dim=64, dtype=torch.bfloat16)
+    need = attention.tree_workspace_bytes(4 * 40, 40, 16, 4, 64, 1000, 4)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device=device)
+    for requests in (40, 32, 31, 3, 1):
+        print(f"tree attention, {requests} requests of 40", flush=True)
+        c = Cache(device, 980 + requests, [(37 * i) % 130 + 800 * (i == 0) for i in range(requests)], [4] * requests, **shape)
+        seen, mask = c.masks("tree")
+        _check(c, _run(c, mask=mask, workspace=ws, max_len=1000), c.visible(seen))
