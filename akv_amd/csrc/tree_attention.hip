@@ -64,7 +64,8 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
 // A weight sum above 2^32 takes exact maxima (the keys alone add up to 2^30).  Values
-// up to 2^94 stay finite in the products.
+// up to 2^94 stay finite in a wave's products; waves and pieces are joined by shares
+// of their sums, which stay between the values.
 constexpr float kHuge = 4294967296.f;
 
 // Keys of a tile (32 KiB of K and V), and the tiles in LDS: one is worked on while
@@ -105,7 +106,7 @@ struct TreeArgs {
   float scale_log2;
   void* out;
   int64_t o_st, o_sh;
-  float* part_o;   // [2 kGroups][rows of a block][D]
+  float* part_o;   // [2 kGroups][rows of a block][D], each divided by its piece's sum
   float* part_ml;  // [2 kGroups][rows of a block][2]
   int32_t* owner;  // [tokens][q heads][4]: the workgroups with the row's first (-1: all) and last keys, its row
   int64_t n_tokens, max_len;
@@ -787,11 +788,11 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
           lt = lt * by + (top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - top));
           scale = by;
         }
-        scale *= inverse(lt);
         s_out[mine] = row * a.o_st + head * a.o_sh;
       } else {
         *reinterpret_cast<f32x2*>(part_ml + 2 * mine) = f32x2{m, lt};
       }
+      scale *= inverse(lt);
       for (int w = group; w < kWaves; w += groups) s_m[w][in] = __builtin_amdgcn_exp2f(s_m[w][in] - base) * scale;
       if (!a.whole) {
         int32_t* owner = a.owner + 4 * (row * a.q_heads + head);
@@ -910,7 +911,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a, con
   // (indptrs that descend leave rows without owners)
   if (first < 0 || last < first || last >= kGroups || r < 0 || r >= block_rows) return;
   float m = -INFINITY, l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};  // of the pieces so far, divided by l
   for (int w = first + way; w <= last; w += AHEAD * WAYS) {
     f32x2 ml[AHEAD];
     f32x4 x[AHEAD];
@@ -926,33 +927,36 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a, con
     for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, ml[i].x);
     const float base = top == -INFINITY ? 0.f : top;
     // a piece without a key carries m = -inf, l = 0 and O = 0
-    const float by = __builtin_amdgcn_exp2f(m - base);
-    l *= by;
-    o *= by;
+    const float kept = l * __builtin_amdgcn_exp2f(m - base);
+    l = kept;
     m = top;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      if (w + i * WAYS > last) continue;
-      const float mine = __builtin_amdgcn_exp2f(ml[i].x - base);
-      l += ml[i].y * mine;
-      o += x[i] * mine;
+      ml[i].y = w + i * WAYS <= last ? ml[i].y * __builtin_amdgcn_exp2f(ml[i].x - base) : 0.f;
+      l += ml[i].y;
     }
+    const float inv = inverse(l);
+    o *= kept * inv;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (w + i * WAYS <= last) o += x[i] * (ml[i].y * inv);
   }
   float top = fmaxf(m, sink);
 #pragma unroll
   for (int off = kLanes; off < kLanes * WAYS; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
   const float base = top == -INFINITY ? 0.f : top;
-  const float by = __builtin_amdgcn_exp2f(m - base);
-  l *= by;
-  o *= by;
+  const float mine = l * __builtin_amdgcn_exp2f(m - base);
+  l = mine;
+#pragma unroll
+  for (int off = kLanes; off < kLanes * WAYS; off <<= 1) l += __shfl_xor(l, off);
+  if (a.sinks) l += __builtin_amdgcn_exp2f(sink - base);
+  o *= mine * inverse(l);
 #pragma unroll
   for (int off = kLanes; off < kLanes * WAYS; off <<= 1) {
-    l += __shfl_xor(l, off);
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], off);
   }
-  if (a.sinks) l += __builtin_amdgcn_exp2f(sink - base);
-  if (way == 0 && d < a.head_dim) store_four<T>(a, token * a.o_st + head * a.o_sh + d, o * inverse(l));
+  if (way == 0 && d < a.head_dim) store_four<T>(a, token * a.o_st + head * a.o_sh + d, o);
 }
 
 int tile_dim(int32_t head_dim) { return head_dim <= 64 ? 64 : 128; }

@@ -461,3 +461,33 @@ def test_one_workspace_while_a_batch_drains(device):
         c = Cache(device, 980 + requests, [(37 * i) % 130 + 800 * (i == 0) for i in range(requests)], [4] * requests, **shape)
         seen, mask = c.masks("tree")
         _check(c, _run(c, mask=mask, workspace=ws, max_len=1000), c.visible(seen))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_largest_values_in_every_piece(device, d):
+    """bf16 values of 2^94, in pieces that each begin with low scores and end with
+    a weight of 2^31.9 against them in every wave: 512 pieces of 8 units (a piece's
+    tiles of 128 / 64 keys, with 2 / 3 units before the first one).  All values of a
+    dim are equal, so the result is that value whatever the weights: each wave's
+    sums of weights and of weighted values add some 40 terms each, their joining
+    512 and about 64 products, each off by 2^-24."""
+    keys = 128 if d == 64 else 64
+    ahead = 2 if d == 64 else 3
+    tiles = 512 * 8 - ahead
+    n_keys, n, heads = tiles * keys, 2, 4
+    k = torch.zeros((n_keys, 1, d), dtype=torch.bfloat16, device=device)
+    rank = torch.arange(n_keys, device=device)
+    k[(rank // keys % 8 == 7 - ahead) & (rank % 32 == 9), 0, 0] = 11.0625  # 2 x 11.0625 x log2(e) = 31.92
+    value = torch.tensor([2.0 ** 94, -2.0 ** 94, 1.0, 2.0 ** -90], device=device).repeat(d // 4).to(torch.bfloat16)
+    v = value.expand(n_keys, 1, d).contiguous()
+    q = torch.zeros((n, heads, d), dtype=torch.bfloat16, device=device)
+    q[:, :, 0] = 2.0
+    out = torch.empty((n, heads, d), dtype=torch.float32, device=device)
+    indptr = lambda x: torch.tensor([0, x], dtype=torch.int32, device=device)  # noqa: E731
+    for sinks in (None, torch.full((heads,), 2.0, device=device)):
+        attention.tree_attention(q, k, v, indptr(n), indptr(n_keys), rank.int(), out, scale=1.0, max_len=n_keys,
+                                 max_new=n, sinks=sinks)
+        # (e^2 beside more than 512 weights of e^22)
+        tol = 656 * 2.0 ** -24 + (0 if sinks is None else np.exp(2 - 22.125) / 512)
+        worst = ((out - value.float()).abs() / value.float().abs()).max().item()
+        assert worst <= tol, f"off by {worst:.3g} of the value, {tol:.3g} allowed"
