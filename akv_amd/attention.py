@@ -93,8 +93,8 @@ def tree_attention(q, k_buffer, v_buffer, qo_indptr, kv_indptr, kv_indices, out,
     the pages of row b of a 2-D block table (``context_step_maps``), with
     ``page_size`` slots each.  Token i sees the request's earlier keys from
     rank ``key_starts[i]`` on (None: all), and of the drafted tokens those whose
-    bit is set in its ``tree_mask`` row (int64 words ``[N, words]``; None: a
-    chain, each token itself and those before it).  A token that sees no key
+    bit is set in its ``tree_mask`` row (int64 words ``[N, words]``, 0 past the
+    last; None: a chain, each token itself and those before it).  A token that sees no key
     gets 0; a key at a slot outside the pool is seen by none.  ``sinks``: f32
     ``[q_heads]``.  ``max_len`` (keys a request's tokens reach: its keys, or
     window + n + 1) and ``max_new`` (its tokens) are host bounds that size the
@@ -141,7 +141,8 @@ def tree_attention(q, k_buffer, v_buffer, qo_indptr, kv_indptr, kv_indices, out,
         if tree_mask.dtype != torch.int64 or len(mask_shape) != 2 or mask_shape[0] != n \
                 or (mask_stride[1] != 1 and tree_mask.numel()) or tree_mask.get_device() != at:
             raise ValueError("tree_mask must be int64 words [tokens, words] on q's device")
-        mask_args = (tree_mask.data_ptr(), mask_stride[0], mask_shape[1])
+        # (an empty tensor has no address, and no address is a chain: words of none are never read)
+        mask_args = (tree_mask.data_ptr() or q_ptr, mask_stride[0], mask_shape[1])
     if key_starts is not None and (key_starts.dtype != torch.int32 or key_starts.ndim != 1 or key_starts.numel() != n
                                    or not key_starts.is_contiguous() or key_starts.get_device() != at):
         raise ValueError("key_starts must be contiguous int32 [tokens] on q's device")

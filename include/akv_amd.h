@@ -820,7 +820,8 @@ int akv_qk_norm_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  * q[qo_indptr[b] .. qo_indptr[b + 1]), n of them; its kv_indptr[b + 1] -
  * kv_indptr[b] keys end in the tokens' own n.  Token i sees an earlier key of
  * rank j when j >= key_starts[token] (NULL: always), and the request's new
- * token a when bit a of its tree_mask row is set (NULL: a <= i).  GQA, scaled
+ * token a when bit a of its tree_mask row is set (mask_words 64-bit words, bits
+ * past them are 0; NULL: a <= i).  GQA, scaled
  * scores, sinks in the denominator as in akv_decode_attention; a token that
  * sees no key gets 0.  q, K and V are bf16 or fp16, the output q's type or
  * f32; head_dim a multiple of 8 up to 128, any number of q heads per KV head.

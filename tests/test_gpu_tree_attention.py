@@ -491,3 +491,14 @@ def test_largest_values_in_every_piece(device, d):
         tol = 656 * 2.0 ** -24 + (0 if sinks is None else np.exp(2 - 22.125) / 512)
         worst = ((out - value.float()).abs() / value.float().abs()).max().item()
         assert worst <= tol, f"off by {worst:.3g} of the value, {tol:.3g} allowed"
+
+
+@pytest.mark.parametrize("bound", [1, 5000])
+def test_a_mask_without_words_shows_no_drafted_token(device, bound):
+    c = Cache(device, 990, [700, 0, 40], [6, 3, 9], q_heads=8, kv_heads=2, head_dim=64, dtype=torch.bfloat16)
+    none = [np.zeros((n, n), dtype=bool) for n in c.new]
+    mask = torch.zeros((c.total, 0), dtype=torch.int64, device=device)
+    _check(c, _run(c, mask=mask, max_len=bound), c.visible(none))
+    # the words of a wider store, none of them taken
+    store = torch.full((c.total, 2), -1, dtype=torch.int64, device=device)
+    _check(c, _run(c, mask=store[:, :0], max_len=bound), c.visible(none))
