@@ -367,10 +367,11 @@ extern "C" int akv_qk_norm_rope(const void* q, int64_t q_stride_t, int64_t q_str
   if (static_cast<int64_t>(q_heads) + 2 * static_cast<int64_t>(kv_heads) > 65535)
     return fail(AKV_EINVAL, "akv_qk_norm_rope: %d q and %d KV heads", q_heads, kv_heads);
   if (n_tokens == 0 || q_heads + kv_heads == 0) return AKV_OK;
-  const bool pool = k_pool || v_pool;
+  // (a pool without slots need not have an address: it takes no row)
+  const bool pool = k_pool || v_pool || (slots && pool_slots == 0);
   if ((q_heads && (!q || !q_out)) || (kv_heads && !k) || !positions || !cos_sin)
     return fail(AKV_EINVAL, "akv_qk_norm_rope: null device pointer");
-  if (pool && (!k_pool || !v_pool || !v || !slots))
+  if (pool && ((pool_slots > 0 && (!k_pool || !v_pool)) || (kv_heads && !v) || !slots))
     return fail(AKV_EINVAL, "akv_qk_norm_rope: the pool needs K, V and slots");
   if (kv_heads && !pool && !k_out) return fail(AKV_EINVAL, "akv_qk_norm_rope: the keys have nowhere to go");
   NormArgs a{};

@@ -307,7 +307,7 @@ extern "C" int akv_step_maps(const int64_t* registry, const int32_t* table, int6
   if ((window_mask || window_starts) && (window < 0 || window >= (1ll << 31)))
     return fail(AKV_EINVAL, "akv_step_maps: the window's outputs need a window of [0, 2^31)");
   if (!qo_indptr || !kv_indptr || (n_tokens > 0 && (!slot_map || !positions)) ||
-      (n_requests > 0 && (!registry || !table || !rows || !seq_lens || !new_lens)))
+      (n_requests > 0 && (!registry || (table_width > 0 && !table) || !rows || !seq_lens || !new_lens)))
     return fail(AKV_EINVAL, "akv_step_maps: null device pointer");
   MapArgs a{};
   a.registry = registry;

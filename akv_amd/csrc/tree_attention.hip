@@ -1134,7 +1134,9 @@ extern "C" int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_s
   if (table_stride == 0 && page_size != 1)
     return fail(AKV_EINVAL, "akv_tree_attention: pages need a block table (a list holds one slot per key)");
   if (!(scale > 0.f) || std::isinf(scale)) return fail(AKV_EINVAL, "akv_tree_attention: scale must be positive and finite");
-  if (!q || !k_buffer || !v_buffer || !qo_indptr || !kv_indptr || !kv_indices || !out || !workspace)
+  // (an empty pool or list need not have an address: every key is a hole then)
+  if (!q || (pool_slots > 0 && (!k_buffer || !v_buffer)) || !qo_indptr || !kv_indptr ||
+      (table_width > 0 && !kv_indices) || !out || !workspace)
     return fail(AKV_EINVAL, "akv_tree_attention: null device pointer");
   if ((q_stride_t | q_stride_h | k_stride_slot | k_stride_head | v_stride_slot | v_stride_head) % 8 != 0 ||
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_buffer) |

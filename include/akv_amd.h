@@ -791,7 +791,8 @@ int akv_step_maps(const int64_t* registry, const int32_t* table,
  * q_out (which may be q), k rows to k_out (which may be k; NULL: nowhere) and,
  * with pools, to k_pool[slots[t]]; v rows are copied to v_pool[slots[t]].  A
  * slot outside [0, pool_slots) writes no pool row.  A position outside
- * [0, rope_rows) gives NaN rows and no K pool row.  A NULL weight is 1.
+ * [0, rope_rows) gives NaN rows and no K pool row.  A NULL weight is 1.  Pools
+ * of no slots may be NULL beside slots: the keys then go to k_out alone.
  * Strides are in elements, the last dimension's is 1; slots are distinct.
  *
  * No counterpart in the reference, whose engine's model code norms and rotates
@@ -831,7 +832,7 @@ int akv_qk_norm_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  * row kv_indices + b * table_stride of table_width pages:
  * page(j / page_size) * page_size + j % page_size.  A key whose slot lies
  * outside [0, pool_slots), or whose entry outside the list, is seen by no
- * token.  max_len (keys a request's tokens reach) and max_new (its tokens) are
+ * token (a pool or list of none may be NULL).  max_len (keys a request's tokens reach) and max_new (its tokens) are
  * host bounds that only size the launch: results do not depend on them (but
  * for the order of their fp32 sums).  A request has up to 2^30 keys; out must
  * not overlap q.

@@ -272,3 +272,16 @@ def test_a_workspace_serves_every_smaller_batch(q_heads, kv_heads, head_dim):
         sizes = [attention.tree_workspace_bytes(4000, 16, q_heads, kv_heads, head_dim, max_len, n)
                  for n in (1, 2, 5, 8, 9, 17, 64, 65, 300)]
         assert sizes == sorted(sizes)
+
+
+@pytest.mark.parametrize("name,change,message", [
+    ("akv_tree_attention", dict(k_buffer=None), "null device pointer"),
+    ("akv_tree_attention", dict(kv_indices=None, table_width=1), "null device pointer"),
+    ("akv_qk_norm_rope", dict(v_pool=None), "the pool needs"),
+    ("akv_qk_norm_rope", dict(k_pool=None, v_pool=None, pool_slots=1), "nowhere to go"),
+    ("akv_qk_norm_rope", dict(k_pool=None, v_pool=None, pool_slots=0, slots=None), "nowhere to go"),
+    ("akv_step_maps", dict(table=None), "null device pointer"),
+])
+def test_no_address_is_for_nothing_alone(name, change, message):
+    assert _call(name, **change) == _lib.AKV_EINVAL
+    assert message in _lib.last_error()

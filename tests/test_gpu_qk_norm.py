@@ -182,3 +182,21 @@ def test_around_the_split_of_a_token(device, n, d, dtype):
     qk_norm.qk_norm_rope(c["q"], c["k"], c["v"], *c["w"], c["positions"], c["table"], q_out, k_out=k_out,
                          slot_map=c["slots"], k_buffer=c["pool"][0], v_buffer=c["pool"][1])
     _check(c, q_out, k_out)
+
+
+@pytest.mark.parametrize("d", [64, 40])
+def test_a_pool_without_slots(device, d):
+    """Every token's slot is outside it: the call is the one without a pool."""
+    gen = torch.Generator().manual_seed(d)
+    q, k, v = (torch.randn(7, h, d, generator=gen).to(torch.bfloat16).to(device) for h in (4, 2, 2))
+    table = torch.randn(9, d, generator=gen).to(device)
+    positions, slots = torch.arange(7, device=device), torch.arange(7, device=device)
+    pools = [torch.empty(0, 2, d, dtype=torch.bfloat16, device=device) for _ in range(2)]
+    assert pools[0].data_ptr() == 0
+    outs = [(torch.empty_like(q), torch.empty_like(k)) for _ in range(3)]
+    qk_norm.qk_norm_rope(q, k, None, None, None, positions, table, outs[0][0], k_out=outs[0][1])
+    pool = dict(slot_map=slots, k_buffer=pools[0], v_buffer=pools[1])
+    qk_norm.qk_norm_rope(q, k, v, None, None, positions, table, outs[1][0], k_out=outs[1][1], **pool)
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    qk_norm.qk_norm_rope(q, k, v, None, None, positions, table, outs[2][0], **pool)
+    assert torch.equal(outs[0][0], outs[2][0])

@@ -194,3 +194,11 @@ def test_long_requests_on_both_sides_of_the_batch_rule(device, copies):
         np.testing.assert_array_equal(positions.cpu().numpy(), np.concatenate(want["positions"]))
         if window:
             np.testing.assert_array_equal(starts.cpu().numpy(), np.concatenate(want["starts"]))
+
+
+def test_side_rows_beside_a_table_without_columns(device):
+    """Requests whose rows all lie elsewhere: the table need not hold anything."""
+    b = Batch(device, 30, [0, 50, 0, 9], [0, 4, 0, 3], kept=[0, 1, 0, 0], side=True)
+    b.table = b.table[:, :0].clone()
+    assert b.table.data_ptr() == 0
+    _run(b, window=20)

@@ -502,3 +502,27 @@ def test_a_mask_without_words_shows_no_drafted_token(device, bound):
     # the words of a wider store, none of them taken
     store = torch.full((c.total, 2), -1, dtype=torch.int64, device=device)
     _check(c, _run(c, mask=store[:, :0], max_len=bound), c.visible(none))
+
+
+@pytest.mark.parametrize("bound", [1, 5000])
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("d", [64, 128, 40])
+def test_pools_and_lists_of_nothing(device, bound, page, d):
+    """A pool without slots, and a list or block table without entries: holes alone."""
+    c = Cache(device, 995, [700, 3], [6, 9], q_heads=8, kv_heads=2, head_dim=d, dtype=torch.bfloat16, page=page)
+    seen, mask = c.masks("tree")
+    sinks = torch.zeros(8, device=device)
+    for kind in ("pool", "list"):
+        print(f"tree attention without a {kind}, bound {bound} page {page} d {d}", flush=True)
+        k, v = c.k.to(device), c.v.to(device)
+        indices = c.indices
+        if kind == "pool":
+            k, v = k[:0].clone(), v[:0].clone()
+            assert k.data_ptr() == 0
+        else:
+            c.indices = indices[..., :0].contiguous()
+            assert c.indices.data_ptr() == 0
+        for s in (None, sinks):
+            out = _run(c, mask=mask, k=k, v=v, sinks=s, max_len=bound)
+            assert (out[: c.total] == 0).all()
+        c.indices = indices
