@@ -9,14 +9,17 @@
 // the call writes
 //   qo_indptr, kv_indptr   cumulative sums of n and L
 //   slot_map[qo + i]       slot(L - n + i), -1 behind the last token
-//   positions[qo + i]      pos(L - n) + depth(i), 0 behind the last token
+//   positions[qo + i]      pos(L - n) + depth(i), without parents pos(L - n + i);
+//                          0 behind the last token
 //   block_tables[b][j]     slot(j P) / P for j P < L, -1 behind
 //   tree_mask[qo + i]      bits of the request's new tokens: i and its ancestors
-//   window_mask[qo + i]    those at most `window` levels up
+//   window_mask[qo + i]    those whose position is at least positions[qo + i] - window
 //   window_starts[qo + i]  first rank of [0, L - n) whose position is at least
 //                          positions[qo + i] - window
-// where depth(i) is the length of i's path through `parents` (without them the
-// chain i - 1: depth i).
+// where depth(i) is the length of i's path through `parents` (so an ancestor's
+// position is as many less as it is levels up).  Without them token i follows
+// i - 1; behind the registry's active ranks its position is one more, among them
+// (a chunk of a prompt with dropped spans) it may be further.
 //
 // One launch.  Grid (token blocks + table blocks, B + 1): the first workgroups
 // of request b share its tokens, the others its block table; row B fills what
@@ -181,16 +184,26 @@ __device__ __forceinline__ void token_maps(const MapArgs& a, int b) {
   for (int64_t i = begin + tid; i < n; i += static_cast<int64_t>(a.token_blocks) * kThreads) {
     const int64_t t = tok0 + i;
     store_index(a.slot_map, a.slots64, t, r.slot_at(r.raw_of(old + i)));
-    int64_t depth = 0;
     uint64_t* tree = a.tree_mask ? a.tree_mask + t * a.tree_stride : nullptr;
     uint64_t* near = a.window_mask ? a.window_mask + t * a.near_stride : nullptr;
+    int64_t pos;
     if (!a.parents) {
-      depth = i;
+      pos = r.pos_of(old + i);
+      int64_t lo = i - a.window;
+      if (near && r.raw_ids && old < r.active) {
+        // among active ranks: positions ascend, maybe by more than one
+        int64_t hi = i;
+        lo = lo < 0 ? 0 : lo;
+        while (lo < hi) {
+          const int64_t mid = (lo + hi) >> 1;
+          if (r.pos_of(old + mid) < pos - a.window) lo = mid + 1; else hi = mid;
+        }
+      }
       for (int w = 0; tree && w < a.tree_words; ++w) tree[w] = bits_of(0, i, w);
-      for (int w = 0; near && w < a.near_words; ++w) near[w] = bits_of(i - a.window, i, w);
+      for (int w = 0; near && w < a.near_words; ++w) near[w] = bits_of(lo, i, w);
     } else {
       // ancestors have smaller numbers, so the words fill from the last one down
-      int64_t w = i >> 6, at = i;
+      int64_t w = i >> 6, at = i, depth = 0;
       uint64_t all = 0, close = 0;
       for (int64_t u = w + 1; tree && u < a.tree_words; ++u) tree[u] = 0;
       for (int64_t u = w + 1; near && u < a.near_words; ++u) near[u] = 0;
@@ -209,8 +222,8 @@ __device__ __forceinline__ void token_maps(const MapArgs& a, int b) {
         at = up;
         ++depth;
       }
+      pos = root + depth;
     }
-    const int64_t pos = root + depth;
     store_index(a.positions, a.pos64, t, pos);
     if (a.window_starts) {
       const int64_t lower = pos - a.window;
@@ -218,9 +231,9 @@ __device__ __forceinline__ void token_maps(const MapArgs& a, int b) {
       if (!r.raw_ids) {
         lo = lower < 0 ? 0 : (lower < old ? lower : old);
       } else {
-        // positions ascend, so the first key is at most `depth` ranks on
+        // positions ascend, so the first key is at most pos - root ranks on
         lo = first;
-        int64_t hi = first + depth < old ? first + depth : old;
+        int64_t hi = first + (pos - root) < old ? first + (pos - root) : old;
         while (lo < hi) {
           const int64_t mid = (lo + hi) >> 1;
           const int64_t at = mid - first < kThreads ? keys[mid - first] : r.pos_of(mid);

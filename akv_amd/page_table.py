@@ -182,9 +182,11 @@ def context_step_maps(registry, table, rows, seq_lens, new_lens, qo_indptr, kv_i
       a is i or one of its ancestors.  ``parents`` int32 ``[N]`` names each
       token's parent by its number among the request's new tokens (an earlier
       one; anything else: none); without it a request's tokens are a chain.  A
-      token's position is its root's plus its depth;
+      tree's node i has the position of the first new rank plus its depth, a
+      chain's that of its own rank;
     * for layers with a sliding ``window`` (a key is visible when
-      ``q_pos - k_pos <= window``): ``window_mask``, the ancestors inside it,
+      ``q_pos - k_pos <= window``): ``window_mask``, the ancestors inside it
+      (itself too),
       and ``window_starts`` int32 ``[N]``, the first earlier key inside it.
 
     ``rows`` may be int32 or int64; ``seq_lens`` and ``new_lens`` share either,

@@ -747,11 +747,13 @@ int akv_gather_slots(int32_t slot_dtype, const int64_t* sources,
  * akv_decode_indices.  Written, with P = page_size and W = window:
  *   qo_indptr, kv_indptr [B + 1]  cumulative sums of n and L
  *   slot_map[qo + i]       slot(L - n + i); -1 behind the last token
- *   positions[qo + i]      position(L - n) + depth(i); 0 behind the last token
+ *   positions[qo + i]      position(L - n) + depth(i), without parents
+ *                          position(L - n + i); 0 behind the last token
  *   block_tables[b][j]     slot(j P) / P for j P < L, -1 behind (and for ranks
  *                          without a slot); NULL: none
  *   tree_mask[qo + i]      bit a: new token a is i or an ancestor of i
- *   window_mask[qo + i]    bit a: the same, at most W levels up
+ *   window_mask[qo + i]    bit a: the same, if a's position is at least
+ *                          positions[qo + i] - W (in a tree: at most W levels up)
  *   window_starts[qo + i]  first rank of [0, L - n) whose position is at least
  *                          positions[qo + i] - W (positions ascend
  *                          strictly)

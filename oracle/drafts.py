@@ -47,9 +47,13 @@ def pack_bits(seen, words):
     return np.packbits(bits, axis=1, bitorder="little").view(np.int64).reshape(len(seen), words)
 
 
-def step_maps(requests, new_lens, *, page_size=1, pages=0, parents=None, words=1, window=None, capacity=None):
+def step_maps(requests, new_lens, *, page_size=1, pages=0, parents=None, words=1, window=None, capacity=None,
+              chunk=False):
     """``requests``: per request (slots, positions) of all its ranks, slots -1
-    where it has none; ``parents``: per request, or None for chains."""
+    where it has none; ``parents``: per request, or None for chains.  A node's
+    position is the first new rank's plus its depth; with ``chunk`` a chain's
+    tokens have their own ranks' (the same wherever those ascend by one, as they
+    do behind a registry row's active ranks)."""
     new = [max(0, min(int(n), len(s))) for (s, _), n in zip(requests, new_lens)]
     total = sum(new)
     capacity = total if capacity is None else capacity
@@ -72,10 +76,12 @@ def step_maps(requests, new_lens, *, page_size=1, pages=0, parents=None, words=1
         tree = list(range(-1, n - 1)) if parents is None else parents[b]
         here = slice(at, at + n)
         out["slot_map"][here] = slots[old:]
-        out["positions"][here] = positions[old] + depths(tree)
+        at_pos = positions[old:] if chunk and parents is None else positions[old] + depths(tree)
+        out["positions"][here] = at_pos
         out["tree_mask"][here] = pack_bits(ancestors(tree), words)
         if window is not None:
-            out["window_mask"][here] = pack_bits(ancestors(tree, window), words)
+            inside = at_pos[:, None] - at_pos[None] <= window
+            out["window_mask"][here] = pack_bits(ancestors(tree) & inside, words)
             out["window_starts"][here] = np.searchsorted(positions[:old], out["positions"][here] - window, side="left")
         at += n
     return out

@@ -1,5 +1,7 @@
 """The metadata of a step's new tokens on the GPU against the oracle."""
 
+import functools
+
 import numpy as np
 import pytest
 import torch
@@ -202,3 +204,28 @@ def test_side_rows_beside_a_table_without_columns(device):
     b.table = b.table[:, :0].clone()
     assert b.table.data_ptr() == 0
     _run(b, window=20)
+
+
+@pytest.mark.parametrize("gaps", [True, False])
+@pytest.mark.parametrize("active", ["some", "all", "beyond"])
+def test_chunks_that_begin_among_the_active_ranks(device, monkeypatch, active, gaps):
+    """A prompt's next chunk: some or all of its ranks, or not even the last of
+    them, are the registry's kept tokens, whose positions have gaps."""
+    monkeypatch.setattr(drafts, "step_maps", functools.partial(drafts.step_maps, chunk=True))
+    old, new = [300, 1, 90, 20, 5], [70, 300, 64, 20, 600]
+    extra = {"some": 20, "all": 20, "beyond": 20}[active]
+    if active == "all":
+        new = [20] * 5
+    b = Batch(device, 40, old, new, kept=[1, 1, 1, 0, 1], gaps=gaps, extra_generated=-extra)
+    if active == "beyond":
+        # the batch ends 5 ranks before the active ones do
+        new = [15] * 5
+        b.new = new
+        b.requests = [(s[: o + 15], p[: o + 15]) for (s, p), o in zip(b.requests, old)]
+        b.seq, b.fresh = (torch.tensor(x, device=device) for x in ([o + 15 for o in old], new))
+        b.trees = [random_tree(np.random.default_rng(2), 15) for _ in old]
+    for window in (None, 0, 1, 9, 100, 5000, 2 ** 31 - 1):
+        for tree in (False, True):
+            print(f"step maps chunk {active} window {window} tree {tree}", flush=True)
+            _run(b, window=window, tree=tree, page=1)
+    _run(b, window=9, tree=False, words=1)

@@ -91,3 +91,16 @@ def test_rows_without_keys_are_zero():
     seen = np.array([[False, False], [True, False]])
     got, _, _ = drafts.tree_attention(q, k, 3 * k, [(0, [9, 1], seen)], 1.0)
     assert (got == 0).all()  # nothing seen; the only seen key lies outside the pool
+
+
+def test_a_chunk_has_its_ranks_positions():
+    """New ranks among kept tokens whose positions have gaps."""
+    slots, positions = np.arange(10, 16), np.array([0, 2, 7, 8, 30, 31])
+    got = drafts.step_maps([(slots, positions)], [4], window=6, chunk=True)
+    assert got["positions"].tolist() == [7, 8, 30, 31]
+    assert got["window_starts"].tolist() == [1, 1, 2, 2]  # of the ranks at 0 and 2
+    assert got["tree_mask"][:, 0].tolist() == [1, 3, 7, 15]
+    assert got["window_mask"][:, 0].tolist() == [1, 3, 4, 12]
+    tree = drafts.step_maps([(slots, positions)], [4], window=1, parents=[[-1, 0, 0, 2]])
+    assert tree["positions"].tolist() == [7, 8, 8, 9]
+    assert tree["window_mask"][:, 0].tolist() == [1, 3, 5, 12]
