@@ -216,13 +216,14 @@ __device__ __forceinline__ int32_t here_only(int32_t v) {
 
 // Loads straight into LDS: lane l's bytes go to `to` + 16 l (4 l).  In asm, since
 // the compiler takes every later LDS read for one that may meet them and waits
-// for all of them; arrive() does the waiting.  (Nothing else in these kernels
-// uses m0.)
+// for all of them; arrive() does the waiting.
 __device__ __forceinline__ void load_16(const void* from, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to)
+               : "memory", "m0");
 }
 __device__ __forceinline__ void load_4(const void* from, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(to)
+               : "memory", "m0");
 }
 
 __device__ __forceinline__ uint32_t lds_address(const void* p) {

@@ -1,6 +1,9 @@
 """What the drafted-token operators refuse, without a GPU: the wrappers'
 checks and the C ABI's, none of which reaches a launch."""
 
+import re
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -285,3 +288,16 @@ def test_a_workspace_serves_every_smaller_batch(q_heads, kv_heads, head_dim):
 def test_no_address_is_for_nothing_alone(name, change, message):
     assert _call(name, **change) == _lib.AKV_EINVAL
     assert message in _lib.last_error()
+
+
+def test_asm_names_the_registers_it_writes():
+    """Scalar registers that an asm statement writes by name are among its
+    clobbers, so that the compiler keeps nothing in them across it."""
+    found = 0
+    for path in (Path(_lib.__file__).parent / "csrc").iterdir():
+        text = path.read_text() if path.suffix in (".hip", ".h") else ""
+        for asm in re.findall(r"\basm(?:\s+volatile)?\s*\((.*?)\);", text, re.S):
+            for register in re.findall(r"\bs_mov_b(?:32|64)\s+(m0|vcc|exec|s\d+)\b", asm):
+                found += 1
+                assert f'"{register}"' in asm, (path.name, asm)
+    assert found >= 2
