@@ -16,6 +16,8 @@
 // rows of 64 in bf16: 680 MB in 135 us, 5.0 TB/s, what a large copy reaches; 8191 of
 // 24 rows of 128: 103 MB in 22 us (28 from cold caches, where a copy takes 21); one
 // token 3.7 us.
+#include <type_traits>
+
 #include "common.h"
 
 namespace akv {
@@ -300,6 +302,30 @@ __global__ void __launch_bounds__(kThreads) qk_norm_generic_kernel(const NormArg
   }
 }
 
+// Workgroups of a launch: a grid has fewer than 2^32 threads.  More tokens take
+// several launches.
+constexpr int64_t kMostBlocks = 1 << 23;
+
+// Calls start(args, blocks) for stretches of the tokens, each with `waves` waves.
+template <typename T, typename F>
+int in_stretches(const NormArgs& args, int64_t waves, F start) {
+  const int64_t most = kMostBlocks * (kThreads / 64) / waves;
+  for (int64_t t = 0; t < args.n_tokens; t += most) {
+    NormArgs a = args;
+    a.n_tokens = args.n_tokens - t < most ? args.n_tokens - t : most;
+    auto on = [&](auto*& p, int64_t bytes) {
+      if (p) p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(reinterpret_cast<uintptr_t>(p) + t * bytes);
+    };
+    constexpr int64_t e = sizeof(T);
+    on(a.q, e * a.q_st), on(a.k, e * a.k_st), on(a.v, e * a.v_st), on(a.q_out, e * a.qo_st), on(a.k_out, e * a.ko_st);
+    on(a.positions, a.pos64 ? 8 : 4), on(a.slots, a.slots64 ? 8 : 4);
+    start(a, dim3(static_cast<unsigned>((a.n_tokens * waves + kThreads / 64 - 1) / (kThreads / 64))));
+    const int rc = check_launch("akv_qk_norm_rope");
+    if (rc) return rc;
+  }
+  return AKV_OK;
+}
+
 template <typename T>
 int launch_vector(const NormArgs& args, hipStream_t st) {
   NormArgs a = args;
@@ -312,29 +338,25 @@ int launch_vector(const NormArgs& args, hipStream_t st) {
   // wave and with one per round, 64 + 16 heads of 64: 1024 tokens 8.9, 7.2; 2048
   // 11.5, 12.9; 16384 72.8, 85.6; 32 + 16 heads of 128: 1024 9.5, 8.8; 2048 12.5, 14.8)
   a.parts = a.n_tokens >= 2048 ? 1 : rounds;
-  const int64_t waves = a.n_tokens * a.parts;
-  const int64_t blocks = (waves + kThreads / 64 - 1) / (kThreads / 64);
-  if (blocks > 0x7fffffffLL) return fail(AKV_EINVAL, "akv_qk_norm_rope: too many tokens");
-  const dim3 grid(static_cast<unsigned>(blocks)), block(kThreads);
-  switch (lanes) {
-    case 1: hipLaunchKernelGGL((qk_norm_kernel<T, 1>), grid, block, 0, st, a); break;
-    case 2: hipLaunchKernelGGL((qk_norm_kernel<T, 2>), grid, block, 0, st, a); break;
-    case 4: hipLaunchKernelGGL((qk_norm_kernel<T, 4>), grid, block, 0, st, a); break;
-    case 8: hipLaunchKernelGGL((qk_norm_kernel<T, 8>), grid, block, 0, st, a); break;
-    case 16: hipLaunchKernelGGL((qk_norm_kernel<T, 16>), grid, block, 0, st, a); break;
-    default: hipLaunchKernelGGL((qk_norm_kernel<T, 32>), grid, block, 0, st, a); break;
-  }
-  return check_launch("akv_qk_norm_rope");
+  return in_stretches<T>(a, a.parts, [&](const NormArgs& part, dim3 grid) {
+    const dim3 block(kThreads);
+    switch (lanes) {
+      case 1: hipLaunchKernelGGL((qk_norm_kernel<T, 1>), grid, block, 0, st, part); break;
+      case 2: hipLaunchKernelGGL((qk_norm_kernel<T, 2>), grid, block, 0, st, part); break;
+      case 4: hipLaunchKernelGGL((qk_norm_kernel<T, 4>), grid, block, 0, st, part); break;
+      case 8: hipLaunchKernelGGL((qk_norm_kernel<T, 8>), grid, block, 0, st, part); break;
+      case 16: hipLaunchKernelGGL((qk_norm_kernel<T, 16>), grid, block, 0, st, part); break;
+      default: hipLaunchKernelGGL((qk_norm_kernel<T, 32>), grid, block, 0, st, part); break;
+    }
+  });
 }
 
 template <typename T>
 int launch(const NormArgs& a, bool vector, hipStream_t st) {
   if (vector) return launch_vector<T>(a, st);
-  const int64_t units = a.n_tokens * a.rows;
-  const int64_t blocks = (units + kThreads / 64 - 1) / (kThreads / 64);
-  if (blocks > 0x7fffffffLL) return fail(AKV_EINVAL, "akv_qk_norm_rope: too many tokens");
-  hipLaunchKernelGGL(qk_norm_generic_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, a);
-  return check_launch("akv_qk_norm_rope");
+  return in_stretches<T>(a, a.rows, [&](const NormArgs& part, dim3 grid) {
+    hipLaunchKernelGGL(qk_norm_generic_kernel<T>, grid, dim3(kThreads), 0, st, part);
+  });
 }
 
 }  // namespace

@@ -200,3 +200,47 @@ def test_a_pool_without_slots(device, d):
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
     qk_norm.qk_norm_rope(q, k, v, None, None, positions, table, outs[2][0], **pool)
     assert torch.equal(outs[0][0], outs[2][0])
+
+
+@pytest.mark.parametrize("hq,hk,d,n,vector", [(60, 2, 2, 1_100_001, False), (1, 1, 16, 67_200_003, True)])
+def test_more_tokens_than_one_launch_has_threads_for(device, hq, hk, d, n, vector):
+    """A wave per row (any widths) or per token: 2^26 of them have 2^32 threads.
+    The tokens at both ends and around every 2^20th are those of small calls."""
+    print(f"norms of {n} tokens, {hq} + {hk} heads of {d}", flush=True)
+    gen = torch.Generator(device=device).manual_seed(n)
+    q = torch.randn(n, hq, d, generator=gen, device=device, dtype=torch.bfloat16)
+    k = q[:, -hk:]
+    table = torch.randn(50, d, generator=gen, device=device)
+    positions = torch.randint(0, 50, (n,), generator=gen, device=device, dtype=torch.int32)
+    outs = [torch.full_like(q, 7), torch.full_like(q[:, :hk], 7)]
+    qk_norm.qk_norm_rope(q, k, None, None, None, positions, table, outs[0], k_out=outs[1])
+    at = torch.arange(0, n, 1 << 20, device=device)[:, None] + torch.arange(-4, 5, device=device)
+    at = torch.cat((at.flatten(), torch.arange(n - 9, n, device=device)))
+    at = at[(at >= 0) & (at < n)]
+    want = [torch.empty_like(t[at]) for t in outs]
+    qk_norm.qk_norm_rope(q[at], k[at], None, None, None, positions[at], table, want[0], k_out=want[1])
+    for got, w in zip(outs, want):
+        assert torch.equal(got[at], w)
+        assert not (got == 7).all(-1).any()
+
+
+def test_stretches_of_tokens_with_a_pool(device):
+    """The same with slots and a pool that holds some of the tokens."""
+    n, d, slots = 1_500_000, 2, 1000
+    gen = torch.Generator(device=device).manual_seed(5)
+    x = torch.randn(n, 50, d, generator=gen, device=device, dtype=torch.bfloat16)
+    q, k, v = x.split((46, 2, 2), 1)
+    table = torch.randn(50, d, generator=gen, device=device)
+    positions = torch.randint(0, 50, (n,), generator=gen, device=device)
+    taken = torch.arange(slots, device=device) * 1499 + 700
+    slot_map = torch.full((n,), -1, dtype=torch.int64, device=device)
+    slot_map[taken] = torch.randperm(slots, generator=gen, device=device)
+    pools = [torch.zeros(slots, 2, d, dtype=torch.bfloat16, device=device) for _ in range(2)]
+    out = torch.empty(n, 46, d, dtype=torch.bfloat16, device=device)
+    qk_norm.qk_norm_rope(q, k, v, None, None, positions, table, out, slot_map=slot_map, k_buffer=pools[0],
+                         v_buffer=pools[1])
+    at = taken.clone()
+    few, k_few = torch.empty(slots, 46, d, dtype=torch.bfloat16, device=device), torch.empty_like(pools[0])
+    qk_norm.qk_norm_rope(q[at], k[at], None, None, None, positions[at], table, few, k_out=k_few)
+    assert torch.equal(out[at], few)
+    assert torch.equal(pools[0][slot_map[at]], k_few) and torch.equal(pools[1][slot_map[at]], v[at])
