@@ -896,9 +896,9 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const TreeA
 // Merges the pieces of rows that a cut went through, and the sink: WAYS x D / 4
 // lanes per (token, head), each way every WAYS-th piece, AHEAD of them in flight.
 template <typename T, int D, int WAYS, int AHEAD>
-__global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a, const int block_rows) {
+__global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a, const int block_rows, const int64_t row0) {
   constexpr int kLanes = D / 4;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / (kLanes * WAYS)) + threadIdx.x / (kLanes * WAYS);
+  const int64_t row = row0 + static_cast<int64_t>(blockIdx.x) * (256 / (kLanes * WAYS)) + threadIdx.x / (kLanes * WAYS);
   const int d = 4 * (threadIdx.x % kLanes), way = threadIdx.x / kLanes % WAYS;
   const int64_t token = row / a.q_heads;
   const int head = static_cast<int>(row - token * a.q_heads);
@@ -976,6 +976,10 @@ int subtiles_for(int d, int64_t rows) {
   return sub;
 }
 
+// Workgroups of 256 threads in a launch: a grid has fewer than 2^32 threads, and
+// what is beyond is left out without an error.
+constexpr int64_t kMostBlocks = 1 << 23;
+
 struct Launch {
   int d, sub;
   bool whole;
@@ -1008,7 +1012,9 @@ Launch plan(int64_t n_tokens, int64_t n_requests, int64_t q_heads, int64_t kv_he
   // (32 requests, 8 KV heads, 128 rows of 64 over a window's 145 keys: 16.5 us in
   // blocks of 128 rows, 18.2 in 256; 128 requests of 64 rows: no difference)
   if (p.whole && p.sub == 4 && n_requests * kv_heads * ((rows + 127) / 128) <= kGroups) p.sub = 2;
-  p.row_blocks = static_cast<int32_t>(std::min<int64_t>(blocks(), 4096));
+  // (further blocks of rows follow in the same workgroup)
+  const int64_t room = std::max<int64_t>(1, kMostBlocks / std::max<int64_t>(1, n_requests * kv_heads));
+  p.row_blocks = static_cast<int32_t>(std::min(blocks(), std::min<int64_t>(room, 4096)));
   return p;
 }
 
@@ -1051,8 +1057,11 @@ constexpr int64_t kFewRows = 4096, kFewestRows = 512;
 template <typename T, int D, int WAYS, int AHEAD>
 void merge_by(const TreeArgs& a, const Launch& p, hipStream_t st) {
   constexpr int kRows = 256 / (D / 4 * WAYS);
-  const dim3 grid(static_cast<unsigned>((a.n_tokens * a.q_heads + kRows - 1) / kRows));
-  hipLaunchKernelGGL((tree_combine_kernel<T, D, WAYS, AHEAD>), grid, dim3(256), 0, st, a, 16 * kWaves * p.sub);
+  const int64_t rows = a.n_tokens * a.q_heads;
+  for (int64_t row0 = 0; row0 < rows; row0 += kMostBlocks * kRows) {
+    const dim3 grid(static_cast<unsigned>(std::min(kMostBlocks, (rows - row0 + kRows - 1) / kRows)));
+    hipLaunchKernelGGL((tree_combine_kernel<T, D, WAYS, AHEAD>), grid, dim3(256), 0, st, a, 16 * kWaves * p.sub, row0);
+  }
 }
 
 template <typename T, int D>
@@ -1070,7 +1079,6 @@ void merge(const TreeArgs& a, const Launch& p, hipStream_t st) {
 template <typename T>
 int launch(const TreeArgs& a, const Launch& p, hipStream_t st) {
   const int64_t blocks = p.whole ? static_cast<int64_t>(a.n_requests) * a.kv_heads * a.row_blocks : kGroups;
-  if (blocks > 0x7fffffffLL) return fail(AKV_EINVAL, "akv_tree_attention: batch too large");
   const dim3 grid(static_cast<unsigned>(blocks));
   if (p.d == 64) {
     if (p.sub == 1) start<T, 64, 1>(a, grid, st);

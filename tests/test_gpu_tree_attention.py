@@ -458,7 +458,8 @@ def test_one_workspace_while_a_batch_drains(device):
     ws = torch.full((need,), 255, dtype=torch.uint8, device=device)
     for requests in (40, 32, 31, 3, 1):
         print(f"tree attention, {requests} requests of 40", flush=True)
-        c = Cache(device, 980 + requests, [(37 * i) % 130 + 800 * (i == 0) for i in range(requests)], [4] * requests, **shape)
+        old = [(37 * i) % 130 + 800 * (i == 0) for i in range(requests)]
+        c = Cache(device, 980 + requests, old, [4] * requests, **shape)
         seen, mask = c.masks("tree")
         _check(c, _run(c, mask=mask, workspace=ws, max_len=1000), c.visible(seen))
 
@@ -526,3 +527,49 @@ def test_pools_and_lists_of_nothing(device, bound, page, d):
             out = _run(c, mask=mask, k=k, v=v, sinks=s, max_len=bound)
             assert (out[: c.total] == 0).all()
         c.indices = indices
+
+
+@pytest.mark.parametrize("d,heads", [(8, 64), (128, 2)])
+def test_more_rows_than_one_launch_has_threads_for(device, d, heads):
+    """Outputs made for 2^32 threads' worth of rows, of which the last 40 tokens'
+    and the first ones' are the batch's: 16 (32) threads of the merge for each."""
+    rows = (1 << 32) // (16 if d == 8 else 32)
+    capacity = rows // heads + 100
+    print(f"tree attention, capacity of {capacity} tokens, {heads} heads of {d}", flush=True)
+    c = Cache(device, 1000 + d, [900, 1200], [7, 40], q_heads=heads, kv_heads=2, head_dim=d, dtype=torch.bfloat16)
+    requests = c.visible(c.masks("chain")[0])
+    q = torch.zeros(capacity, heads, d, dtype=torch.bfloat16, device=device)
+    out = torch.full_like(q, 7.0)
+    for first in (0, capacity - 47):
+        q[first: first + 47] = c.q
+        attention.tree_attention(q, c.k.to(device), c.v.to(device), c.qo + first, c.kv, c.indices, out,
+                                 scale=d ** -0.5, max_len=5000, max_new=40)
+        _check(c, out[first: first + 47], requests)
+        out[first: first + 47] = 7.0
+        assert (out[:100] == 7).all() and (out[-100:] == 7).all()
+
+
+def test_more_row_blocks_than_one_launch_has_threads_for(device):
+    """4096 short requests under a bound of a million new tokens each."""
+    capacity, batch = 1 << 20, 4096
+    rng = np.random.default_rng(4)
+    old, new = rng.integers(0, 60, batch), rng.integers(0, 4, batch)
+    old[-1], new[-1] = 100, 90
+    c = Cache(device, 1010, old.tolist(), new.tolist(), q_heads=64, kv_heads=8, head_dim=8, dtype=torch.bfloat16)
+    want = _run(c, mask=None)
+    q = torch.zeros(capacity, 64, 8, dtype=torch.bfloat16, device=device)
+    q[: c.total] = c.q
+    out = torch.full_like(q, 7.0)
+    attention.tree_attention(q, c.k.to(device), c.v.to(device), c.qo, c.kv, c.indices, out, scale=8 ** -0.5,
+                             max_len=c.max_len, max_new=capacity)
+    # (blocks of other sizes than under the tight bound: both within their bound of the same rows)
+    seen = c.visible(c.masks("chain")[0])
+    last = len(seen) - 1
+    for b in (0, 1, batch // 2, last - 1, last):
+        first, slots, keys = seen[b]
+        here = slice(first, first + len(keys))
+        y, size, spread = drafts.tree_attention(f64(c.q[here]), f64(c.k), f64(c.v), [(0, slots, keys)], 8 ** -0.5)
+        tol = attention_tolerance(c.q.dtype, c.q.dtype, c.max_len, y, size, spread, 0)
+        for got in (out, want):
+            assert (np.abs(f64(got[here]) - y) <= tol).all(), b
+    assert not (out[: c.total] == 7).all(-1).any() and (out[c.total:] == 7).all()
