@@ -95,7 +95,8 @@ __device__ __forceinline__ void lengths_of(const MapArgs& a, int64_t b, int64_t*
 __device__ __forceinline__ Request request_of(const MapArgs& a, int b) {
   Request r;
   lengths_of(a, b, &r.len, &r.fresh);
-  const int64_t id = load_index(a.rows, a.rows64, b);
+  // (a request without ranks, as a padded batch's last ones, may name any row)
+  const int64_t row = load_index(a.rows, a.rows64, b), id = r.len > 0 ? row : 0;
   const int64_t* entry = a.registry + id * 6;
   r.raw_ids = reinterpret_cast<const int32_t*>(entry[0]);
   r.positions = reinterpret_cast<const int32_t*>(entry[1]);

@@ -190,7 +190,8 @@ def context_step_maps(registry, table, rows, seq_lens, new_lens, qo_indptr, kv_i
       and ``window_starts`` int32 ``[N]``, the first earlier key inside it.
 
     ``rows`` may be int32 or int64; ``seq_lens`` and ``new_lens`` share either,
-    as do the indptrs; a mask has a word per 64 new tokens of a request.
+    as do the indptrs; a mask has a word per 64 new tokens of a request.  A
+    request of length 0 (a padded batch's last ones) may name any row.
     ``status``: as for ``context_decode_indices``.
     """
     # one read of every property: the checks are most of the call's time

@@ -762,8 +762,8 @@ int akv_gather_slots(int32_t slot_dtype, const int64_t* sources,
  * *_words 64-bit words, *_stride words apart; tokens past 64 words have no
  * bits.  n_tokens is the capacity of the token vectors; seq_lens and new_lens
  * share lens_dtype, the indptrs indptr_dtype.  table_width bounds the table's
- * rows (a rank past it has no slot); side rows are not bounded.  status as in
- * akv_decode_indices.
+ * rows (a rank past it has no slot); side rows are not bounded.  rows[b] is
+ * not used where seq_lens[b] is 0.  status as in akv_decode_indices.
  *
  * The reading side's counterpart of the reference is
  * akv/system/sglang/kernels/ops/attention/context_page_table.py:7-76; the

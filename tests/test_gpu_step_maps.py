@@ -229,3 +229,12 @@ def test_chunks_that_begin_among_the_active_ranks(device, monkeypatch, active, g
             print(f"step maps chunk {active} window {window} tree {tree}", flush=True)
             _run(b, window=window, tree=tree, page=1)
     _run(b, window=9, tree=False, words=1)
+
+
+@pytest.mark.parametrize("row", [-1, 10 ** 6, 2 ** 40])
+def test_requests_without_ranks_may_name_any_row(device, row):
+    """What a padded batch leaves in its last rows is not followed."""
+    b = Batch(device, 50, [30, 0, 900, 0, 0], [4, 0, 9, 0, 0], kept=[1, 0, 1, 0, 0])
+    b.rows[b.seq == 0] = row
+    for window in (None, 20):
+        _run(b, window=window, capacity=20)
