@@ -238,3 +238,12 @@ def test_requests_without_ranks_may_name_any_row(device, row):
     b.rows[b.seq == 0] = row
     for window in (None, 20):
         _run(b, window=window, capacity=20)
+
+
+def test_the_largest_batch(device):
+    """65534 requests, most of them of one new token."""
+    rng = np.random.default_rng(8)
+    old, new = rng.integers(0, 5, 65534), np.minimum(rng.integers(0, 9, 65534), 2) // 2
+    kept = rng.random(65534) < 0.001
+    b = Batch(device, 60, old.tolist(), new.tolist(), kept=kept)
+    _run(b, window=2, tree=False)

@@ -573,3 +573,28 @@ def test_more_row_blocks_than_one_launch_has_threads_for(device):
         for got in (out, want):
             assert (np.abs(f64(got[here]) - y) <= tol).all(), b
     assert not (out[: c.total] == 7).all(-1).any() and (out[c.total:] == 7).all()
+
+
+@pytest.mark.parametrize("bound", [1, 5000])
+def test_the_largest_batch(device, bound):
+    """65534 requests of one drafted token over one key, every 1000th without."""
+    batch, d = 65534, 8
+    gen = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(s, 1, d, generator=gen).to(torch.bfloat16).to(device) for s in (batch, 2 * batch, 2 * batch))
+    lens = torch.full((batch,), 2)
+    lens[::1000] = 1
+    kv = torch.cat((torch.zeros(1, dtype=torch.int64), lens.cumsum(0)))
+    slots = torch.randperm(2 * batch, generator=gen)
+    qo = torch.arange(batch + 1, dtype=torch.int32, device=device)
+    out = torch.empty(batch, 1, d, dtype=torch.float32, device=device)
+    attention.tree_attention(q, k, v, qo, kv.int().to(device), slots.int().to(device), out, scale=0.5, max_len=bound,
+                             max_new=1)
+    own, before = slots[kv[1:] - 1].numpy(), slots[kv[:-1]].numpy()
+    scores = 0.5 * np.stack([(f64(q) * f64(k)[at]).sum(-1)[:, 0] for at in (own, before)], -1)
+    spread = 0.5 * np.stack([np.abs(f64(q) * f64(k)[at]).sum(-1)[:, 0] for at in (own, before)], -1).max(-1)[:, None]
+    scores[::1000, 1] = -np.inf
+    w = np.exp(scores - scores.max(-1, keepdims=True))
+    w /= w.sum(-1, keepdims=True)
+    want, size = (w[:, :1, None] * f(f64(v)[own]) + w[:, 1:, None] * f(f64(v)[before]) for f in (np.array, np.abs))
+    tol = attention_tolerance(torch.bfloat16, torch.float32, 2, want, size, spread, 0)
+    assert (np.abs(f64(out) - want) <= tol).all()
