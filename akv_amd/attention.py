@@ -99,9 +99,10 @@ def tree_attention(q, k_buffer, v_buffer, qo_indptr, kv_indptr, kv_indices, out,
     ``[q_heads]``.  ``max_len`` (keys a request's tokens reach: its keys, or
     window + n + 1) and ``max_new`` (its tokens) are host bounds that size the
     launch and the workspace; the results depend on them only in the order of
-    their fp32 sums.  Rows of ``out``, which must not overlap ``q``, behind the
-    last token stay as they are.  Head dims: multiples of 8
-    up to 128.  Weights are relative to a row's first scores and may grow to
+    their fp32 sums (and in whether an infinite value that a token sees makes
+    that dim of its row infinite or NaN).  Rows of ``out``, which must not
+    overlap ``q``, behind the last token stay as they are.  Head dims: multiples
+    of 8 up to 128.  Weights are relative to a row's first scores and may grow to
     2^32 before they are rescaled, so bf16 values that a token sees are taken
     up to 2^94 in magnitude.  ``status``: as for ``decode_attention``.
     """

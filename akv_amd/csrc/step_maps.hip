@@ -26,7 +26,8 @@
 // lies behind the last token.  A table entry is two dependent loads (raw id,
 // row entry), four chains of them in flight per thread.  Bound by such round trips:
 // one request of 4096 ranks 3.6 us, 32 of 20k with a page per rank, trees of 16 and
-// a window 8.4 us (7.7 MB), 64 of 2k to 64k with pages of 16 7.8 us.
+// a window 8.4 us (7.7 MB), 64 of 2k to 64k with pages of 16 8.0 us.  A token walks
+// to its root by itself, so a tree's masks cost the sum of its depths.
 #include "common.h"
 
 namespace akv {

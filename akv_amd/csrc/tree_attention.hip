@@ -13,14 +13,18 @@
 //
 // The n tokens x G heads of a KV head's group are the rows of one product with
 // that head's keys, so K and V are read once for a block of 64 SUB rows, and
-// again for every further one.  All the batch's tiles of keys lie on a line, and
-// 512 workgroups of four waves, two per CU, take equal stretches of it; where a
-// cut falls among a request's tiles, a second launch merges the parts.  Tiles of
+// again for every further one.  All the batch's tiles of keys lie on a line (a
+// request's blocks of rows far apart), and 512 workgroups of four waves, two per
+// CU, take equal stretches of it; where a cut falls among a request's tiles, a
+// second launch merges the parts.  Tiles of
 // K and V stream into LDS (two places) while the one before is worked on, 32 keys
 // (a quarter of a tile at D = 64) at a time, 16 SUB rows per wave:
 //   S^T[32 x 16 SUB] = K . Q^T              v_mfma_f32_16x16x32
-//   P^T = 2^(scale log2(e) S^T - m)         in the storage type
+//   P^T = 2^(scale log2(e) S^T - m)         rounded once to the storage type
 //   l += 1^T . P^T,  O^T[D x 16 SUB] += V^T . P^T
+// (the matrix cores take P in V's type; the sum takes the rounded weights too, so
+// that they add up to one.  A row's error against 64 bits is 0.0023 of it in bf16
+// and 0.00027 in fp16; the output's own rounding alone is 0.0017 and 0.00021).
 // A block with at most half (a quarter of) its rows has two (four) waves share
 // each group of rows: they take the quarters in turn and meet at the end.
 // P^T leaves the first product in the operand layout of the second; V^T comes
@@ -28,11 +32,13 @@
 // weights outgrow their types.
 //
 // Bound: HBM while a KV head has up to about 128 rows (16 tokens x 8 heads of 64
-// over 32 requests of 20k keys: 1.30 GB in 278-306 us, 4.3-4.7 TB/s; 5 to 32 tokens x
+// over 32 requests of 20k keys: 1.30 GB in 272-306 us, 4.3-4.8 TB/s; 5 to 32 tokens x
 // 4 heads of 128 over 12 paged requests: 0.50 GB in 124 us, 4.0 TB/s); matrix and
-// vector work above (64 tokens over 8 requests of 25k: 203 GFLOP in 255-280 us,
+// vector work above (64 tokens over 8 requests of 25k: 203 GFLOP in 255-284 us,
 // 720-800 TFLOP/s); round trips where there is little (8 tokens over 4096 keys: 13
-// us and 4 for the merge; a window's 145 keys x 32 requests: 16 us).
+// us and 5 for the merge; a window's 145 keys x 32 requests: 16-17 us).  Every
+// instance moves 120 to 198 scalars to vector lanes, SUB = 4 takes all 256 vector
+// registers and keeps one in scratch.
 //
 // Lane layouts (verified on gfx950): v_mfma_f32_16x16x32 -- lane l supplies
 // A[l%16][k(l,i)], B[k(l,i)][l%16] for i < 8 and holds D[4(l/16)+i][l%16];

@@ -25,7 +25,8 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, positions, cos_sin_cache, q_out, *
     fused projection will do: any token and head strides); ``q_weight`` /
     ``k_weight`` ``[D]`` or None (1); ``positions`` int32 or int64 ``[N]``, rows
     of ``cos_sin_cache`` ``[positions, rotary_dim]``.  Norm and rotation are in
-    fp32, rounded once.  q goes to ``q_out`` (which may be ``q``), k to
+    fp32 (a row's squares too: past its range the row comes out as 0), rounded
+    once.  q goes to ``q_out`` (which may be ``q``), k to
     ``k_out`` (which may be ``k``) and, with ``k_buffer`` / ``v_buffer``
     ``[slots, kv_heads, D]``, k and v to rows ``slot_map`` int32 or int64
     ``[N]``, whose valid entries are distinct.  A token whose slot is outside

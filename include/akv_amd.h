@@ -762,7 +762,8 @@ int akv_gather_slots(int32_t slot_dtype, const int64_t* sources,
  * *_words 64-bit words, *_stride words apart; tokens past 64 words have no
  * bits.  n_tokens is the capacity of the token vectors; seq_lens and new_lens
  * share lens_dtype, the indptrs indptr_dtype.  table_width bounds the table's
- * rows (a rank past it has no slot); side rows are not bounded.  rows[b] is
+ * rows (a rank past it has no slot); side rows are not bounded.  Each token
+ * walks to its root, so a tree costs the sum of its depths.  rows[b] is
  * not used where seq_lens[b] is 0.  status as in akv_decode_indices.
  *
  * The reading side's counterpart of the reference is
@@ -824,20 +825,21 @@ int akv_qk_norm_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  * kv_indptr[b] keys end in the tokens' own n.  Token i sees an earlier key of
  * rank j when j >= key_starts[token] (NULL: always), and the request's new
  * token a when bit a of its tree_mask row is set (mask_words 64-bit words, bits
- * past them are 0; NULL: a <= i).  GQA, scaled
- * scores, sinks in the denominator as in akv_decode_attention; a token that
- * sees no key gets 0.  q, K and V are bf16 or fp16, the output q's type or
- * f32; head_dim a multiple of 8 up to 128, any number of q heads per KV head.
+ * past them are 0; NULL: a <= i).  GQA, scaled scores, sinks in the denominator
+ * as in akv_decode_attention; a token that sees no key gets 0.  q, K and V are
+ * bf16 or fp16, the output q's type or f32; head_dim a multiple of 8 up to 128,
+ * any number of q heads per KV head.
  *
  * Slots: kv_indices[kv_indptr[b] + j] of a flat list of table_width entries
  * (table_stride 0, page_size 1), or, with table_stride > 0, the block table
  * row kv_indices + b * table_stride of table_width pages:
  * page(j / page_size) * page_size + j % page_size.  A key whose slot lies
  * outside [0, pool_slots), or whose entry outside the list, is seen by no
- * token (a pool or list of none may be NULL).  max_len (keys a request's tokens reach) and max_new (its tokens) are
- * host bounds that only size the launch: results do not depend on them (but
- * for the order of their fp32 sums).  A request has up to 2^30 keys; out must
- * not overlap q.
+ * token (a pool or list of none may be NULL).  max_len (keys a request's tokens
+ * reach) and max_new (its tokens) are host bounds that only size the launch:
+ * results do not depend on them (but for the order of their fp32 sums, and
+ * whether an infinite value that a token sees makes that dimension infinite or
+ * NaN).  A request has up to 2^30 keys; out must not overlap q.
  * n_tokens is the capacity of q and out; rows behind qo_indptr[B] stay as they
  * are.  workspace: akv_tree_attention_workspace_bytes with the same arguments
  * or with larger n_tokens, n_requests, max_len and max_new (it does not fall as
