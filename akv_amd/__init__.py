@@ -13,6 +13,10 @@ A drop-in for the KV-cache hot path of thu-nics/AKV:
   ``akv_amd.attention.tree_attention`` -- the step that verifies drafted
   tokens: metadata of the new tokens, per-head norms with the rotation and the
   pool write, attention of token trees (beside ``decode_attention``);
+* ``akv_amd.kv8`` -- the same path over a cache held in 8 bits with a scale for
+  each block of slots and head: rows appended with the rotation on the way, the
+  all-layer Reposition, attention of new tokens (windows with first keys that
+  stay visible);
 * ``akv_amd.context_attention.extend_attention_fwd`` -- prefill attention
   over the compacted rows with context positions;
 * ``akv_amd.plan.compile_context_layout`` -- the host event compiler;

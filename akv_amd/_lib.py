@@ -18,6 +18,7 @@ AKV_EINVAL = -22
 AKV_EHIP = -5
 AKV_ERUNTIME = -71
 AKV_F32, AKV_F16, AKV_BF16 = 0, 1, 2
+AKV_E4M3, AKV_E5M2 = 3, 4
 AKV_I32, AKV_I64 = 0, 1
 # status word of akv_compact_rows
 AKV_STATUS_SIZES, AKV_STATUS_INCOMPLETE, AKV_STATUS_REBUILT = 1, 2, 4
@@ -99,6 +100,30 @@ _SIGNATURES = {
          c_int32, c_int32, c_int32, _P, _P, c_int32, ctypes.c_float, _P, c_int32, _P, c_int32, c_int64,
          c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int32, _P, _P, c_int64, c_int64, c_int64,
          c_int64, c_int64, _P],
+    ),
+    "akv_kv8_append": (
+        c_int32,
+        [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, c_int32, c_int64, c_int32, c_int32,
+         c_int32, c_int32, c_int32, _P, c_int32, _P, c_int32, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int32,
+         _P, _P, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, c_int32, c_int64, c_int64, c_int64,
+         c_int64, _P],
+    ),
+    "akv_kv8_reposition": (
+        c_int32,
+        [_P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64,
+         c_int32, c_int64, c_int64, c_int64, c_int64, _P, _P, _P, c_int64, c_int64, _P, c_int32, c_int64, c_int64,
+         c_int32, c_int32, _P, _P],
+    ),
+    "akv_kv8_attention_workspace_bytes": (
+        c_int64,
+        [c_int64, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64],
+    ),
+    "akv_kv8_attention": (
+        c_int32,
+        [_P, c_int64, c_int64, c_int32, _P, _P, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, c_int32,
+         c_int64, c_int64, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, _P, _P, c_int32, _P,
+         c_int64, c_int64, c_int32, _P, c_int64, c_int32, _P, c_int32, _P, ctypes.c_float, _P, c_int32, c_int64,
+         c_int64, c_int64, c_int64, _P, c_int64, _P, _P],
     ),
     "akv_step_maps": (
         c_int32,

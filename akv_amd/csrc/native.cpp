@@ -76,6 +76,10 @@ PyObject* invoke(R (*fn)(A...), PyObject* slow, PyObject* const* args, Py_ssize_
   X(akv_tree_attention_workspace_bytes)   \
   X(akv_tree_attention)                   \
   X(akv_qk_norm_rope)                     \
+  X(akv_kv8_append)                       \
+  X(akv_kv8_reposition)                   \
+  X(akv_kv8_attention_workspace_bytes)    \
+  X(akv_kv8_attention)                    \
   X(akv_step_maps)                        \
   X(akv_context_attention)                \
   X(akv_context_attention_sized)          \

@@ -34,6 +34,10 @@ extern "C" {
 #define AKV_F16 1
 #define AKV_BF16 2
 
+/* 8-bit floats of KV buffers with scales (akv_kv8_*). */
+#define AKV_E4M3 3
+#define AKV_E5M2 4
+
 /* Integer dtypes of index vectors. */
 #define AKV_I32 0
 #define AKV_I64 1
@@ -872,6 +876,122 @@ int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                        int64_t out_stride_h, int64_t max_len, int64_t max_new,
                        void* workspace, int64_t workspace_bytes,
                        const int32_t* status, void* stream);
+
+/*
+ * A KV cache held in 8 bits.  Codes are 8-bit floats (AKV_E4M3: OCP e4m3 without
+ * infinities, largest F = 448; AKV_E5M2: F = 57344) in [slots, kv_heads, head_dim]
+ * buffers; scales are f32 [slots / scale_block, kv_heads], one for each block of
+ * scale_block slots (a power of two up to 64; block s / scale_block) and head, for K
+ * and for V; a value is code * scale.  head_dim is a multiple of 16 up to 128.
+ * Strides of codes and scales are in elements, the dims of a row are adjacent.
+ *
+ * The writers fill blocks in ascending order of their slots: the rows that a call
+ * brings to a block follow one another in its list, slots ascending by 1, slots are
+ * distinct, and the slots of the block below the first of them hold earlier rows
+ * (what lies above the last of them holds nothing any more).  With A the largest
+ * finite magnitude of these rows in a head, the block's scale becomes
+ *   first row at the block's first slot: the smallest power of two s >= 2^-100
+ *     with A <= F s;
+ *   else: s0 2^k, s0 the scale it has, with the least k >= 0 that gives
+ *     A <= F s0 2^k; for k > 0 the codes below become round(code * 2^-k).  (A
+ *     scale that is not positive and finite scales nothing: those codes become 0.  One
+ *     below 2^-100 that is too small gives way to the first rule's.)
+ * and each value y becomes round(y / s), to nearest, ties to even; values that are
+ * not finite become the format's NaN or infinity (e4m3: NaN).
+ *
+ * akv_kv8_append: K rows k[t], rotated by row positions[t] of cos_sin as in
+ * akv_qk_norm_rope (products and sums rounded one by one in fp32; rotary_dim 0: no
+ * rotation, then q_heads is 0), and V rows v[t] go to slot slots[t]; q rows, rotated
+ * and rounded to `dtype`, to q_out (which may be q).  A slot outside [0,
+ * pool_slots) takes nothing (-1: padding).  A position outside [0, rope_rows)
+ * gives NaN q and K rows.
+ *
+ * No counterpart in the reference, whose Reposition takes unquantized KV only
+ * (akv/system/sglang/kernels/ops/attention/context_reposition.py:149-152).
+ */
+int akv_kv8_append(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                   const void* k, int64_t k_stride_t, int64_t k_stride_h,
+                   const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                   int32_t dtype, int64_t n_tokens, int32_t q_heads,
+                   int32_t kv_heads, int32_t head_dim, int32_t rotary_dim,
+                   int32_t is_neox, const void* positions,
+                   int32_t positions_dtype, const void* cos_sin,
+                   int32_t cos_sin_dtype, int64_t rope_stride,
+                   int64_t rope_rows, void* q_out, int64_t qo_stride_t,
+                   int64_t qo_stride_h, const void* slots, int32_t slots_dtype,
+                   void* k_pool, void* v_pool, int32_t format,
+                   int64_t pool_slots, int64_t kp_stride_slot,
+                   int64_t kp_stride_head, int64_t vp_stride_slot,
+                   int64_t vp_stride_head, float* k_scales, float* v_scales,
+                   int32_t scale_block, int64_t ks_stride_block,
+                   int64_t ks_stride_head, int64_t vs_stride_block,
+                   int64_t vs_stride_head, void* stream);
+
+/*
+ * akv_reposition_kv_layers_gated over such caches: for every layer, the values of
+ * slot src[t] go to slot dst[t], K's rotary part turned from position pairs[t][0]
+ * to pairs[t][1] by the factors c = (cn co + sn so) / (co^2 + so^2), s = (sn co - cn
+ * so) / (co^2 + so^2) in fp32 (not at all where the two are equal), and are
+ * stored as above.  Sources lie outside the blocks that the call writes.  The four
+ * pointer tables are DEVICE arrays of n_layers base addresses of buffers and scales
+ * that share the given strides.  An entry whose dst is outside [0, pool_slots)
+ * (or, with skip_unmapped, 0) is passed over; one whose src is, is not written.  A
+ * position outside [0, rope_rows) gives a NaN K row unless both are equal.
+ * status as in akv_reposition_kv_layers_gated.
+ */
+int akv_kv8_reposition(const uint64_t* k_ptrs, const uint64_t* v_ptrs,
+                       const uint64_t* k_scale_ptrs,
+                       const uint64_t* v_scale_ptrs, int32_t n_layers,
+                       int32_t format, int32_t n_heads, int32_t head_dim,
+                       int32_t rotary_dim, int64_t pool_slots,
+                       int64_t k_stride_slot, int64_t k_stride_head,
+                       int64_t v_stride_slot, int64_t v_stride_head,
+                       int32_t scale_block, int64_t ks_stride_block,
+                       int64_t ks_stride_head, int64_t vs_stride_block,
+                       int64_t vs_stride_head, const int32_t* src,
+                       const int32_t* dst, const int32_t* pairs,
+                       int64_t pair_stride, int64_t n_tokens,
+                       const void* cos_sin, int32_t cos_sin_dtype,
+                       int64_t rope_stride, int64_t rope_rows, int32_t is_neox,
+                       int32_t skip_unmapped, const int32_t* status,
+                       void* stream);
+
+/*
+ * akv_tree_attention over a cache held in 8 bits (akv_kv8_append), of any number of
+ * new tokens per request: a key's score is scale * its K scale * (q . its codes), its
+ * value its V scale * its codes.  q is bf16 or fp16, out has q's type or is f32.  An
+ * earlier key of rank j is seen by token i when j < first_keys or j >=
+ * key_starts[i] (NULL: always): a window with a few first keys that stay visible.
+ * What no token sees of the earlier keys is not read, so max_len is first_keys +
+ * window + n + 1 for a window.  Rows of K and V are 16-byte aligned, scales may have
+ * any strides; everything else is as in akv_tree_attention.
+ */
+int64_t akv_kv8_attention_workspace_bytes(int64_t n_tokens, int32_t n_requests,
+                                          int32_t q_heads, int32_t kv_heads,
+                                          int32_t head_dim, int64_t max_len,
+                                          int64_t max_new);
+int akv_kv8_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                      int32_t dtype, const void* k_buffer,
+                      const void* v_buffer, int32_t format,
+                      int64_t k_stride_slot, int64_t k_stride_head,
+                      int64_t v_stride_slot, int64_t v_stride_head,
+                      int64_t pool_slots, const float* k_scales,
+                      const float* v_scales, int32_t scale_block,
+                      int64_t ks_stride_block, int64_t ks_stride_head,
+                      int64_t vs_stride_block, int64_t vs_stride_head,
+                      int64_t n_tokens, int32_t n_requests, int32_t q_heads,
+                      int32_t kv_heads, int32_t head_dim,
+                      const void* qo_indptr, const void* kv_indptr,
+                      int32_t indptr_dtype, const int32_t* kv_indices,
+                      int64_t table_stride, int64_t table_width,
+                      int32_t page_size, const uint64_t* tree_mask,
+                      int64_t mask_stride, int32_t mask_words,
+                      const int32_t* key_starts, int32_t first_keys,
+                      const float* sinks, float scale, void* out,
+                      int32_t out_dtype, int64_t out_stride_t,
+                      int64_t out_stride_h, int64_t max_len, int64_t max_new,
+                      void* workspace, int64_t workspace_bytes,
+                      const int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }
