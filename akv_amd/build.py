@@ -31,7 +31,7 @@ HIP_SOURCES = [
     "common.hip", "reposition.hip", "compact.hip", "compact_pages.hip", "decode_meta.hip", "decode_attention.hip",
     "context_attention.hip", "bind_occurrences.hip", "kv_transfer.hip", "gather_slots.hip",
     "step_maps.hip", "qk_norm.hip", "tree_attention.hip",
-    "kv8_rows.hip", "kv8_attention.hip",
+    "kv8_append.hip", "kv8_move.hip", "kv8_attention.hip",
 ]
 CXX_SOURCES = ["event_plan.cpp", "occurrence_window.cpp", "ownership.cpp"]
 

@@ -896,8 +896,9 @@ int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  *     A <= F s0 2^k; for k > 0 the codes below become round(code * 2^-k).  (A
  *     scale that is not positive and finite scales nothing: those codes become 0.  One
  *     below 2^-100 that is too small gives way to the first rule's.)
- * and each value y becomes round(y / s), to nearest, ties to even; values that are
- * not finite become the format's NaN or infinity (e4m3: NaN).
+ * and each value y becomes round(y / s), to nearest, ties to even (y times 1 / s in
+ * fp32, which is exact unless s0 is no power of two); values that are not finite
+ * become the format's NaN or infinity (e4m3: NaN).
  *
  * akv_kv8_append: K rows k[t], rotated by row positions[t] of cos_sin as in
  * akv_qk_norm_rope (products and sums rounded one by one in fp32; rotary_dim 0: no
@@ -931,8 +932,8 @@ int akv_kv8_append(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  * akv_reposition_kv_layers_gated over such caches: for every layer, the values of
  * slot src[t] go to slot dst[t], K's rotary part turned from position pairs[t][0]
  * to pairs[t][1] by the factors c = (cn co + sn so) / (co^2 + so^2), s = (sn co - cn
- * so) / (co^2 + so^2) in fp32 (not at all where the two are equal), and are
- * stored as above.  Sources lie outside the blocks that the call writes.  The four
+ * so) / (co^2 + so^2) in fp32, in units of the source's scale (not at all where the
+ * two are equal), and are stored as above.  Sources lie outside the blocks that the call writes.  The four
  * pointer tables are DEVICE arrays of n_layers base addresses of buffers and scales
  * that share the given strides.  An entry whose dst is outside [0, pool_slots)
  * (or, with skip_unmapped, 0) is passed over; one whose src is, is not written.  A

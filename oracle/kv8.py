@@ -93,17 +93,21 @@ def runs(slots, block, total):
     return out
 
 
-def store(codes, scales, rows, slots, block, form, live=None):
-    """Rows ``[N, heads, D]`` into ``codes`` ``[slots, heads, D]`` (the codes'
-    values) and ``scales`` ``[blocks, heads]``, in place.  ``live``: rows that are written."""
+def store(codes, scales, rows, slots, block, form, live=None, units=1.0):
+    """Rows ``[N, heads, D]`` in units ``[N, heads, 1]`` into ``codes`` ``[slots,
+    heads, D]`` (the codes' values) and ``scales`` ``[blocks, heads]``, in place.
+    ``live``: rows that are written."""
     rows, real = np.asarray(rows), np.asarray(rows).dtype.type
+    units = np.broadcast_to(np.asarray(units, dtype=real), (*rows.shape[:2], 1))
     for t, n in runs(slots, block, len(codes)):
         at, first = slots[t] // block, slots[t] % block
         here = np.arange(t, t + n)
         if live is not None:
             here = here[np.asarray(live)[t: t + n]]
-        x = rows[here]
-        top = np.where(np.isfinite(x), np.abs(x), 0).max((0, 2), initial=0)
+        x, unit = rows[here], units[here]
+        with np.errstate(over="ignore", invalid="ignore"):
+            y = x * unit
+        top = np.where(np.isfinite(y), np.abs(y), 0).max((0, 2), initial=0)
         before = scales[at].copy()
         after = grown(top, before, form) if first else fitting(top, form)
         scales[at] = after
@@ -114,14 +118,17 @@ def store(codes, scales, rows, slots, block, form, live=None):
             changed = after != before
             codes[lower] = np.where(changed[None, :, None], rounded(codes[lower] * ratio[None, :, None], form), codes[lower])
         with np.errstate(over="ignore", invalid="ignore"):
-            codes[np.asarray(slots)[here]] = rounded(x / after.astype(real)[None, :, None], form)
+            by = unit * (real(1) / after.astype(real))[None, :, None]
+            by = np.where((by == np.inf) & (unit < np.inf), np.finfo(real).max, by)  # (a row of zeros)
+            codes[np.asarray(slots)[here]] = rounded(x * by, form)
 
 
 def moved_rows(codes, scales, src, pairs, table, block, rotary_dim, neox, real, rotates):
-    """The values of slots ``src``, K's turned from pairs[:, 0] to pairs[:, 1]."""
-    x = codes[src].astype(real) * scales[np.asarray(src) // block].astype(real)[..., None]
+    """The values of slots ``src``, K's turned from pairs[:, 0] to pairs[:, 1], and
+    the units they are in, their scales."""
+    x, unit = codes[src].astype(real), scales[np.asarray(src) // block].astype(real)[..., None]
     if not rotates:
-        return x
+        return x, unit
     half, pairs = rotary_dim // 2, np.asarray(pairs, dtype=np.int64)
     known = ((pairs >= 0) & (pairs < len(table))).all(1)
     old, new = (np.asarray(table, dtype=real)[np.where(known, pairs[:, i], 0)] for i in (0, 1))
@@ -131,4 +138,4 @@ def moved_rows(codes, scales, src, pairs, table, block, rotary_dim, neox, real, 
     out[~known] = np.nan
     same = pairs[:, 0] == pairs[:, 1]
     out[same] = x[same]
-    return out
+    return out, unit

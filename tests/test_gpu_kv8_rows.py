@@ -12,12 +12,12 @@ from tests.kv8 import FORMATS, LARGEST, layer, paged_slots, same, values
 pytestmark = pytest.mark.gpu
 
 
-def _want(cache, rows, slots, block, form, live=None):
+def _want(cache, rows, slots, block, form, live=None, units=(1.0, 1.0)):
     """What the oracle leaves of [[k codes, k scales], [v codes, v scales]]."""
     out = []
-    for (codes, scales), x in zip(cache, rows):
+    for (codes, scales), x, unit in zip(cache, rows, units):
         w, s = values(codes), f64(scales).copy()
-        oracle.store(w, s, x, slots, block, form, live)
+        oracle.store(w, s, x, slots, block, form, live, unit)
         out.append((w, s))
     return out
 
@@ -251,7 +251,9 @@ def _move(device, seed, src, dst, pairs, slots, *, layers=3, heads=2, d=64, rota
     for cache in caches:
         rows = [oracle.moved_rows(values(c), f64(s), at, pairs, _f32(table), block, rotary, neox, np.float32, i == 0)
                 for i, (c, s) in enumerate(cache)]
-        want.append([(values(c), f64(s)) for c, s in cache] if untouched else _want(cache, rows, to, block, form, usable))
+        rows, units = zip(*rows)
+        want.append([(values(c), f64(s)) for c, s in cache] if untouched
+                    else _want(cache, rows, to, block, form, usable, units))
     dev = lambda x: torch.from_numpy(np.ascontiguousarray(x, dtype=np.int32)).to(device)  # noqa: E731
     pointers = [torch.tensor([c[i][j].data_ptr() for c in caches], dtype=torch.int64, device=device)
                 for j in (0, 1) for i in (0, 1)]

@@ -236,8 +236,8 @@ def test_turn_end_over_an_8_bit_cache(device, page, block):
     at = rope_table.cpu().numpy()
     for cache, held in zip(caches, before):
         for i, ((codes, scales), (c, s)) in enumerate(zip(cache, held)):
-            moved = oracle.moved_rows(c, s, src, pairs, at, block, d, True, np.float32, i == 0)
-            oracle.store(c, s, moved, dst, block, "e4m3")
+            moved, units = oracle.moved_rows(c, s, src, pairs, at, block, d, True, np.float32, i == 0)
+            oracle.store(c, s, moved, dst, block, "e4m3", units=units)
             np.testing.assert_array_equal(values(codes), c)
             np.testing.assert_array_equal(f64(scales), s)
     # one token decodes over what was kept

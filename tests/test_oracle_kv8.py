@@ -89,7 +89,7 @@ def test_fp32_rows_are_the_64_bit_rows(form, neox):
     scales = np.exp2(rng.integers(-9, -5, (16, 2)).astype(np.float64))
     src, pairs = rng.permutation(64)[:30], rng.integers(0, 900, (30, 2))
     pairs[::5, 1] = pairs[::5, 0]
-    got, want = (oracle.moved_rows(codes, scales, src, pairs, table, 4, 32, neox, real, True)
+    got, want = (np.multiply(*oracle.moved_rows(codes, scales, src, pairs, table, 4, 32, neox, real, True))
                  for real in (np.float32, np.float64))
     size = np.abs(want).max()
     assert np.abs(got - want).max() <= 10 * 2.0 ** -24 * 2 * size
