@@ -164,18 +164,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     const int32_t n = q1 > q0 ? static_cast<int32_t>(q1 - q0) : 0;
     return Cost{units_of(keys_in(b), n, rb), n * a.group};
   };
-  int32_t lane_units = 0;  // of request `lane`, for the block of rows last summed
-  auto sum_of = [&](int rb, int32_t* most_rows) -> int64_t {
+  auto sum_of = [&](int rb) -> int64_t {
     int64_t sum = 0;
-    int32_t most = 0;
-    lane_units = 0;
-    for (int b = lane; b < a.n_requests; b += 64) {
-      const Cost c = cost_of(b, rb);
-      if (b < 64) lane_units = c.units;
-      sum += c.units;
-      most = max(most, c.rows);
-    }
-    *most_rows = uniform(__ockl_wfred_max_i32(most));
+    for (int b = lane; b < a.n_requests; b += 64) sum += cost_of(b, rb).units;
     return uniform(static_cast<int64_t>(__ockl_wfred_add_i64(sum)));
   };
 
@@ -192,17 +183,17 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
   } else {
     // all work on a line: blocks of rows, KV heads, requests (fastest).  The
     // workgroups take equal stretches of it; a cut falls among a request's tiles.
-    int32_t most_rows;
-    int64_t sum = sum_of(0, &most_rows);
-    blocks = (most_rows + R - 1) / R;
-    int64_t all = sum;
-    const int32_t first_units = lane_units;
-    for (int i = 1; i < blocks; ++i) {
-      int32_t unused;
-      all += sum_of(i, &unused);
+    int32_t most = 0;
+    for (int i = lane; i < a.n_requests; i += 64) most = max(most, cost_of(i, 0).rows);
+    blocks = (uniform(__ockl_wfred_max_i32(most)) + R - 1) / R;
+    const int64_t items = static_cast<int64_t>(blocks) * a.n_requests;
+    int64_t mine = 0;
+    for (int64_t i = lane; i < items; i += 64) {
+      const int64_t at = items >> 31 ? i / a.n_requests : static_cast<uint32_t>(i) / static_cast<uint32_t>(a.n_requests);
+      mine += cost_of(i - at * a.n_requests, static_cast<int>(at)).units;
     }
-    all *= a.kv_heads;
-    lane_units = first_units;
+    const int64_t until = __ockl_wfscan_add_i64(mine, true);
+    const int64_t all = uniform(__shfl(until, 63)) * a.kv_heads;
     if (all == 0) return;
     // 2^k stretches: all of the workgroups, or as many as get their least share
     int k = kGroupsShift;
@@ -211,25 +202,38 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     auto cut = [&](int64_t i) { return (all >> k) * i + (((all & ((1 << k) - 1)) * i) >> k); };  // all * i / 2^k
     int64_t x = cut(group_id);
     budget = cut(group_id + 1) - x;
-    rb = 0;
-    while (x >= sum * a.kv_heads) {
-      int32_t unused;
-      x -= sum * a.kv_heads;
-      sum = sum_of(++rb, &unused);
-    }
-    for (g = 0; x >= sum; ++g) x -= sum;
-    b = 0;
-    for (int b0 = 0; b0 < a.n_requests; b0 += 64) {
-      const int32_t mine = b0 == 0 ? lane_units : b0 + lane < a.n_requests ? cost_of(b0 + lane, rb).units : 0;
-      const int64_t until = __ockl_wfscan_add_i64(mine, true);
-      const uint64_t past = __builtin_amdgcn_ballot_w64(until > x);
-      if (past) {
-        const int at = __builtin_ctzll(past);
-        b = b0 + at;
-        off = uniform(x - __shfl(until - mine, at));
-        break;
+    if (items <= 64) {
+      // a lane has an item, all of a block's side by side
+      rb = __builtin_ctzll(__builtin_amdgcn_ballot_w64(until * a.kv_heads > x)) / a.n_requests;
+      const int at = rb * a.n_requests;
+      const int64_t before = uniform(__shfl(until - mine, at));
+      const int64_t sum = uniform(__shfl(until, at + a.n_requests - 1)) - before;
+      x -= before * a.kv_heads;
+      for (g = 0; x >= sum; ++g) x -= sum;
+      const int item = __builtin_ctzll(__builtin_amdgcn_ballot_w64(until - before > x));
+      off = x - (uniform(__shfl(until - mine, item)) - before);
+      b = item - at;
+    } else {
+      rb = 0;
+      int64_t sum = sum_of(0);
+      while (x >= sum * a.kv_heads) {
+        x -= sum * a.kv_heads;
+        sum = sum_of(++rb);
       }
-      x -= __shfl(until, 63);
+      for (g = 0; x >= sum; ++g) x -= sum;
+      b = 0;
+      for (int b0 = 0; b0 < a.n_requests; b0 += 64) {
+        const int32_t units = b0 + lane < a.n_requests ? cost_of(b0 + lane, rb).units : 0;
+        const int64_t up = __ockl_wfscan_add_i64(units, true);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(up > x);
+        if (past) {
+          const int at = __builtin_ctzll(past);
+          b = b0 + at;
+          off = uniform(x - __shfl(up - units, at));
+          break;
+        }
+        x -= __shfl(up, 63);
+      }
     }
   }
 
@@ -620,6 +624,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     __syncthreads();
     if (tiles > 0) stage(0);
     arrive();
+    // keys that all of the wave's rows are late enough for
+    const int sure = a.mask ? old : old + uniform(min(row0, rows - 1) / a.group) + 1;
     // this wave's parts of a tile
     uint32_t parts = 0;
 #pragma unroll
@@ -631,23 +637,29 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
       const CodeTile<D>& t = buffers[it % kBuffers];
       const int t0 = begin + it * kKeys;
       const uint32_t* dead = s_dead[it % (2 * kEntryTiles)];
-      uint32_t holes = dead[0];
-#pragma unroll
-      for (int kk = 1; kk < kParts; ++kk) holes |= dead[kk];
-      uint32_t todo = parts;
-      if (!unset && t0 + kKeys + gap <= old && (t0 + gap >= hi_start || t0 + kKeys <= kept) && uniform(holes) == 0) {
+      // the parts that all of the wave's rows see: behind their windows' starts or in the
+      // first keys, before their tokens, without a hole
+      auto below = [&](int at) -> uint32_t {  // parts that end at `at` or before
+        const int x = (at - t0) >> 5;
+        return x >= kParts ? (2u << (kParts - 1)) - 1 : x <= 0 ? 0 : (1u << x) - 1;
+      };
+      const uint32_t holes = __builtin_amdgcn_ballot_w64(dead[lane % kParts] != 0);
+      uint32_t ready = below(sure - gap) & ~(below(hi_start - gap + 31) & ~below(kept)) & ~holes;
+      uint32_t todo = parts & below(end + 31);
 #pragma nounroll
-        for (uint32_t rest = todo; rest; rest &= rest - 1) {
-          const int kk = __builtin_ctz(rest);
-          if (!quick(t, it, kk)) break;
-          todo &= ~(1u << kk);
+      while (todo) {
+        if (!unset) {
+#pragma nounroll
+          for (uint32_t rest = todo & ready; rest; rest &= rest - 1) {
+            const int kk = __builtin_ctz(rest);
+            if (!quick(t, it, kk)) break;
+            todo &= ~(1u << kk);
+          }
         }
-      }
-#pragma nounroll
-      for (; todo; todo &= todo - 1) {
-        const int kk = __builtin_ctz(todo), v0 = t0 + 32 * kk;
-        if (v0 >= end) break;
-        part(t, it, kk, v0, uniform(dead[kk]));
+        if (todo == 0) break;
+        const int kk = __builtin_ctz(todo);
+        part(t, it, kk, t0 + 32 * kk, uniform(dead[kk]));
+        todo &= todo - 1;
       }
       arrive();
     }
