@@ -441,12 +441,19 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
 #pragma unroll
     for (int dt = 0; dt < kDTiles; ++dt) v_at[dt] = vr * D + 16 * (dt ^ swz_v<D>(vr)) + 8 * (col & 1);
     // products of the 32 keys of a part: S^T[16 j + 4 quad + i][row 16 s + col]
-    auto scores = [&](const CodeTile<D>& t, int kk, f32x4 (&sc)[2][SUB]) KV8_INLINE {
+    auto codes_of = [&](const CodeTile<D>& t, int kk, u32x4 (&k)[2][kSteps / 2]) KV8_INLINE {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < kSteps / 2; ++h)
+          k[j][h] = *reinterpret_cast<const u32x4*>(t.k + (32 * kk + 16 * j) * D + k_at[h]);
+    };
+    auto scores = [&](const u32x4 (&k)[2][kSteps / 2], f32x4 (&sc)[2][SUB]) KV8_INLINE {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int h = 0; h < kSteps / 2; ++h) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(t.k + (32 * kk + 16 * j) * D + k_at[h]);
+          const u32x4 w = k[j][h];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const x8 kop = operand<T, E5>(u32x2{w[2 * half], w[2 * half + 1]});
@@ -494,9 +501,16 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     // nothing done, where a sum outgrows kHuge
     auto quick = [&](const CodeTile<D>& t, int it, int kk) KV8_INLINE -> bool {
       f32x4 sc[2][SUB], ks[2], vs[2];
+      u32x4 k[2][kSteps / 2];
+      u32x2 v[kDTiles];
+      // all reads first: none of them waits behind a matrix product or the branch
+      codes_of(t, kk, k);
       scales_of(it, 0, kk, ks);
       scales_of(it, 1, kk, vs);
-      scores(t, kk, sc);
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt) v[dt] = v_tile(t, kk, dt);
+      __builtin_amdgcn_sched_barrier(0);
+      scores(k, sc);
       ks[0] *= a.scale_log2;
       ks[1] *= a.scale_log2;
       Weights p[SUB];
@@ -522,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
 #pragma unroll
       for (int s = 0; s < SUB; ++s) l[s] = sum[s];
 #pragma unroll
-      for (int dt = 0; dt < kDTiles; ++dt) add_values(v_tile(t, kk, dt), dt, p);
+      for (int dt = 0; dt < kDTiles; ++dt) add_values(v[dt], dt, p);
       return true;
     };
     // any 32 keys; v0: the first one's number
@@ -530,7 +544,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
       f32x4 sc[2][SUB], ks[2], vs[2];
       scales_of(it, 0, kk, ks);
       scales_of(it, 1, kk, vs);
-      scores(t, kk, sc);
+      u32x4 k[2][kSteps / 2];
+      codes_of(t, kk, k);
+      scores(k, sc);
       uint32_t seen[SUB];  // bit 4 j + i: key 16 j + 4 quad + i
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
