@@ -44,8 +44,8 @@ typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
 #define KV8_INLINE __attribute__((always_inline))
 
-// Keys of a tile (32 KiB of K and V), and the tiles in LDS.
-constexpr int keys_of(int d) { return d == 64 ? 256 : 128; }
+// Keys of a tile of rows of `width` bytes (32 KiB of K and V), and the tiles in LDS.
+constexpr int keys_of(int width) { return width == 64 ? 256 : 128; }
 constexpr int kBuffers = 2;
 
 // What a piece costs beside its tiles, and the least a workgroup is given, in keys.
@@ -57,16 +57,17 @@ struct Kv8Args {
   const float* v_scales;
   int64_t ks_sb, ks_sh, vs_sb, vs_sh;
   int32_t log2_block, first_keys;
+  int32_t block_rows;  // rows of a block where a workgroup has two heads
 };
 
 // 16-byte chunk c of row r lies at chunk c ^ swz(r): the 16 rows of an operand read
 // (K), and the rows 4 g + i, 16 + 4 g + i of a transposed read's lanes (V), take
 // distinct banks.
-template <int D>
-__device__ __forceinline__ int swz_k(int r) { return D == 64 ? (r >> 2) & 3 : (r >> 1) & 7; }
-template <int D>
+template <int W>
+__device__ __forceinline__ int swz_k(int r) { return W == 64 ? (r >> 2) & 3 : (r >> 1) & 7; }
+template <int W>
 __device__ __forceinline__ int swz_v(int r) {
-  return D == 64 ? (r >> 2 & 1) | (r >> 4 & 1) << 1 : (r >> 1 & 3) | (r >> 4 & 1) << 2;
+  return W == 64 ? (r >> 2 & 1) | (r >> 4 & 1) << 1 : (r >> 1 & 3) | (r >> 4 & 1) << 2;
 }
 
 // Eight codes as an operand of the matrix cores.
@@ -98,33 +99,38 @@ __device__ __forceinline__ uint32_t odd_bytes(uint32_t w) {
   return E5 ? ((w & 0x7c7c7c7cu) + 0x04040404u) & 0x80808080u : ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
 
-template <int D>
+template <int W>
 struct alignas(16) CodeTile {
-  char k[keys_of(D) * D];  // key-major, 16-byte chunks swizzled per row (swz_k)
-  char v[keys_of(D) * D];  // key-major, read transposed, swizzled (swz_v)
+  char k[keys_of(W) * W];  // key-major, 16-byte chunks swizzled per row (swz_k)
+  char v[keys_of(W) * W];  // key-major, read transposed, swizzled (swz_v)
 };
 
 // T: q's type.  D: 64 or 128, the tile's head width.  SUB: a wave's row subtiles of 16.
-template <typename T, bool E5, int D, int SUB>
+// HEADS: a workgroup's KV heads, side by side in a tile's rows; of two, waves 0 and 1
+// have the first and the others the second.  To the line of work, the cuts and the
+// merge the two are one head of twice the group (`ka.t` comes so): row r of a block
+// is that of token r / (2 G) and of the first head while r % (2 G) < G.
+template <typename T, bool E5, int D, int SUB, int HEADS>
 __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Args ka) {
   const TreeArgs& a = ka.t;
   using x8 = typename Vec<T>::x8;
   using b4 = Vec<__bf16>::x4;
   using b8 = Vec<__bf16>::x8;
   constexpr bool kSplit = !__is_same(T, __bf16);  // weights as two bf16 values
-  constexpr int kKeys = keys_of(D);
+  constexpr int W = D * HEADS;                 // bytes of a tile's row
+  constexpr int kKeys = keys_of(W);
   constexpr int kParts = kKeys / 32;
   constexpr int kSteps = D / 32;
   constexpr int kDTiles = D / 16;
-  constexpr int kChunks = D / 16;              // 16-byte chunks of a row
+  constexpr int kChunks = W / 16;              // 16-byte chunks of a row
   constexpr int kLoadRows = 64 / kChunks;      // rows of one wave-wide load
   constexpr int kWaveKeys = kKeys / kWaves;    // keys of a tile that a wave asks for
   constexpr int kEntryTiles = 64 / kWaveKeys;  // tiles whose keys of this wave fill a vector register
   constexpr int kOver = (kPieceCost + kKeys - 1) / kKeys;
   constexpr int kGroupRows = 16 * SUB;         // rows of a wave
-  constexpr int R = kWaves * kGroupRows;       // rows of a block
-  __shared__ CodeTile<D> buffers[kBuffers];
-  __shared__ __attribute__((aligned(16))) float s_scale[kBuffers][kWaves][2][kWaveKeys];  // the tiles' a_j and c_j
+  const int R = HEADS == 1 ? kWaves * kGroupRows : ka.block_rows;  // rows of a block
+  __shared__ CodeTile<W> buffers[kBuffers];
+  __shared__ __attribute__((aligned(16))) float s_scale[kBuffers][kWaves][2][kWaveKeys * HEADS];  // the tiles' a_j and c_j
   __shared__ int32_t s_entry[kWaves][2][64];  // list entries of the waves' keys, kEntryTiles tiles at a time
   __shared__ uint32_t s_dead[2 * kEntryTiles][kParts];  // the tiles' keys that no token sees
   __shared__ float s_m[kWaves][kGroupRows], s_l[kWaves][kGroupRows];
@@ -281,12 +287,15 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
 
     // (an empty pool holds no key: every slot is a hole, and zeros are read)
     const bool pool = a.pool_slots > 0;
-    const char* kbase = pool ? a.k + g * a.k_sh : reinterpret_cast<const char*>(zero_row);
-    const char* vbase = pool ? a.v + g * a.v_sh : reinterpret_cast<const char*>(zero_row);
-    const float* ks_base = pool ? ka.k_scales + g * ka.ks_sh : reinterpret_cast<const float*>(zero_row);
-    const float* vs_base = pool ? ka.v_scales + g * ka.vs_sh : reinterpret_cast<const float*>(zero_row);
+    const char* kbase = pool ? a.k + static_cast<int64_t>(HEADS) * g * a.k_sh : reinterpret_cast<const char*>(zero_row);
+    const char* vbase = pool ? a.v + static_cast<int64_t>(HEADS) * g * a.v_sh : reinterpret_cast<const char*>(zero_row);
+    const float* ks_base = pool ? ka.k_scales + HEADS * g * ka.ks_sh : reinterpret_cast<const float*>(zero_row);
+    const float* vs_base = pool ? ka.v_scales + HEADS * g * ka.vs_sh : reinterpret_cast<const float*>(zero_row);
     const uint32_t k_ss = pool ? a.k_ss : 0, v_ss = pool ? a.v_ss : 0;
     const int64_t ks_sb = pool ? ka.ks_sb : 0, vs_sb = pool ? ka.vs_sb : 0;
+    // from the first head to the second
+    const int64_t k_next = pool ? a.k_sh : 0, v_next = pool ? a.v_sh : 0;
+    const int64_t ks_next = pool ? ka.ks_sh : 0, vs_next = pool ? ka.vs_sh : 0;
     const int32_t* list = a.kv_indices + (a.paged ? b * a.table_stride : kv0);
     // entries of the list that exist
     const int64_t left = a.paged ? a.table_width : kv0 < 0 ? 0 : a.table_width - kv0;
@@ -334,49 +343,59 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
         look_up(it / kEntryTiles);
         fetch(it / kEntryTiles + 1);
       }
-      CodeTile<D>& t = buffers[it % kBuffers];
+      CodeTile<W>& t = buffers[it % kBuffers];
 #pragma unroll
       for (int u = 0; u < kWaveKeys / kLoadRows; ++u) {
         const int mine = u * kLoadRows + lane / kChunks, r = kWaveKeys * wave + mine;
         const uint64_t from = __shfl(slots, it % kEntryTiles * kWaveKeys + mine);
-        const int ck = (lane % kChunks) ^ swz_k<D>(r), cv = (lane % kChunks) ^ swz_v<D>(r);
-        const char* krow = kbase + from * k_ss + 16 * ck;
-        const char* vrow = vbase + from * v_ss + 16 * cv;
+        const int ck = (lane % kChunks) ^ swz_k<W>(r), cv = (lane % kChunks) ^ swz_v<W>(r);
+        const int dk = 16 * ck % D, dv = 16 * cv % D;
+        const char* krow = kbase + from * k_ss + dk;
+        const char* vrow = vbase + from * v_ss + dv;
+        if constexpr (HEADS == 2) {
+          krow += 16 * ck < D ? 0 : k_next;
+          vrow += 16 * cv < D ? 0 : v_next;
+        }
         // dims past head_dim read zeros
-        krow = 16 * ck < a.head_dim ? krow : reinterpret_cast<const char*>(zero_row);
-        vrow = 16 * cv < a.head_dim ? vrow : reinterpret_cast<const char*>(zero_row);
-        const int place = (kWaveKeys * wave + u * kLoadRows) * D;
+        krow = dk < a.head_dim ? krow : reinterpret_cast<const char*>(zero_row);
+        vrow = dv < a.head_dim ? vrow : reinterpret_cast<const char*>(zero_row);
+        const int place = (kWaveKeys * wave + u * kLoadRows) * W;
         load_16(krow, uniform(lds_address(t.k + place)));
         load_16(vrow, uniform(lds_address(t.v + place)));
       }
-      // a_j of the wave's keys, then c_j: one load of 64 lanes each, or half of it
+      // a_j of the wave's keys, then c_j, 64 lanes at a time; of two heads those of a
+      // key side by side
 #pragma unroll
-      for (int u = 0; u < 2 * kWaveKeys; u += 64) {
-        const bool is_v = u + lane >= kWaveKeys;
-        const uint32_t block = __shfl(slots, it % kEntryTiles * kWaveKeys + lane % kWaveKeys) >> ka.log2_block;
-        load_4(is_v ? vs_base + block * vs_sb : ks_base + block * ks_sb,
-               uniform(lds_address(s_scale[it % kBuffers][wave][0] + u)));
+      for (int u = 0; u < 2 * HEADS * kWaveKeys; u += 64) {
+        const bool is_v = u + lane >= HEADS * kWaveKeys;
+        const uint32_t block = __shfl(slots, it % kEntryTiles * kWaveKeys + lane / HEADS % kWaveKeys) >> ka.log2_block;
+        const float* from = is_v ? vs_base + block * vs_sb : ks_base + block * ks_sb;
+        if constexpr (HEADS == 2) from += lane % 2 == 0 ? 0 : is_v ? vs_next : ks_next;
+        load_4(from, uniform(lds_address(s_scale[it % kBuffers][wave][0] + u)));
       }
     };
     if (tiles > 0) fetch(0);
-    // groups of rows, and the waves that share one
-    int groups = kWaves, sharers = 1;
-    while (groups > 1 && sharers < kParts && rows - rb * R <= (groups >> 1) * kGroupRows) {
+    // a head's groups of rows, and the waves that share one
+    constexpr int kHeadWaves = kWaves / HEADS;
+    const int heads_group = a.group / HEADS, head_rows = n * heads_group, block_row0 = rb * (R / HEADS);
+    const int hw = wave / kHeadWaves;  // the wave's head
+    int groups = kHeadWaves, sharers = 1;
+    while (groups > 1 && sharers < kParts && head_rows - block_row0 <= (groups >> 1) * kGroupRows) {
       groups >>= 1;
       sharers <<= 1;
     }
-    const int row0 = rb * R + (wave & (groups - 1)) * kGroupRows;
-    const int share = uniform(wave / groups);
-    // this lane's rows: r = row0 + 16 s + col, token r / G, head g G + r % G
+    const int row0 = block_row0 + (wave & (groups - 1)) * kGroupRows;
+    const int share = uniform(wave % kHeadWaves / groups);
+    // this lane's rows of the head: r = row0 + 16 s + col, token r / G, q head r % G of its G
     // (rows past the last repeat it and are never stored).  Step st of a product takes
     // bytes 8 (st % 2) of the 16 code bytes 64 (st / 2) + 16 quad.
     x8 qop[SUB][kSteps];
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-      const int r = min(row0 + 16 * s + col, rows - 1);
-      const int tok = r / a.group;
+      const int r = min(row0 + 16 * s + col, head_rows - 1);
+      const int tok = r / heads_group;
       const T* row = static_cast<const T*>(a.q) + (q0 + tok) * a.q_st +
-                     static_cast<int64_t>(g * a.group + r - tok * a.group) * a.q_sh;
+                     static_cast<int64_t>(g * a.group + hw * heads_group + r - tok * heads_group) * a.q_sh;
 #pragma unroll
       for (int st = 0; st < kSteps; ++st) {
         u32x4 w = {0u, 0u, 0u, 0u};
@@ -425,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
       return static_cast<uint32_t>(bits);
     };
     if (lane < kGroupRows) {
-      const int tok = min(row0 + lane, rows - 1) / a.group;
+      const int tok = min(row0 + lane, head_rows - 1) / heads_group;
       s_tok[wave][lane] = tok;
       s_start[wave][lane] = start_of(tok);
 #pragma unroll
@@ -437,16 +456,16 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     uint32_t k_at[kSteps / 2], v_at[kDTiles];
     const int vi = col >> 1, vr = 4 * quad + (vi & 3) + 16 * (vi >> 2);
 #pragma unroll
-    for (int h = 0; h < kSteps / 2; ++h) k_at[h] = col * D + 16 * ((4 * h + quad) ^ swz_k<D>(col));
+    for (int h = 0; h < kSteps / 2; ++h) k_at[h] = col * W + 16 * ((hw * (D / 16) + 4 * h + quad) ^ swz_k<W>(col));
 #pragma unroll
-    for (int dt = 0; dt < kDTiles; ++dt) v_at[dt] = vr * D + 16 * (dt ^ swz_v<D>(vr)) + 8 * (col & 1);
+    for (int dt = 0; dt < kDTiles; ++dt) v_at[dt] = vr * W + 16 * ((hw * kDTiles + dt) ^ swz_v<W>(vr)) + 8 * (col & 1);
     // products of the 32 keys of a part: S^T[16 j + 4 quad + i][row 16 s + col]
-    auto codes_of = [&](const CodeTile<D>& t, int kk, u32x4 (&k)[2][kSteps / 2]) KV8_INLINE {
+    auto codes_of = [&](const CodeTile<W>& t, int kk, u32x4 (&k)[2][kSteps / 2]) KV8_INLINE {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int h = 0; h < kSteps / 2; ++h)
-          k[j][h] = *reinterpret_cast<const u32x4*>(t.k + (32 * kk + 16 * j) * D + k_at[h]);
+          k[j][h] = *reinterpret_cast<const u32x4*>(t.k + (32 * kk + 16 * j) * W + k_at[h]);
     };
     auto scores = [&](const u32x4 (&k)[2][kSteps / 2], f32x4 (&sc)[2][SUB]) KV8_INLINE {
 #pragma unroll
@@ -465,14 +484,21 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
       }
     };
     // codes V[key][16 dt + col] of keys 4 quad + i (i < 4) of the part, then 16 keys on
-    auto v_tile = [&](const CodeTile<D>& t, int kk, int dt) KV8_INLINE -> u32x2 {
-      return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(t.v + 32 * kk * D + v_at[dt])));
+    auto v_tile = [&](const CodeTile<W>& t, int kk, int dt) KV8_INLINE -> u32x2 {
+      return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(t.v + 32 * kk * W + v_at[dt])));
     };
     // a part's a_j (which 0) or c_j (1) of keys 4 quad + i, and 16 keys on
     auto scales_of = [&](int it, int which, int kk, f32x4 (&x)[2]) KV8_INLINE {
-      const float* from = s_scale[it % kBuffers][32 * kk / kWaveKeys][which] + 32 * kk % kWaveKeys + 4 * quad;
-      x[0] = *reinterpret_cast<const f32x4*>(from);
-      x[1] = *reinterpret_cast<const f32x4*>(from + 16);
+      const float* from = s_scale[it % kBuffers][32 * kk / kWaveKeys][which] + (32 * kk % kWaveKeys + 4 * quad) * HEADS;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if constexpr (HEADS == 1) {
+          x[j] = *reinterpret_cast<const f32x4*>(from + 16 * j);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[j][i] = from[(16 * j + i) * HEADS + hw];
+        }
+      }
     };
     struct Weights {
       b8 hi, lo;
@@ -499,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     };
     // 32 keys that every row sees, when every row has a maximum; false, with
     // nothing done, where a sum outgrows kHuge
-    auto quick = [&](const CodeTile<D>& t, int it, int kk) KV8_INLINE -> bool {
+    auto quick = [&](const CodeTile<W>& t, int it, int kk) KV8_INLINE -> bool {
       f32x4 sc[2][SUB], ks[2], vs[2];
       u32x4 k[2][kSteps / 2];
       u32x2 v[kDTiles];
@@ -540,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
       return true;
     };
     // any 32 keys; v0: the first one's number
-    auto part = [&](const CodeTile<D>& t, int it, int kk, int v0, uint32_t dead) KV8_INLINE {
+    auto part = [&](const CodeTile<W>& t, int it, int kk, int v0, uint32_t dead) KV8_INLINE {
       f32x4 sc[2][SUB], ks[2], vs[2];
       scales_of(it, 0, kk, ks);
       scales_of(it, 1, kk, vs);
@@ -641,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     if (tiles > 0) stage(0);
     arrive();
     // keys that all of the wave's rows are late enough for
-    const int sure = a.mask ? old : old + uniform(min(row0, rows - 1) / a.group) + 1;
+    const int sure = a.mask ? old : old + uniform(min(row0, head_rows - 1) / heads_group) + 1;
     // this wave's parts of a tile
     uint32_t parts = 0;
 #pragma unroll
@@ -650,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     for (int it = 0; it < tiles; ++it) {
       // into the place that was last read before the barrier
       if (it + 1 < tiles) stage(it + 1);
-      const CodeTile<D>& t = buffers[it % kBuffers];
+      const CodeTile<W>& t = buffers[it % kBuffers];
       const int t0 = begin + it * kKeys;
       const uint32_t* dead = s_dead[it % (2 * kEntryTiles)];
       // the parts that all of the wave's rows see: behind their windows' starts or in the
@@ -699,7 +725,17 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
       }
     }
     __syncthreads();
-    const int here = min(rows - rb * R, groups * kGroupRows);
+    const int here = HEADS == 1 ? min(rows - rb * R, groups * kGroupRows) : min(rows - rb * R, R);
+    // where row i of the block is: the first of its waves, a row of theirs
+    struct Spot {
+      int wave, in;
+    };
+    auto spot_of = [&](int i) KV8_INLINE -> Spot {
+      if constexpr (HEADS == 1) return Spot{i / kGroupRows, i % kGroupRows};
+      const int tok = i / a.group, in = i - tok * a.group, second = in >= heads_group;
+      const int r = tok * heads_group + in - (second ? heads_group : 0);
+      return Spot{second * kHeadWaves + r / kGroupRows, r % kGroupRows};
+    };
     // an unfinished piece: a stretch has at most one that continues an earlier
     // stretch's, and one that the next continues
     const int64_t place = 2 * group_id + (first ? 1 : 0);
@@ -711,12 +747,13 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     if (mine < here) {
       const int r = rb * R + mine, token = r / a.group, head = g * a.group + r - token * a.group;
       const int64_t row = q0 + token;
-      const int group = mine / kGroupRows, in = mine % kGroupRows;
+      const auto [w0, in] = spot_of(mine);
+      const int w1 = w0 / kHeadWaves * kHeadWaves + kHeadWaves;
       float m = -INFINITY, lt = 0.f;
-      for (int w = group; w < kWaves; w += groups) m = fmaxf(m, s_m[w][in]);
+      for (int w = w0; w < w1; w += groups) m = fmaxf(m, s_m[w][in]);
       // a wave that has seen no key carries m = -inf, l = 0 and O = 0
       float base = m == -INFINITY ? 0.f : m;
-      for (int w = group; w < kWaves; w += groups) lt += s_l[w][in] * __builtin_amdgcn_exp2f(s_m[w][in] - base);
+      for (int w = w0; w < w1; w += groups) lt += s_l[w][in] * __builtin_amdgcn_exp2f(s_m[w][in] - base);
       float scale = 1.f;
       if (first && last) {
         if (a.sinks) {
@@ -730,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
         *reinterpret_cast<f32x2*>(part_ml + 2 * mine) = f32x2{m, lt};
       }
       scale *= inverse(lt);
-      for (int w = group; w < kWaves; w += groups) s_m[w][in] = __builtin_amdgcn_exp2f(s_m[w][in] - base) * scale;
+      for (int w = w0; w < w1; w += groups) s_m[w][in] = __builtin_amdgcn_exp2f(s_m[w][in] - base) * scale;
       if (!a.whole) {
         int32_t* owner = a.owner + 4 * (row * a.q_heads + head);
         if (first) {
@@ -746,9 +783,10 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     if (d < a.head_dim) {
 #pragma unroll 2
       for (int r = mine / (D / 4); r < here; r += kRowsAtOnce) {
-        const int group = r / kGroupRows, in = r % kGroupRows;
+        const auto [w0, in] = spot_of(r);
+        const int w1 = w0 / kHeadWaves * kHeadWaves + kHeadWaves;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int w = group; w < kWaves; w += groups)
+        for (int w = w0; w < w1; w += groups)
           o += *reinterpret_cast<const f32x4*>(result_of(w) + in * D + (d ^ (in & 7) << 2)) * s_m[w][in];
         if (first && last)
           store_four<T>(a, s_out[r] + d, o);
@@ -796,9 +834,9 @@ int subtiles_for(int d, int64_t rows) {
 }
 
 struct Launch {
-  int d, sub;
+  int d, sub, heads;
   bool whole;
-  int32_t row_blocks;
+  int32_t row_blocks, block_rows;
 };
 
 constexpr int64_t kWholeKeys = 512, kFullKeys = 1024, kFullGroups = 128;
@@ -814,6 +852,9 @@ Launch plan(int64_t n_tokens, int64_t n_requests, int64_t q_heads, int64_t kv_he
   // (further blocks of rows follow in the same workgroup)
   const int64_t room = std::max<int64_t>(1, kMostBlocks / std::max<int64_t>(1, n_requests * kv_heads));
   p.row_blocks = static_cast<int32_t>(std::min(blocks(), std::min<int64_t>(room, 4096)));
+  const int64_t group = q_heads / kv_heads, head_rows = 16 * kWaves / 2 * p.sub;
+  p.heads = !p.whole && p.d == 64 && kv_heads % 2 == 0 && rows <= head_rows ? 2 : 1;
+  p.block_rows = static_cast<int32_t>(p.heads == 2 ? head_rows / group * 2 * group : 16 * kWaves * p.sub);
   return p;
 }
 
@@ -835,20 +876,25 @@ template <typename T, bool E5>
 int launch(const Kv8Args& a, const Launch& p, hipStream_t st) {
   const int64_t blocks = p.whole ? static_cast<int64_t>(a.t.n_requests) * a.t.kv_heads * a.t.row_blocks : kGroups;
   const dim3 grid(static_cast<unsigned>(blocks)), threads(kThreads);
-  if (p.d == 64) {
-    if (p.sub == 1) hipLaunchKernelGGL((kv8_attention_kernel<T, E5, 64, 1>), grid, threads, 0, st, a);
-    else if (p.sub == 2) hipLaunchKernelGGL((kv8_attention_kernel<T, E5, 64, 2>), grid, threads, 0, st, a);
-    else hipLaunchKernelGGL((kv8_attention_kernel<T, E5, 64, 4>), grid, threads, 0, st, a);
+  auto start = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, threads, 0, st, a); };
+  if (p.heads == 2) {
+    if (p.sub == 1) start(kv8_attention_kernel<T, E5, 64, 1, 2>);
+    else if (p.sub == 2) start(kv8_attention_kernel<T, E5, 64, 2, 2>);
+    else start(kv8_attention_kernel<T, E5, 64, 4, 2>);
+  } else if (p.d == 64) {
+    if (p.sub == 1) start(kv8_attention_kernel<T, E5, 64, 1, 1>);
+    else if (p.sub == 2) start(kv8_attention_kernel<T, E5, 64, 2, 1>);
+    else start(kv8_attention_kernel<T, E5, 64, 4, 1>);
   } else {
-    if (p.sub == 1) hipLaunchKernelGGL((kv8_attention_kernel<T, E5, 128, 1>), grid, threads, 0, st, a);
-    else hipLaunchKernelGGL((kv8_attention_kernel<T, E5, 128, 2>), grid, threads, 0, st, a);
+    if (p.sub == 1) start(kv8_attention_kernel<T, E5, 128, 1, 1>);
+    else start(kv8_attention_kernel<T, E5, 128, 2, 1>);
   }
   int rc = check_launch("akv_kv8_attention");
   if (rc || p.whole) return rc;
   if (p.d == 64)
-    merge<T, 64>(a.t, 16 * kWaves * p.sub, st);
+    merge<T, 64>(a.t, p.block_rows, st);
   else
-    merge<T, 128>(a.t, 16 * kWaves * p.sub, st);
+    merge<T, 128>(a.t, p.block_rows, st);
   return check_launch("akv_kv8_attention (combine)");
 }
 
@@ -949,13 +995,13 @@ extern "C" int akv_kv8_attention(const void* q, int64_t q_stride_t, int64_t q_st
   a.t.o_sh = out_stride_h;
   a.t.owner = static_cast<int32_t*>(workspace);
   a.t.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + owner_bytes(n_tokens, q_heads));
-  a.t.part_ml = a.t.part_o + 2ll * kGroups * (16 * kWaves * p.sub) * p.d;
+  a.t.part_ml = a.t.part_o + 2ll * kGroups * p.block_rows * p.d;
   a.t.n_tokens = n_tokens;
   a.t.max_len = max_len;
   a.t.n_requests = n_requests;
   a.t.q_heads = q_heads;
-  a.t.kv_heads = kv_heads;
-  a.t.group = q_heads / kv_heads;
+  a.t.kv_heads = kv_heads / p.heads;
+  a.t.group = q_heads / kv_heads * p.heads;
   a.t.head_dim = head_dim;
   a.t.page_size = page_size;
   a.t.row_blocks = p.row_blocks;
@@ -973,6 +1019,7 @@ extern "C" int akv_kv8_attention(const void* q, int64_t q_stride_t, int64_t q_st
   a.vs_sh = vs_stride_head;
   a.log2_block = __builtin_ctz(static_cast<uint32_t>(scale_block));
   a.first_keys = first_keys;
+  a.block_rows = p.block_rows;
   hipStream_t st = as_stream(stream);
   if (dtype == AKV_F16) return format == AKV_E5M2 ? launch<_Float16, true>(a, p, st) : launch<_Float16, false>(a, p, st);
   return format == AKV_E5M2 ? launch<__bf16, true>(a, p, st) : launch<__bf16, false>(a, p, st);
