@@ -35,6 +35,10 @@
 // of the 8-byte rows read by lanes j/8 + 2i, i < 8.
 #include "tree_common.h"
 
+#ifndef WA
+#define WA 2
+#define WB 3
+#endif
 namespace akv {
 namespace {
 
@@ -126,7 +130,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
   constexpr int kLoadRows = 64 / kChunks;      // rows of one wave-wide load
   constexpr int kWaveKeys = kKeys / kWaves;    // keys of a tile that a wave asks for
   constexpr int kEntryTiles = 64 / kWaveKeys;  // tiles whose keys of this wave fill a vector register
-  constexpr int kOver = (kPieceCost + kKeys - 1) / kKeys;
+  constexpr int kHeadWaves = kWaves / HEADS;   // waves of a head
+  constexpr int kOver = 2 * ((kPieceCost + kKeys - 1) / kKeys);
   constexpr int kGroupRows = 16 * SUB;         // rows of a wave
   const int R = HEADS == 1 ? kWaves * kGroupRows : ka.block_rows;  // rows of a block
   __shared__ CodeTile<W> buffers[kBuffers];
@@ -152,13 +157,22 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     const int64_t tokens = ((rb + 1) * static_cast<int64_t>(R) + a.group - 1) / a.group;
     return a.mask || tokens >= n || n > len ? len : len - n + tokens;
   };
-  // One wave's view of the batch.  A request costs its tiles and kOver for every
-  // block of rows; block rb's cost is 0 where the request has no such rows.
+  // groups of rows that a head's `left` rows from a block's first on make
+  auto groups_of = [&](int left) -> int {
+    int groups = kHeadWaves;
+    while (groups > 1 && kHeadWaves / groups < kParts && left <= (groups >> 1) * kGroupRows) groups >>= 1;
+    return groups;
+  };
+  // One wave's view of the batch.  A request costs its tiles, by what the waves have to do
+  // there, and kOver for every block of rows; block rb's cost is 0 where it has no such rows.
   auto units_of = [&](int64_t len, int32_t n, int rb) -> int32_t {
     len = reach(len, n, rb);
     if (a.key_starts && len > a.max_len) len = a.max_len;  // what a window reaches is not known here
     const int64_t tiles = len > kKeys ? (len + kKeys - 1) / kKeys : 1;
-    return static_cast<int64_t>(rb) * R < static_cast<int64_t>(n) * a.group ? static_cast<int32_t>(tiles + kOver) : 0;
+    const int64_t left = static_cast<int64_t>(n) * a.group - static_cast<int64_t>(rb) * R;
+    if (left <= 0) return 0;
+    const int groups = groups_of(static_cast<int>(std::min<int64_t>(left, R)) / HEADS);
+    return static_cast<int32_t>(tiles * (groups == 1 ? WA : groups == 2 ? WB : 4)) + kOver;
   };
   struct Cost {
     int32_t units, rows;
@@ -203,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     if (all == 0) return;
     // 2^k stretches: all of the workgroups, or as many as get their least share
     int k = kGroupsShift;
-    while (k > 0 && (static_cast<int64_t>((kLeastShare + kKeys - 1) / kKeys) << k) > all) --k;
+    while (k > 0 && (static_cast<int64_t>(2 * ((kLeastShare + kKeys - 1) / kKeys)) << k) > all) --k;
     if (group_id >> k) return;
     auto cut = [&](int64_t i) { return (all >> k) * i + (((all & ((1 << k) - 1)) * i) >> k); };  // all * i / 2^k
     int64_t x = cut(group_id);
@@ -376,14 +390,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     };
     if (tiles > 0) fetch(0);
     // a head's groups of rows, and the waves that share one
-    constexpr int kHeadWaves = kWaves / HEADS;
     const int heads_group = a.group / HEADS, head_rows = n * heads_group, block_row0 = rb * (R / HEADS);
     const int hw = wave / kHeadWaves;  // the wave's head
-    int groups = kHeadWaves, sharers = 1;
-    while (groups > 1 && sharers < kParts && head_rows - block_row0 <= (groups >> 1) * kGroupRows) {
-      groups >>= 1;
-      sharers <<= 1;
-    }
+    const int groups = groups_of(min(head_rows - block_row0, R / HEADS)), sharers = kHeadWaves / groups;
     const int row0 = block_row0 + (wave & (groups - 1)) * kGroupRows;
     const int share = uniform(wave % kHeadWaves / groups);
     // this lane's rows of the head: r = row0 + 16 s + col, token r / G, q head r % G of its G
