@@ -43,12 +43,13 @@ enum Fate : int32_t { kTurned, kAtItsPlace, kUnknown, kLeft };
 //
 // Bound by HBM: 19.9k scattered tokens of 36 layers, 8 heads of 64: 1.57 GB in 381 us, 4.1
 // TB/s; 16.4k of 32 layers, 8 heads of 128, in blocks and pages of 16: 2.17 GB in 483 us, 4.5 TB/s
-// (a copy: 5.16).  The arithmetic hides behind it (without any of it 441 and 532 us in an
+// (a copy: 5.16).  In blocks of 32 and 64, a wave's rounds held as codes and decoded three times,
+// 649 and 739 us (with the values kept in registers, a wave a SIMD, 1530 and 973).  The arithmetic hides behind it (without any of it 441 and 532 us in an
 // earlier order).  What is missing in the first are the scales: 32 bytes a token and
 // layer, alone in their lines; with none of them stored a raw copy of these rows takes 307 us,
 // with them 460.
 template <bool E5, int LANES, int ITERS, bool SINGLE, bool VEC>
-__global__ void __launch_bounds__(kThreads, ITERS <= 2 && !SINGLE ? 3 : 1) kv8_move_kernel(const MoveArgs a) {
+__global__ void __launch_bounds__(kThreads, SINGLE ? 1 : ITERS <= 2 ? 3 : 2) kv8_move_kernel(const MoveArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int kRows = 64 / LANES;
@@ -257,6 +258,11 @@ __global__ void __launch_bounds__(kThreads, ITERS <= 2 && !SINGLE ? 3 : 1) kv8_m
           entry[it] = x.entry[it];
         }
         auto decode = [&](int it, float (&y)[16]) KV8_INLINE {
+          if constexpr (kHeld < ITERS) {
+            // (as if unknown: the values of a round are not kept from the first time)
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" : "+v"(x.lo[it]), "+v"(x.hi[it]));
+          }
           decode8<E5>(x.lo[it], y);
           decode8<E5>(x.hi[it], y + 8);
         };
@@ -388,7 +394,9 @@ extern "C" int akv_kv8_reposition(const uint64_t* k_ptrs, const uint64_t* v_ptrs
     if (single) hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, 1, true, kVec>), grid, threads, lds, st, a);
     else if (rounds == 1) hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, 1, false, kVec>), grid, threads, lds, st, a);
     else if (rounds == 2) hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, 2, false, kVec>), grid, threads, lds, st, a);
-    else hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, kLanes, false, kVec>), grid, threads, lds, st, a);
+    else if (rounds == 4) hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, 4, false, kVec>), grid, threads, lds, st, a);
+    else if constexpr (kLanes == 8)
+      hipLaunchKernelGGL((kv8_move_kernel<kE5, 8, 8, false, kVec>), grid, threads, lds, st, a);
   };
   auto by_lanes = [&](auto e5, auto by_chunk) {
     if (lanes == 4) start(e5, Number<4>{}, by_chunk);
