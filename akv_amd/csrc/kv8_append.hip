@@ -1,4 +1,19 @@
 // New rows into a cache held in 8 bits, K (and q) rotated on the way (gfx950).
+//
+// K's row x at position p becomes, pair by pair, (x c - y s, y c + x s) with the p-th row
+// (c, s) of the table, in fp32 from its load on; its codes and scales, and V's, are
+// those of kv8_rows.h.  q's rows take the same turn and one rounding, in the same launch.
+//
+// A wave takes a block's tokens of one head (or of several, blocks being small), rows
+// being the K heads, then the V heads; a run of tokens belongs to the wave whose
+// window holds the run's first entry.  q rows go 64 / LANES heads to a wave, with the
+// token's table row read once: all of a token's heads in one wave from 2048 tokens
+// on, else a wave for each lot of heads, for latency.
+//
+// Bound by HBM from thousands of tokens on, by the launch below: 32768 tokens of 64 q heads and 8
+// KV heads of 64, 647 MB in 143 us, 4.5 TB/s (a copy: 5.16); one token 4.5 us, 64 4.9.  Rotations
+// of an odd number of eights, whose halves end inside a chunk, load and store quads instead
+// (80 dims of which 40 turn: 284 us; element by element 1239; with all 80 turned 196).
 #include "kv8_rows.h"
 
 namespace akv {
@@ -25,9 +40,7 @@ struct AppendArgs {
   bool slots64, pos64;
 };
 
-// VEC: whole chunks of 8, pairs of the rotation within a lane; else element by
-// element.
-template <typename T, bool E5, int LANES, int ITERS, bool VEC>
+template <typename T, bool E5, int LANES, int ITERS, int MODE>
 __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendArgs a) {
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Rope& rope = a.rope;
@@ -36,9 +49,9 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendArgs a
     return p >= 0 && p < rope.rows ? p : -1;
   };
   // cos and sin of a lane's eight pairs
-  auto coefficients = [&](int64_t p, int u, float (&c)[8], float (&s)[8]) KV8_INLINE {
-    load8(rope.table, rope.dtype, p * rope.stride + 8 * u, c);
-    load8(rope.table, rope.dtype, p * rope.stride + rope.dim / 2 + 8 * u, s);
+  auto coefficients = [&](int64_t p, int u, bool all, float (&c)[8], float (&s)[8]) KV8_INLINE {
+    load8<MODE == kByQuad>(rope.table, rope.dtype, p * rope.stride + 8 * u, c, all ? 4 : 0);
+    load8<MODE == kByQuad>(rope.table, rope.dtype, p * rope.stride + rope.dim / 2 + 8 * u, s, all ? 4 : 0);
   };
   // part u of a row, element by element; rotates: by the row p of the table
   auto by_element = [&](const T* from, int u, bool rotates, int64_t p, float (&y)[16]) KV8_INLINE {
@@ -59,8 +72,13 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendArgs a
   };
   auto part = [&](const T* from, Place place, float (&y)[16]) KV8_INLINE {
     Chunk<T> x0, x1;
-    x0.load(from + place.at0);
-    x1.load(from + place.at1);
+    if constexpr (MODE == kByQuad) {
+      x0.load_quads(from + place.at0, place.mid0);
+      x1.load_quads(from + place.at1, place.mid1);
+    } else {
+      x0.load(from + place.at0);
+      x1.load(from + place.at1);
+    }
     float (&lo)[8] = *reinterpret_cast<float (*)[8]>(y), (&hi)[8] = *reinterpret_cast<float (*)[8]>(y + 8);
     x0.get(lo);
     x1.get(hi);
@@ -73,16 +91,16 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendArgs a
     const int64_t t = mine / a.q_parts;
     const int first = static_cast<int>(mine - t * a.q_parts);
     const int u = threadIdx.x % LANES, sub = (threadIdx.x & 63) / LANES;
-    const Place place = place_of<VEC>(u, true, rope);
+    const Place place = place_of<MODE>(u, true, rope);
     const int64_t p = position(t);
     float c[8], s[8];
-    if (place.turned && p >= 0) coefficients(p, u, c, s);
+    if (place.turned && p >= 0) coefficients(p, u, place.all, c, s);
     for (int head = first * (64 / LANES) + sub; head < a.q_heads; head += static_cast<int>(a.q_parts) * (64 / LANES)) {
       if (16 * u >= a.c.head_dim) break;
       const T* from = static_cast<const T*>(a.q) + t * a.q_st + head * a.q_sh;
       T* to = static_cast<T*>(a.q_out) + t * a.qo_st + head * a.qo_sh;
       float y[16];
-      if constexpr (!VEC) {
+      if constexpr (MODE == kByElement) {
         // (q_out may be q: all of a row is read before any of it is written)
         by_element(from, u, true, p, y);
         __builtin_amdgcn_wave_barrier();
@@ -90,7 +108,7 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendArgs a
         for (int e = 0; e < 16; ++e) to[16 * u + e] = static_cast<T>(p < 0 ? nan32() : y[e]);
       } else {
         part(from, place, y);
-        if (place.turned && p >= 0) turn_either(y, c, s, rope.neox);
+        if (place.turned && p >= 0) turn_place<MODE>(y, c, s, rope.neox, place.all);
         if (p < 0) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) y[e] = nan32();
@@ -98,8 +116,13 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendArgs a
         Chunk<T> x0, x1;
         x0.set(*reinterpret_cast<float (*)[8]>(y));
         x1.set(*reinterpret_cast<float (*)[8]>(y + 8));
-        x0.store(to + place.at0);
-        x1.store(to + place.at1);
+        if constexpr (MODE == kByQuad) {
+          x0.store_quads(to + place.at0, place.mid0);
+          x1.store_quads(to + place.at1, place.mid1);
+        } else {
+          x0.store(to + place.at0);
+          x1.store(to + place.at1);
+        }
       }
     }
     return;
@@ -112,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendArgs a
   const bool is_v = row >= a.c.heads;
   const int head = is_v ? row - a.c.heads : row;
   const bool rotates = !is_v && rope.dim > 0;
-  const Place place = place_of<VEC>(at.u, rotates, rope);
+  const Place place = place_of<MODE>(at.u, rotates, rope);
   const T* rows = is_v ? static_cast<const T*>(a.v) + head * a.v_sh : static_cast<const T*>(a.k) + head * a.k_sh;
   const int64_t row_stride = is_v ? a.v_st : a.k_st;
   uint8_t* pool = is_v ? a.v_pool + head * a.c.v_sh : a.k_pool + head * a.c.k_sh;
@@ -132,19 +155,19 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendArgs a
       int64_t off[ITERS ? ITERS : 1];
 #pragma unroll
       for (int it = 0; it < (ITERS ? ITERS : 1); ++it) off[it] = (first + it * at.rows + at.r) * slot_stride + place.at0;
-      write_run<E5, LANES, ITERS, false>(
+      write_run<E5, LANES, ITERS, MODE, false>(
           at, in, run.len, first, pool + (block << a.c.log2_block) * slot_stride, slot_stride, off,
-          place.at1 - place.at0, scales + block * block_stride, [&](int, int i, float (&y)[16], float&) KV8_INLINE {
+          place, scales + block * block_stride, [&](int, int i, float (&y)[16], float&) KV8_INLINE {
             const T* from = rows + (t + i) * row_stride;
             const int64_t p = rotates ? position(t + i) : 0;
-            if constexpr (!VEC) {
+            if constexpr (MODE == kByElement) {
               by_element(from, at.u, rotates, p, y);
             } else {
               part(from, place, y);
               if (place.turned && p >= 0) {
                 float c[8], s[8];
-                coefficients(p, at.u, c, s);
-                turn_either(y, c, s, rope.neox);
+                coefficients(p, at.u, place.all, c, s);
+                turn_place<MODE>(y, c, s, rope.neox, place.all);
               }
             }
             if (p < 0) {
@@ -172,14 +195,16 @@ Shape shape_of(const Cache& c) {
   return s;
 }
 
-// Calls f with the kernel's LANES, ITERS and VEC as constants.
+// Calls f with the kernel's LANES, ITERS and MODE as constants.
 template <typename F>
-void with_shape(const Shape& s, bool vec, F f) {
+void with_shape(const Shape& s, Mode mode, F f) {
   auto of_lanes = [&](auto lanes) {
-    if (!vec) f(lanes, Number<0>{}, Number<0>{});
-    else if (s.iters == 1) f(lanes, Number<1>{}, Number<1>{});
-    else if (s.iters == 2) f(lanes, Number<2>{}, Number<1>{});
-    else f(lanes, Number<0>{}, Number<1>{});
+    if (mode == kByElement) f(lanes, Number<0>{}, Number<kByElement>{});
+    else if (mode == kByQuad && s.iters == 1) f(lanes, Number<1>{}, Number<kByQuad>{});
+    else if (mode == kByQuad) f(lanes, Number<0>{}, Number<kByQuad>{});
+    else if (s.iters == 1) f(lanes, Number<1>{}, Number<kByChunk>{});
+    else if (s.iters == 2) f(lanes, Number<2>{}, Number<kByChunk>{});
+    else f(lanes, Number<0>{}, Number<kByChunk>{});
   };
   if (s.lanes == 4) of_lanes(Number<4>{});
   else of_lanes(Number<8>{});
@@ -243,16 +268,18 @@ extern "C" int akv_kv8_append(const void* q, int64_t q_stride_t, int64_t q_strid
   a.q_heads = q_heads;
   a.slots64 = slots_dtype == AKV_I64;
   a.pos64 = positions_dtype == AKV_I64;
-  // whole chunks of 8 on 16-byte boundaries, pairs within a lane
+  // whole chunks on 16-byte boundaries, pairs within a lane
   const int e = dtype == AKV_F32 ? 4 : 2, te = cos_sin_dtype == AKV_F32 ? 4 : 2;
   const bool vec =
-      rotary_dim % 16 == 0 && aligned(k, 16) && aligned(v, 16) &&
+      rotary_dim % 8 == 0 && aligned(k, 16) && aligned(v, 16) &&
           ((k_stride_t | k_stride_h | v_stride_t | v_stride_h) * e) % 16 == 0 &&
           (!rotary_dim || (aligned(cos_sin, 16) && rope_stride * te % 16 == 0)) &&
           (!q_heads || (aligned(q, 16) && aligned(q_out, 16) &&
                         ((q_stride_t | q_stride_h | qo_stride_t | qo_stride_h) * e) % 16 == 0));
+  const Mode mode = !vec ? kByElement : rotary_dim % 16 ? kByQuad : kByChunk;
   const Shape shape = shape_of(a.c);
   a.head_groups = shape.groups;
+  // entries of a wave: one as long as the waves are few, so that no run waits behind another
   a.window = 1;
   while (a.window < scale_block && n_tokens * shape.groups > 16384ll * a.window) a.window *= 2;
   a.kv_units = pool_slots ? (n_tokens + a.window - 1) / a.window * shape.groups : 0;
@@ -265,9 +292,9 @@ extern "C" int akv_kv8_append(const void* q, int64_t q_stride_t, int64_t q_strid
   hipStream_t st = as_stream(stream);
   auto start = [&](auto type, auto e5) {
     using T = decltype(type);
-    with_shape(shape, vec, [&](auto lanes, auto iters, auto by_chunk) {
+    with_shape(shape, mode, [&](auto lanes, auto iters, auto m) {
       hipLaunchKernelGGL((kv8_append_kernel<T, decltype(e5)::value != 0, decltype(lanes)::value, decltype(iters)::value,
-                                            decltype(by_chunk)::value != 0>),
+                                            decltype(m)::value>),
                          dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, a);
     });
   };

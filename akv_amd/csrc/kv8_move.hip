@@ -48,7 +48,7 @@ enum Fate : int32_t { kTurned, kAtItsPlace, kUnknown, kLeft };
 // earlier order).  What is missing in the first are the scales: 32 bytes a token and
 // layer, alone in their lines; with none of them stored a raw copy of these rows takes 307 us,
 // with them 460.
-template <bool E5, int LANES, int ITERS, bool SINGLE, bool VEC>
+template <bool E5, int LANES, int ITERS, bool SINGLE, int MODE>
 __global__ void __launch_bounds__(kThreads, SINGLE ? 1 : ITERS <= 2 ? 3 : 2) kv8_move_kernel(const MoveArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kThreads, SINGLE ? 1 : ITERS <= 2 ? 3 : 2) kv8
       s_factor[most_factors + i] = (sn * co - cn * so) / norm;
     }
     const bool some_at_place = __syncthreads_or(at_place);
-    const bool fast = __syncthreads_and(VEC && plain);
+    const bool fast = __syncthreads_and(MODE != kByElement && plain);
 
     // lots of rows: K's, then V's; a wave takes every fourth
     const int lots = SINGLE ? (len * heads + kRows - 1) / kRows : (heads + a.heads_at_once - 1) / a.heads_at_once;
@@ -138,34 +138,37 @@ __global__ void __launch_bounds__(kThreads, SINGLE ? 1 : ITERS <= 2 ? 3 : 2) kv8
             in = in_row && entry0 < len;
             to_block = in ? s_dst[1 + e0 + entry0] : -1;
           }
-          const Place place = place_of<VEC>(at.u, !is_v, rope);
+          const Place place = place_of<MODE>(at.u, !is_v, rope);
           const int64_t slot_stride = is_v ? a.c.v_ss : a.c.k_ss, head_at = head * (is_v ? a.c.v_sh : a.c.k_sh);
           const int64_t scale_stride = is_v ? a.c.vs_sb : a.c.ks_sb, scale_at = head * (is_v ? a.c.vs_sh : a.c.ks_sh);
           uint8_t* codes = reinterpret_cast<uint8_t*>(lane_value(is_v ? my_v : my_k, l)) + head_at;
           float* scales = reinterpret_cast<float*>(lane_value(is_v ? my_vs : my_ks, l)) + scale_at;
           const int64_t off = (first + at.r) * slot_stride + place.at0;
-          write_run<E5, LANES, 0, true>(
+          write_run<E5, LANES, 0, MODE, true>(
               at, in && to_block >= 0, SINGLE ? 1 : len, first, codes + (to_block << a.c.log2_block) * slot_stride,
-              slot_stride, &off, place.at1 - place.at0, scales + to_block * scale_stride,
+              slot_stride, &off, place, scales + to_block * scale_stride,
               [&](int, int i, float (&z)[16], float& by) KV8_INLINE {
                 const int entry = entry0 + i, fate = s_fate[entry];
                 if (fate == kLeft) return false;
                 const int64_t src = s_src[e0 + entry];
                 const uint8_t* from = codes + src * slot_stride;
                 by = load_scale(scales + (src >> a.c.log2_block) * scale_stride);
-                decode8<E5>(load_codes(from + place.at0), z);
-                decode8<E5>(load_codes(from + place.at1), z + 8);
+                decode8<E5>(load_chunk<MODE>(from + place.at0, place.mid0), z);
+                decode8<E5>(load_chunk<MODE>(from + place.at1, place.mid1), z + 8);
                 if (is_v || fate == kAtItsPlace) return true;
                 const float* f = s_factor + entry * half;
                 if (fate == kUnknown) {
 #pragma unroll
                   for (int e = 0; e < 16; ++e) z[e] = nan32();
-                } else if constexpr (VEC) {
+                } else if constexpr (MODE != kByElement) {
                   if (place.turned) {
                     float c[8], s[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) c[i] = f[8 * at.u + i], s[i] = f[most_factors + 8 * at.u + i];
-                    turn_either(z, c, s, rope.neox);
+                    for (int i = 0; i < 8; ++i) {
+                      const int pair = 8 * at.u + (MODE == kByChunk || i < 4 || place.all ? i : 0);
+                      c[i] = f[pair], s[i] = f[most_factors + pair];
+                    }
+                    turn_place<MODE>(z, c, s, rope.neox, place.all);
                   }
                 } else {
 #pragma unroll
@@ -186,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, SINGLE ? 1 : ITERS <= 2 ? 3 : 2) kv8
       }
     };
     bool done = false;
-    if constexpr (VEC) {
+    if constexpr (MODE != kByElement) {
       const int total = mine * layers;
       if (fast && total > 0) {
         done = true;
@@ -199,7 +202,8 @@ __global__ void __launch_bounds__(kThreads, SINGLE ? 1 : ITERS <= 2 ? 3 : 2) kv8
         float scale[ITERS];
         uint8_t* to[ITERS];
         float* to_scale;
-        int entry[ITERS], apart;
+        int entry[ITERS];
+        Place place;
         bool is_v;
       };
       int l = 0, n = wave;  // the next lot's
@@ -210,9 +214,10 @@ __global__ void __launch_bounds__(kThreads, SINGLE ? 1 : ITERS <= 2 ? 3 : 2) kv8
         float* scales = reinterpret_cast<float*>(lane_value(is_v ? my_vs : my_ks, l));
         const int64_t slot_stride = is_v ? a.c.v_ss : a.c.k_ss, head_stride = is_v ? a.c.v_sh : a.c.k_sh;
         const int64_t scale_stride = is_v ? a.c.vs_sb : a.c.ks_sb, scale_head = is_v ? a.c.vs_sh : a.c.ks_sh;
-        const Place place = place_of<VEC>(u, !is_v, rope);
+        const Place place = place_of<MODE>(u, !is_v, rope);
         x.is_v = is_v;
-        x.apart = place.at1 - place.at0;
+        x.place = place;
+        const int apart = place.at1 - place.at0;
 #pragma unroll
         for (int it = 0; it < ITERS; ++it) {
           int entry, head;
@@ -229,8 +234,8 @@ __global__ void __launch_bounds__(kThreads, SINGLE ? 1 : ITERS <= 2 ? 3 : 2) kv8
           const int64_t in_row = head * head_stride + place.at0;
           x.entry[it] = entry;
           x.scale[it] = load_scale(scales + (src >> a.c.log2_block) * scale_stride + head * scale_head);
-          x.lo[it] = load_codes(codes + src * slot_stride + in_row);
-          x.hi[it] = load_codes(codes + src * slot_stride + in_row + x.apart);
+          x.lo[it] = load_chunk<MODE>(codes + src * slot_stride + in_row, place.mid0);
+          x.hi[it] = load_chunk<MODE>(codes + src * slot_stride + in_row + apart, place.mid1);
           x.to[it] = codes + ((to_block << a.c.log2_block) + (SINGLE ? 0 : entry)) * slot_stride + in_row;
           x.to_scale = scales + to_block * scale_stride + head * scale_head;
         }
@@ -248,7 +253,8 @@ __global__ void __launch_bounds__(kThreads, SINGLE ? 1 : ITERS <= 2 ? 3 : 2) kv8
         float z[kHeld][16], unit_of[ITERS], top = 0.f;
         uint8_t* to[ITERS];
         float* to_scale = x.to_scale;
-        const int apart = x.apart;
+        const Place place = x.place;
+        const int apart = place.at1 - place.at0;
         const bool turns = !x.is_v && 16 * u < rope.dim;
         int entry[ITERS];
 #pragma unroll
@@ -271,8 +277,11 @@ __global__ void __launch_bounds__(kThreads, SINGLE ? 1 : ITERS <= 2 ? 3 : 2) kv8
           float c[8], s[8];
           const float* f = s_factor + entry[it] * half + 8 * u;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) c[i] = f[i], s[i] = f[most_factors + i];
-          turn_either(y, c, s, rope.neox);
+          for (int i = 0; i < 8; ++i) {
+            const int pair = MODE == kByChunk || i < 4 || place.all ? i : 0;
+            c[i] = f[pair], s[i] = f[most_factors + pair];
+          }
+          turn_place<MODE>(y, c, s, rope.neox, place.all);
         };
         if constexpr (kHeld == ITERS) {
 #pragma unroll
@@ -312,11 +321,18 @@ __global__ void __launch_bounds__(kThreads, SINGLE ? 1 : ITERS <= 2 ? 3 : 2) kv8
           if constexpr (SINGLE) {
             // past the caches: scattered rows' scales, 4 bytes a head, lie in lines that other
             // tokens' are read from and written to (380 us for 404; blocks of 16: 537 for 528)
-            __builtin_nontemporal_store(lo, (global_any_u32x2*)to[it]);
-            __builtin_nontemporal_store(hi, (global_any_u32x2*)(to[it] + apart));
+            if constexpr (MODE == kByQuad) {
+              const uint32_t words[4] = {lo[0], lo[1], hi[0], hi[1]};
+              const int ats[4] = {0, place.mid0, apart, apart + place.mid1};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) __builtin_nontemporal_store(words[i], (global_any_u32*)(to[it] + ats[i]));
+            } else {
+              __builtin_nontemporal_store(lo, (global_any_u32x2*)to[it]);
+              __builtin_nontemporal_store(hi, (global_any_u32x2*)(to[it] + apart));
+            }
           } else {
-            store_codes(to[it], lo);
-            store_codes(to[it] + apart, hi);
+            store_chunk<MODE>(to[it], place.mid0, lo);
+            store_chunk<MODE>(to[it] + apart, place.mid1, hi);
           }
         }
         store_scale(to_scale, scale);
@@ -374,7 +390,7 @@ extern "C" int akv_kv8_reposition(const uint64_t* k_ptrs, const uint64_t* v_ptrs
   a.n_layers = n_layers;
   a.skip_zero = skip_unmapped != 0;
   const int te = cos_sin_dtype == AKV_F32 ? 4 : 2;
-  const bool vec = rotary_dim % 16 == 0 && aligned(cos_sin, 16) && rope_stride * te % 16 == 0;
+  const bool vec = rotary_dim % 8 == 0 && aligned(cos_sin, 16) && rope_stride * te % 16 == 0;
   const int lanes = lanes_of(head_dim), rows = std::min(scale_block, 64 / lanes), rounds = scale_block / rows;
   const bool single = scale_block == 1;
   a.heads_at_once = std::min(64 / (lanes * rows), n_heads);
@@ -388,23 +404,25 @@ extern "C" int akv_kv8_reposition(const uint64_t* k_ptrs, const uint64_t* v_ptrs
   hipStream_t st = as_stream(stream);
   const dim3 threads(kThreads), grid(static_cast<unsigned>(blocks));
   const unsigned lds = static_cast<unsigned>(a.window) * rotary_dim * sizeof(float);
-  auto start = [&](auto e5, auto n, auto by_chunk) {
-    constexpr bool kE5 = decltype(e5)::value != 0, kVec = decltype(by_chunk)::value != 0;
-    constexpr int kLanes = decltype(n)::value;
-    if (single) hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, 1, true, kVec>), grid, threads, lds, st, a);
-    else if (rounds == 1) hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, 1, false, kVec>), grid, threads, lds, st, a);
-    else if (rounds == 2) hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, 2, false, kVec>), grid, threads, lds, st, a);
-    else if (rounds == 4) hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, 4, false, kVec>), grid, threads, lds, st, a);
+  auto start = [&](auto e5, auto n, auto mode) {
+    constexpr bool kE5 = decltype(e5)::value != 0;
+    constexpr int kLanes = decltype(n)::value, kMode = decltype(mode)::value;
+    if (single) hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, 1, true, kMode>), grid, threads, lds, st, a);
+    else if (rounds == 1 || kMode == kByElement) hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, 1, false, kMode>), grid, threads, lds, st, a);
+    else if constexpr (kMode == kByElement) return;
+    else if (rounds == 2) hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, 2, false, kMode>), grid, threads, lds, st, a);
+    else if (rounds == 4) hipLaunchKernelGGL((kv8_move_kernel<kE5, kLanes, 4, false, kMode>), grid, threads, lds, st, a);
     else if constexpr (kLanes == 8)
-      hipLaunchKernelGGL((kv8_move_kernel<kE5, 8, 8, false, kVec>), grid, threads, lds, st, a);
+      hipLaunchKernelGGL((kv8_move_kernel<kE5, 8, 8, false, kMode>), grid, threads, lds, st, a);
   };
-  auto by_lanes = [&](auto e5, auto by_chunk) {
-    if (lanes == 4) start(e5, Number<4>{}, by_chunk);
-    else start(e5, Number<8>{}, by_chunk);
+  auto by_lanes = [&](auto e5, auto mode) {
+    if (lanes == 4) start(e5, Number<4>{}, mode);
+    else start(e5, Number<8>{}, mode);
   };
   auto by_form = [&](auto e5) {
-    if (vec) by_lanes(e5, Number<1>{});
-    else by_lanes(e5, Number<0>{});
+    if (!vec) by_lanes(e5, Number<kByElement>{});
+    else if (rotary_dim % 16) by_lanes(e5, Number<kByQuad>{});
+    else by_lanes(e5, Number<kByChunk>{});
   };
   if (format == AKV_E5M2) by_form(Number<1>{});
   else by_form(Number<0>{});

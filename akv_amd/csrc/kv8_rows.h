@@ -36,7 +36,6 @@ constexpr uint32_t kLeastScale = (127 - 100) << 23;  // 2^-100
 // Workgroups of a launch: a grid has fewer than 2^32 threads.
 constexpr int64_t kMostBlocks = 1 << 23;
 
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // Strides in bytes (codes) and elements (scales).
@@ -113,13 +112,30 @@ __device__ __forceinline__ u32x2 encode8(const float* x) {
 typedef u32x2 any_u32x2 __attribute__((aligned(1)));
 typedef __attribute__((address_space(1))) any_u32x2 global_any_u32x2;
 
-typedef u32x4 any_u32x4 __attribute__((aligned(1)));
-typedef __attribute__((address_space(1))) any_u32x4 global_any_u32x4;
+typedef uint32_t any_u32 __attribute__((aligned(1)));
+typedef __attribute__((address_space(1))) any_u32 global_any_u32;
 
-__device__ __forceinline__ u32x4 load_codes16(const uint8_t* p) { return *((const global_any_u32x4*)p); }
-__device__ __forceinline__ void store_codes16(uint8_t* p, u32x4 w) { *((global_any_u32x4*)p) = w; }
 __device__ __forceinline__ u32x2 load_codes(const uint8_t* p) { return *((const global_any_u32x2*)p); }
 __device__ __forceinline__ void store_codes(uint8_t* p, u32x2 w) { *((global_any_u32x2*)p) = w; }
+
+// How a lane takes its 16 values of a row: element by element, in two chunks of
+// eight, or in two chunks of two quads (a rotation that ends inside a chunk).
+enum Mode { kByElement, kByChunk, kByQuad };
+
+template <int MODE>
+__device__ __forceinline__ u32x2 load_chunk(const uint8_t* p, int mid) {
+  if constexpr (MODE == kByQuad) return u32x2{*((const global_any_u32*)p), *((const global_any_u32*)(p + mid))};
+  return load_codes(p);
+}
+template <int MODE>
+__device__ __forceinline__ void store_chunk(uint8_t* p, int mid, u32x2 w) {
+  if constexpr (MODE == kByQuad) {
+    *((global_any_u32*)p) = w[0];
+    *((global_any_u32*)(p + mid)) = w[1];
+  } else {
+    store_codes(p, w);
+  }
+}
 
 // Scales by address: named as global, since flat accesses wait for everything.
 typedef __attribute__((address_space(1))) float global_float;
@@ -127,17 +143,25 @@ typedef __attribute__((address_space(1))) uint8_t global_byte;
 __device__ __forceinline__ float load_scale(const float* p) { return *((const global_float*)p); }
 __device__ __forceinline__ void store_scale(float* p, float s) { *((global_float*)p) = s; }
 
-// A lane's 16 values of a row, 8 from at0 and 8 from at1 on.
+// A lane's 16 values of a row: 8 from at0 and 8 from at1 on, each in two quads, the
+// second mid0 (mid1) elements behind the first.
 struct Place {
-  int at0, at1;
-  bool turned;  // pairs of the rotation, coefficients 8 u + i (vector kernels)
+  int at0, at1, mid0, mid1;
+  bool turned;  // pairs of the rotation, coefficients 8 u + i
+  bool all;     // all eight pairs, or the first four
 };
 
-template <bool VEC>
+template <int MODE>
 __device__ __forceinline__ Place place_of(int u, bool rotates, const Rope& rope) {
-  const bool turned = VEC && rotates && 16 * u < rope.dim;
+  const bool turned = MODE != kByElement && rotates && 16 * u < rope.dim;
   const bool apart = turned && rope.neox;  // the halves of a neox pair lie R / 2 apart
-  return {apart ? 8 * u : 16 * u, apart ? 8 * u + rope.dim / 2 : 16 * u + 8, turned};
+  Place p{apart ? 8 * u : 16 * u, apart ? 8 * u + rope.dim / 2 : 16 * u + 8, 4, 4, turned, true};
+  if (MODE == kByQuad && turned && 16 * u + 8 == rope.dim) {
+    // the last four pairs, and the eight dims behind the rotation
+    p.all = false;
+    if (rope.neox) p.mid0 = rope.dim - p.at0, p.mid1 = rope.dim + 4 - p.at1;
+  }
+  return p;
 }
 
 // Turns a lane's eight pairs: (x, y) -> (x c - y s, y c + x s).
@@ -157,6 +181,25 @@ __device__ __forceinline__ void turn_either(float (&y)[16], const float (&c)[8],
     turn(y, c, s, true);
   else
     turn(y, c, s, false);
+}
+
+// The same of the first four pairs, where those are all; the others' values stay.
+template <int MODE>
+__device__ __forceinline__ void turn_place(float (&y)[16], const float (&c)[8], const float (&s)[8], bool neox, bool all) {
+  float kept[8];
+  if constexpr (MODE == kByQuad) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) kept[i] = neox && i < 4 ? y[4 + i] : y[8 + i];
+  }
+  turn_either(y, c, s, neox);
+  if constexpr (MODE == kByQuad) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float& x = y[8 + i];
+      x = all || (neox && i < 4) ? x : kept[i];
+      if (i < 4) y[4 + i] = all || !neox ? y[4 + i] : kept[i];
+    }
+  }
 }
 
 // Element i < R of a row, element by element: its pair's number, whether it is the
@@ -262,11 +305,11 @@ __device__ __forceinline__ void rescale(const Stand<LANES>& at, int first, uint8
 // `first` on (uniform).  value(it, i, z, unit) loads the lane's part of the run's row
 // i = it * rows + r, z in units of `unit`, and says whether it is to be written; `block` is
 // the block's first row at this lane's head, off[it] how far behind it the lane's part of
-// the round's row lies, its second chunk `apart` bytes on.  ITERS: rounds of rows that stay
+// the round's row lies (place: its chunks).  ITERS: rounds of rows that stay
 // in registers (0: any number of rounds, loaded twice).  UNITS: units other than 1.
-template <bool E5, int LANES, int ITERS, bool UNITS, typename F>
+template <bool E5, int LANES, int ITERS, int MODE, bool UNITS, typename F>
 __device__ __forceinline__ void write_run(const Stand<LANES>& at, bool in, int len, int first, uint8_t* block,
-                                          int64_t stride, const int64_t* off, int apart, float* scale, F value) {
+                                          int64_t stride, const int64_t* off, Place place, float* scale, F value) {
   constexpr int N = ITERS ? ITERS : 1;
   float z[N][16], unit[N];
   bool live[N];
@@ -311,8 +354,8 @@ __device__ __forceinline__ void write_run(const Stand<LANES>& at, bool in, int l
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[e] *= f;
-    store_codes(row, encode8<E5>(x));
-    store_codes(row + apart, encode8<E5>(x + 8));
+    store_chunk<MODE>(row, place.mid0, encode8<E5>(x));
+    store_chunk<MODE>(row + (place.at1 - place.at0), place.mid1, encode8<E5>(x + 8));
   };
   if constexpr (ITERS > 0) {
 #pragma unroll

@@ -391,6 +391,42 @@ def test_moved_rows_are_those_appended_there(device, form, block):
 
 
 # ---------------------------------------------------------------------------
+# Rotations of an odd number of eights
+
+
+HALF_CHUNKS = [
+    # head_dim, rotary, block
+    (80, 40, 16), (80, 40, 1), (64, 24, 4), (64, 56, 1), (128, 8, 64), (16, 8, 16), (112, 56, 32), (128, 120, 1), (48, 24, 64),
+]
+
+
+@pytest.mark.parametrize("neox", [True, False])
+@pytest.mark.parametrize("case", range(len(HALF_CHUNKS)))
+def test_rotations_that_end_inside_a_chunk(device, case, neox):
+    """Infinities and NaN behind the rotation touch no value of it, and q may be q_out."""
+    d, rotary, block = HALF_CHUNKS[case]
+    slots, total = paged_slots(np.random.default_rng(case), [(0, 90), (3, 20), (7, 8)], 64)
+    slots = np.concatenate(slots)
+    rows = torch.randn((len(slots), 4, d), generator=torch.Generator().manual_seed(case))
+    rows[3, 0, rotary], rows[9, 1, d - 1], rows[17, 2, rotary:] = float("inf"), float("nan"), float("-inf")
+    for dtype, form in ((torch.bfloat16, "e4m3"), (torch.float32, "e5m2"), (torch.float16, "e4m3")):
+        print(f"append {HALF_CHUNKS[case]} {dtype} neox {neox}", flush=True)
+        with np.errstate(all="ignore"):
+            _append(device, case, slots, total, hq=0, hk=2, d=d, rotary=rotary, neox=neox, dtype=dtype, form=form,
+                    block=block, rows=rows.to(dtype))
+        _append(device, case, slots, total, hq=3, hk=2, d=d, rotary=rotary, neox=neox, dtype=dtype, form=form, block=block,
+                q_in_place=True, table_dtype=torch.bfloat16 if case % 2 else torch.float32)
+    print(f"move {HALF_CHUNKS[case]} neox {neox}", flush=True)
+    fresh, total = paged_slots(np.random.default_rng(case), [(0, 100), (0, 65), (0, 9)], 64)
+    src, dst = fresh[0][:74], np.concatenate(fresh[1:])
+    pairs = np.random.default_rng(case).integers(0, 600, (74, 2))
+    pairs[::5, 1] = pairs[::5, 0]
+    _move(device, 70 + case, src, dst, pairs, total, layers=2, heads=3, d=d, rotary=rotary, neox=neox, block=block)
+    pairs[7, 0] = 600  # a position outside the table: the other form of the kernel
+    _move(device, 70 + case, src, dst, pairs, total, layers=2, heads=3, d=d, rotary=rotary, neox=neox, block=block, pad=3)
+
+
+# ---------------------------------------------------------------------------
 # Streams and graphs
 
 
