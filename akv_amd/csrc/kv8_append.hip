@@ -6,12 +6,11 @@
 //
 // A wave takes a block's tokens of one head (or of several, blocks being small), rows
 // being the K heads, then the V heads; a run of tokens belongs to the wave whose
-// window holds the run's first entry.  q rows go 64 / LANES heads to a wave, with the
-// token's table row read once: all of a token's heads in one wave from 2048 tokens
-// on, else a wave for each lot of heads, for latency.
+// window holds the run's first entry.  q rows go 64 / LANES heads to a wave (all of a
+// token's heads in one wave, its table row read once: 142 us for 137 below, and never less).
 //
 // Bound by HBM from thousands of tokens on, by the launch below: 32768 tokens of 64 q heads and 8
-// KV heads of 64, 647 MB in 143 us, 4.5 TB/s (a copy: 5.16); one token 4.5 us, 64 4.9.  Rotations
+// KV heads of 64, 647 MB in 136 us, 4.8 TB/s (a copy: 5.16); one token 4.5 us, 64 4.9.  Rotations
 // of an odd number of eights, whose halves end inside a chunk, load and store quads instead
 // (80 dims of which 40 turn: 284 us; element by element 1239; with all 80 turned 196).
 #include "kv8_rows.h"
@@ -85,7 +84,7 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendArgs a
   };
 
   if (unit >= a.kv_units) {
-    // q rows: 64 / LANES heads at a time, the token's cos and sin kept
+    // q rows, 64 / LANES heads of a token
     const int64_t mine = unit - a.kv_units;
     if (mine >= a.q_units) return;
     const int64_t t = mine / a.q_parts;
@@ -95,8 +94,8 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendArgs a
     const int64_t p = position(t);
     float c[8], s[8];
     if (place.turned && p >= 0) coefficients(p, u, place.all, c, s);
-    for (int head = first * (64 / LANES) + sub; head < a.q_heads; head += static_cast<int>(a.q_parts) * (64 / LANES)) {
-      if (16 * u >= a.c.head_dim) break;
+    const int head = first * (64 / LANES) + sub;
+    if (head < a.q_heads && 16 * u < a.c.head_dim) {
       const T* from = static_cast<const T*>(a.q) + t * a.q_st + head * a.q_sh;
       T* to = static_cast<T*>(a.q_out) + t * a.qo_st + head * a.qo_sh;
       float y[16];
@@ -279,12 +278,16 @@ extern "C" int akv_kv8_append(const void* q, int64_t q_stride_t, int64_t q_strid
   const Mode mode = !vec ? kByElement : rotary_dim % 16 ? kByQuad : kByChunk;
   const Shape shape = shape_of(a.c);
   a.head_groups = shape.groups;
-  // entries of a wave: one as long as the waves are few, so that no run waits behind another
+  // Entries of a wave: one where its waves are up to kFewWaves, so that no run waits
+  // behind another; then more, since most waves find a run that began before them (us
+  // by kFewWaves 1024, 4096, 16384, in blocks of 16: 32768 tokens of 8 heads 136, 137, 142 and
+  // with one entry always 366; 2048 tokens 9.1, 10.7, 17.5; 512 tokens 4.8, 6.2, 7.5).
+  constexpr int64_t kFewWaves = 1024;
   a.window = 1;
-  while (a.window < scale_block && n_tokens * shape.groups > 16384ll * a.window) a.window *= 2;
+  while (a.window < scale_block && n_tokens * shape.groups > kFewWaves * a.window) a.window *= 2;
   a.kv_units = pool_slots ? (n_tokens + a.window - 1) / a.window * shape.groups : 0;
   const int rounds = (q_heads + 64 / shape.lanes - 1) / (64 / shape.lanes);
-  a.q_parts = n_tokens >= 2048 ? 1 : std::max(1, rounds);
+  a.q_parts = std::max(1, rounds);
   a.q_units = q_heads ? n_tokens * a.q_parts : 0;
   const int64_t blocks = waves_to_blocks(a.kv_units + a.q_units);
   if (blocks == 0) return AKV_OK;

@@ -29,16 +29,22 @@
 // Q's follow), V^T comes through ds_read_b64_tr_b8.  m is a row's first maximum and
 // moves only when the weights outgrow their types.
 //
+// Bound, for few rows, by HBM: 32 requests of 20000 keys, 8 heads of 64, one token each, blocks
+// of 1: 690 MB in 161 us, 4.3 TB/s, of which the scales, 32 bytes a key in lines of 128, make
+// 5.9 of what is really read; in blocks of 16 146 us.  For many rows by the vector
+// instructions: a part of 32 keys and 64 rows takes 198 of them (32 exponentials, 32
+// scalings before and 32 behind them, 32 sums, 48 conversions) beside 32 products, and they are issued 67%
+// of the time: 512 tokens of 64 heads over 16000 keys 226 us, 0.6 PFLOP/s.  Few keys are
+// bound by the launches and the chain list - slot - code - product: one request of 4096
+// keys 19 us, of which the merge is 4.  A prologue of 6 us and the pieces' results (64 KB
+// of 128 rows of 128 dims) make what is left of 12 requests of up to 20000 keys.
+//
 // Lane layouts (verified on gfx950): v_mfma_f32_16x16x32 -- lane l supplies
 // A[l%16][k(l,i)], B[k(l,i)][l%16] for i < 8 and holds D[4(l/16)+i][l%16];
 // ds_read_b64_tr_b8 -- within each 16-lane group, lane j receives byte j%8
 // of the 8-byte rows read by lanes j/8 + 2i, i < 8.
 #include "tree_common.h"
 
-#ifndef WA
-#define WA 2
-#define WB 3
-#endif
 namespace akv {
 namespace {
 
@@ -52,8 +58,16 @@ typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 constexpr int keys_of(int width) { return width == 64 ? 256 : 128; }
 constexpr int kBuffers = 2;
 
-// What a piece costs beside its tiles, and the least a workgroup is given, in keys.
+// What a piece costs beside its tiles, and the least a workgroup is given, in keys (pieces at
+// 64 to 512 keys: all within 3%; least shares of 128, 256 and 512, us: one request of 20000
+// keys, 8 heads of 64: 26, 22, 24; one of 4096, 4 heads of 128: 18.5, 19.5, 22.4).
 constexpr int kPieceCost = 256, kLeastShare = 256;
+
+// What a tile costs a request by the waves that share its rows out: four of them (the rows
+// of one wave, read by all) 2, two 3, none 4 (us of 12 requests of 11000 keys, 8 heads of
+// 128: 4 rows a head 84, 64 rows 111, 128 rows 157; mixed, 4 to 64 rows: 276 for 303 with
+// equal costs, of 20 to 128 rows 150 for 157).
+constexpr int cost_of_groups(int groups) { return groups == 1 ? 2 : groups == 2 ? 3 : 4; }
 
 struct Kv8Args {
   TreeArgs t;
@@ -172,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     const int64_t left = static_cast<int64_t>(n) * a.group - static_cast<int64_t>(rb) * R;
     if (left <= 0) return 0;
     const int groups = groups_of(static_cast<int>(std::min<int64_t>(left, R)) / HEADS);
-    return static_cast<int32_t>(tiles * (groups == 1 ? WA : groups == 2 ? WB : 4)) + kOver;
+    return static_cast<int32_t>(tiles * cost_of_groups(groups)) + kOver;
   };
   struct Cost {
     int32_t units, rows;
@@ -833,12 +847,14 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
 
 int tile_dim(int32_t head_dim) { return head_dim <= 64 ? 64 : 128; }
 
-// A wave's row subtiles for requests of up to `rows` rows.
+// A wave's row subtiles for requests of up to `rows` rows: two waves' worth, so that
+// pairs of waves share the keys (one and four waves' worth, us: 32 requests of 20000 keys,
+// 8 heads of 64, 32 rows a head 190 by this rule, 184, 195; 64 rows 225, 234, 271; 12 requests
+// of up to 20000, 8 heads of 128, 24 rows 92, 100, 91; 48 rows 108, 110, 117).
 int subtiles_for(int d, int64_t rows) {
   const int most = d == 64 ? 4 : 2;
-  const int64_t groups = d == 64 ? 2 : 4;
   int sub = 1;
-  while (sub < most && rows > 16 * groups * sub) sub *= 2;
+  while (sub < most && rows > 32 * sub) sub *= 2;
   return sub;
 }
 
@@ -848,7 +864,12 @@ struct Launch {
   int32_t row_blocks, block_rows;
 };
 
-constexpr int64_t kWholeKeys = 512, kFullKeys = 1024, kFullGroups = 128;
+// Short requests are not cut: a workgroup has a request and head whole, and nothing is
+// merged.  Up to kWholeBytes of K a request always, up to kFullBytes where they are
+// kFullGroups (us whole and cut, one token a request of one length, 8 heads of 64: 1 request
+// of 800 keys 16.0, 19.5, of 1600 20.9, 21.1; 16 of 1600 22.7, 22.0; 32 of 1600 23.6, 27.0, of
+// 6000 69, 56; 8 heads of 128: 1 of 800 18.9, 18.9, of 1200 22.5, 19.0; 32 of 1600 29, 34).
+constexpr int64_t kWholeBytes = 96 << 10, kFullBytes = 128 << 10, kFullGroups = 256;
 
 Launch plan(int64_t n_tokens, int64_t n_requests, int64_t q_heads, int64_t kv_heads, int32_t head_dim,
             int64_t max_len, int64_t max_new) {
@@ -857,11 +878,16 @@ Launch plan(int64_t n_tokens, int64_t n_requests, int64_t q_heads, int64_t kv_he
   const int64_t rows = most_rows(n_tokens, q_heads, kv_heads, max_new);
   p.sub = subtiles_for(p.d, rows);
   auto blocks = [&]() -> int64_t { return (rows + 16 * kWaves * p.sub - 1) / (16 * kWaves * p.sub); };
-  p.whole = max_len <= kWholeKeys || (max_len <= kFullKeys && n_requests * kv_heads * blocks() >= kFullGroups);
+  p.whole = max_len <= kWholeBytes / p.d ||
+            (max_len <= kFullBytes / p.d && n_requests * kv_heads * blocks() >= kFullGroups);
   // (further blocks of rows follow in the same workgroup)
   const int64_t room = std::max<int64_t>(1, kMostBlocks / std::max<int64_t>(1, n_requests * kv_heads));
   p.row_blocks = static_cast<int32_t>(std::min(blocks(), std::min<int64_t>(room, 4096)));
   const int64_t group = q_heads / kv_heads, head_rows = 16 * kWaves / 2 * p.sub;
+  // two heads to a workgroup, as long as their rows are one block: their rows of 64 codes
+  // share lines of 128 bytes, and their scales one (us of two and one: 32 requests of 20000
+  // keys, blocks of 1, 167 and 216; of 16, 146 and 165).  Not where nothing is cut: the
+  // workgroups are few (1 request of 1600 keys 30 and 21; 128 of 6000 159 and 176)
   p.heads = !p.whole && p.d == 64 && kv_heads % 2 == 0 && rows <= head_rows ? 2 : 1;
   p.block_rows = static_cast<int32_t>(p.heads == 2 ? head_rows / group * 2 * group : 16 * kWaves * p.sub);
   return p;
@@ -876,8 +902,8 @@ int64_t partial_bytes(const Launch& p, int64_t n_tokens, int64_t q_heads) {
 // chip runs whole, but one of fewer requests under the same bounds is cut.
 int64_t largest_bytes(int64_t n_tokens, int64_t q_heads, int64_t kv_heads, int32_t head_dim, int64_t max_len,
                       int64_t max_new) {
-  if (max_len <= kWholeKeys) return 16;
   const int d = tile_dim(head_dim);
+  if (max_len <= kWholeBytes / d) return 16;
   return cut_bytes(d, subtiles_for(d, most_rows(n_tokens, q_heads, kv_heads, max_new)), n_tokens, q_heads);
 }
 
