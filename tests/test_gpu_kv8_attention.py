@@ -542,3 +542,88 @@ def test_is_tree_attention_of_the_same_values(device):
     want, size, spread = drafts.tree_attention(f64(c.q), f64(c.k), f64(c.v), c.visible(seen), 0.125)
     tol = kv8_tolerance(BF16, F32, c.max_len, want, size, spread) + 2.0 ** -8 * (size + np.abs(want)) * 1.01
     assert (np.abs(f64(out) - f64(other)) <= tol).all()
+
+
+# ---------------------------------------------------------------------------
+# Two heads to a workgroup: cut batches of 64 dims and an even number of KV heads
+
+PAIRS = [
+    # q heads, kv heads, head_dim, q dtype, format, page, block, old, new, bound on the new tokens
+    (8, 8, 64, BF16, "e4m3", 1, 1, [1700, 3], [1, 1], 1),
+    (14, 2, 64, BF16, "e5m2", 1, 1, [900, 0, 77], [1, 5, 9], 9),       # groups of 7: blocks end inside no token
+    (60, 4, 64, F16, "e4m3", 16, 16, [400, 1600], [2, 3], 2),          # groups of 15, a request past its bound
+    (64, 2, 64, BF16, "e4m3", 1, 4, [700, 31], [1, 4], 1),             # groups of 32: a token to a block
+    (82, 2, 64, BF16, "e4m3", 16, 1, [500, 90], [1, 3], 1),            # 41: rows of a half-filled block
+    (10, 2, 48, F16, "e5m2", 5, 2, [300, 0, 1100], [20, 33, 40], 6),   # seven blocks of rows
+    (6, 6, 16, BF16, "e4m3", 1, 8, [640, 20], [65, 2], 32),
+    (4, 2, 64, F16, "e4m3", 64, 64, [257, 511], [64, 128], 64),
+]
+
+
+@pytest.mark.parametrize("kind", ["chain", "tree", "any"])
+@pytest.mark.parametrize("case", range(len(PAIRS)))
+def test_pairs_of_heads(device, case, kind):
+    *shape, most = PAIRS[case]
+    print(f"kv8 attention pairs {PAIRS[case]} {kind}", flush=True)
+    c = _cache(device, 1100 + case, shape, capacity=sum(shape[-1]) + case % 2, holes=case % 3)
+    seen, mask = c.masks(kind)
+    sinks = torch.randn(shape[0], generator=torch.Generator().manual_seed(case)).to(device) if case % 2 else None
+    for most_new in (most, c.max_new):
+        out = _run(c, mask=mask, sinks=sinks, max_len=5000, max_new=most_new, out_dtype=F32 if kind == "any" else None)
+        _check(c, out, c.visible(seen), sinks=sinks)
+    starts = np.concatenate([c.rng.integers(0, o + 1, n) for o, n in zip(shape[-2], shape[-1])])
+    full = np.concatenate((starts, np.zeros(c.capacity - c.total, np.int64)))
+    _check(c, _run(c, mask=mask, starts=full, first=5, max_len=5000), c.visible(seen, starts, 5))
+
+
+@pytest.mark.parametrize("form", list(FORMATS))
+def test_what_one_head_of_a_pair_holds_stays_its_own(device, form):
+    """NaN codes and scales of one head, in keys that are seen, make its rows NaN and no others."""
+    c = Cache8(device, 1200, [900, 40], [3, 5], q_heads=12, kv_heads=4, head_dim=64, dtype=BF16, form=form, block=4, page=16)
+    seen, mask = c.masks("tree")
+    plain = _run(c, mask=mask, max_len=5000)
+    for head in range(4):
+        parts = [[codes.clone(), scales.clone()] for codes, scales in c.parts]
+        parts[1][0].view(torch.uint8)[:, head] = 0x7f
+        parts[0][1][:, head] = float("nan")
+        out = _run(c, mask=mask, parts=parts, max_len=5000)
+        others = [h for h in range(12) if h // 3 != head]
+        assert torch.equal(out[: c.total, others], plain[: c.total, others])
+        assert torch.isnan(out[: c.total, 3 * head: 3 * head + 3].float()).all()
+
+
+@pytest.mark.parametrize("block", [1, 16])
+def test_strides_of_pairs(device, block):
+    """K and V interleaved head by head, padded heads, scales with the heads outside."""
+    c = Cache8(device, 1210, [2000, 60], [7, 4], q_heads=8, kv_heads=4, head_dim=64, dtype=BF16, page=16, block=block)
+    both = torch.stack([p[0].view(torch.uint8) for p in c.parts], 2).view(c.parts[0][0].dtype)
+    wide = torch.zeros((*c.parts[0][0].shape[:2], 112), dtype=torch.uint8, device=device)
+    wide[..., 16:80] = c.parts[0][0].view(torch.uint8)
+    outer = [p[1].T.contiguous().T for p in c.parts]
+    beside = torch.stack([p[1] for p in c.parts], -1)
+    seen, mask = c.masks("tree")
+    plain = _run(c, mask=mask, max_len=5000)
+    _check(c, plain, c.visible(seen))
+    for parts in ([[both[:, :, i], outer[i]] for i in (0, 1)],
+                  [[wide[..., 16:80].view(both.dtype), beside[..., 0]], [c.parts[1][0], beside[..., 1]]]):
+        assert torch.equal(_run(c, mask=mask, parts=parts, max_len=5000), plain)
+
+
+@pytest.mark.parametrize("hk,d", [(4, 64), (3, 64), (2, 128)])
+def test_cut_batches_are_the_same_every_time(device, hk, d):
+    """Whatever an earlier call left in the workspace; with more blocks of rows and
+    requests than a wave has lanes, and in a draining batch."""
+    need = kv8.attention_kv8_workspace_bytes(70 * 9 + 300, 70, 4 * hk, hk, d, 5000, 300)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device=device)
+    for requests, long in ((70, 300), (40, 300), (9, 9), (1, 2)):
+        print(f"kv8 attention, {requests} requests cut, {hk} heads of {d}", flush=True)
+        old = [(37 * i) % 130 + 1100 * (i == 0) for i in range(requests)]
+        new = [1 + i % 9 for i in range(requests)]
+        new[-1] = long
+        c = Cache8(device, 1220 + requests, old, new, q_heads=4 * hk, kv_heads=hk, head_dim=d, dtype=BF16)
+        seen, mask = c.masks("chain")
+        first = _run(c, mask=mask, workspace=ws, max_len=5000)
+        _check(c, first, c.visible(seen))
+        for fill in (0, 170):
+            ws.fill_(fill)
+            assert torch.equal(_run(c, mask=mask, workspace=ws, max_len=5000), first)
