@@ -591,11 +591,17 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     // any 32 keys; v0: the first one's number
     auto part = [&](const CodeTile<W>& t, int it, int kk, int v0, uint32_t dead) KV8_INLINE {
       f32x4 sc[2][SUB], ks[2], vs[2];
+      u32x4 k[2][kSteps / 2];
+      u32x2 v[kDTiles];
+      codes_of(t, kk, k);
       scales_of(it, 0, kk, ks);
       scales_of(it, 1, kk, vs);
-      u32x4 k[2][kSteps / 2];
-      codes_of(t, kk, k);
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt) v[dt] = v_tile(t, kk, dt);
       scores(k, sc);
+      uint32_t odd = 0;  // infinities and NaN among the lane's values
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt) odd |= odd_bytes<E5>(v[dt][0]) | odd_bytes<E5>(v[dt][1]);
       uint32_t seen[SUB];  // bit 4 j + i: key 16 j + 4 quad + i
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
@@ -665,13 +671,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
       }
       // A weight of 0 does not hide an infinity or NaN from the product: such codes
       // are taken out of it, and the dims of the rows that see them become NaN.
+      if (__builtin_amdgcn_ballot_w64(odd != 0)) {
 #pragma unroll
-      for (int dt = 0; dt < kDTiles; ++dt) {
-        u32x2 codes = v_tile(t, kk, dt);
-        const u32x2 odd = {odd_bytes<E5>(codes[0]), odd_bytes<E5>(codes[1])};
-        if (__builtin_amdgcn_ballot_w64((odd[0] | odd[1]) != 0)) {
-          codes &= ~((odd >> 7) * 255u);
-          const b8 which = operand<__bf16, E5>((odd >> 7) * (E5 ? 0x3cu : 0x38u));  // ones
+        for (int dt = 0; dt < kDTiles; ++dt) {
+          const u32x2 here = {odd_bytes<E5>(v[dt][0]), odd_bytes<E5>(v[dt][1])};
+          v[dt] &= ~((here >> 7) * 255u);
+          const b8 which = operand<__bf16, E5>((here >> 7) * (E5 ? 0x3cu : 0x38u));  // ones
 #pragma unroll
           for (int s = 0; s < SUB; ++s) {
             b8 sees;
@@ -682,8 +687,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
             for (int i = 0; i < 4; ++i) acc[s][dt][i] = hits[i] > 0.f ? __builtin_nanf("") : acc[s][dt][i];
           }
         }
-        add_values(codes, dt, p);
       }
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt) add_values(v[dt], dt, p);
     };
     __builtin_amdgcn_s_waitcnt(0);  // (one the compiler sees: Q has arrived)
     __syncthreads();
