@@ -54,14 +54,17 @@ typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
 #define KV8_INLINE __attribute__((always_inline))
 
-// Keys of a tile of rows of `width` bytes (32 KiB of K and V), and the tiles in LDS.
-constexpr int keys_of(int width) { return width == 64 ? 256 : 128; }
-constexpr int kBuffers = 2;
+// Keys of a tile (16 or 32 KiB of K and V), and the tiles in LDS.  (256 keys of 64 bytes: one
+// request of 4096 keys, 16 tokens, 28.1 us for 26.6, of 60000 28.7 for 27.6, long ones alike; 64
+// keys of 128 bytes in four places: 32 requests of 20000 keys 182 for 169.)
+constexpr int kKeys = 128, kBuffers = 2;
 
-// What a piece costs beside its tiles, and the least a workgroup is given, in keys (pieces at
-// 64 to 512 keys: all within 3%; least shares of 128, 256 and 512, us: one request of 20000
-// keys, 8 heads of 64: 26, 22, 24; one of 4096, 4 heads of 128: 18.5, 19.5, 22.4).
-constexpr int kPieceCost = 256, kLeastShare = 256;
+// What a piece costs beside its tiles, in keys (64 to 512: all within 3%), and the least a
+// workgroup is given: 128 keys as long as there is a CU for each, else 256 (us with 128, with
+// 256, one token, 8 heads of 64: 1 request of 2000 keys 16.0, 17.1, of 4096 16.2, 17.2, of 8192
+// 18.3, 17.1; of 128: 17.1, 18.5; 17.6, 18.8; 22.4, 19.7).
+constexpr int kPieceCost = 256;
+constexpr int least_share(int log2_groups) { return log2_groups > 8 ? 256 : 128; }
 
 // What a tile costs a request by the waves that share its rows out: four of them (the rows
 // of one wave, read by all) 2, two 3, none 4 (us of 12 requests of 11000 keys, 8 heads of
@@ -119,8 +122,8 @@ __device__ __forceinline__ uint32_t odd_bytes(uint32_t w) {
 
 template <int W>
 struct alignas(16) CodeTile {
-  char k[keys_of(W) * W];  // key-major, 16-byte chunks swizzled per row (swz_k)
-  char v[keys_of(W) * W];  // key-major, read transposed, swizzled (swz_v)
+  char k[kKeys * W];  // key-major, 16-byte chunks swizzled per row (swz_k)
+  char v[kKeys * W];  // key-major, read transposed, swizzled (swz_v)
 };
 
 // T: q's type.  D: 64 or 128, the tile's head width.  SUB: a wave's row subtiles of 16.
@@ -136,7 +139,6 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
   using b8 = Vec<__bf16>::x8;
   constexpr bool kSplit = !__is_same(T, __bf16);  // weights as two bf16 values
   constexpr int W = D * HEADS;                 // bytes of a tile's row
-  constexpr int kKeys = keys_of(W);
   constexpr int kParts = kKeys / 32;
   constexpr int kSteps = D / 32;
   constexpr int kDTiles = D / 16;
@@ -145,10 +147,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
   constexpr int kWaveKeys = kKeys / kWaves;    // keys of a tile that a wave asks for
   constexpr int kEntryTiles = 64 / kWaveKeys;  // tiles whose keys of this wave fill a vector register
   constexpr int kHeadWaves = kWaves / HEADS;   // waves of a head
-  constexpr int kOver = 2 * ((kPieceCost + kKeys - 1) / kKeys);
+  constexpr int kOver = 2 * kPieceCost / kKeys;
   constexpr int kGroupRows = 16 * SUB;         // rows of a wave
   const int R = HEADS == 1 ? kWaves * kGroupRows : ka.block_rows;  // rows of a block
-  __shared__ CodeTile<W> buffers[kBuffers];
+  // (and behind them the waves' results)
+  constexpr int kPlaces = std::max<int>(kBuffers, kWaves * kGroupRows * D * 4 / sizeof(CodeTile<W>));
+  __shared__ CodeTile<W> buffers[kPlaces];
   __shared__ __attribute__((aligned(16))) float s_scale[kBuffers][kWaves][2][kWaveKeys * HEADS];  // the tiles' a_j and c_j
   __shared__ int32_t s_entry[kWaves][2][64];  // list entries of the waves' keys, kEntryTiles tiles at a time
   __shared__ uint32_t s_dead[2 * kEntryTiles][kParts];  // the tiles' keys that no token sees
@@ -231,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
     if (all == 0) return;
     // 2^k stretches: all of the workgroups, or as many as get their least share
     int k = kGroupsShift;
-    while (k > 0 && (static_cast<int64_t>(2 * ((kLeastShare + kKeys - 1) / kKeys)) << k) > all) --k;
+    while (k > 0 && (static_cast<int64_t>(2 * least_share(k) / kKeys) << k) > all) --k;
     if (group_id >> k) return;
     auto cut = [&](int64_t i) { return (all >> k) * i + (((all & ((1 << k) - 1)) * i) >> k); };  // all * i / 2^k
     int64_t x = cut(group_id);
@@ -359,9 +363,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
       const bool past = begin + e * (kEntryTiles * kKeys) + my_key >= end;
       const uint64_t dead = __builtin_amdgcn_ballot_w64(!there || past);
       if (lane < kEntryTiles) {
-        uint32_t* to = s_dead[(e & 1) * kEntryTiles + lane] + kWaveKeys / 32 * wave;
-        to[0] = static_cast<uint32_t>(dead >> (kWaveKeys * lane % 64));
-        if constexpr (kWaveKeys == 64) to[1] = static_cast<uint32_t>(dead >> 32);
+        uint32_t* to = s_dead[(e & 1) * kEntryTiles + lane] + wave;
+        *to = static_cast<uint32_t>(dead >> (kWaveKeys * lane));
       }
     };
     // a wave's keys of a tile, straight into LDS: lane l of a load fills bytes
@@ -890,11 +893,14 @@ Launch plan(int64_t n_tokens, int64_t n_requests, int64_t q_heads, int64_t kv_he
   const int64_t room = std::max<int64_t>(1, kMostBlocks / std::max<int64_t>(1, n_requests * kv_heads));
   p.row_blocks = static_cast<int32_t>(std::min(blocks(), std::min<int64_t>(room, 4096)));
   const int64_t group = q_heads / kv_heads, head_rows = 16 * kWaves / 2 * p.sub;
-  // two heads to a workgroup, as long as their rows are one block: their rows of 64 codes
-  // share lines of 128 bytes, and their scales one (us of two and one: 32 requests of 20000
-  // keys, blocks of 1, 167 and 216; of 16, 146 and 165).  Not where nothing is cut: the
-  // workgroups are few (1 request of 1600 keys 30 and 21; 128 of 6000 159 and 176)
-  p.heads = !p.whole && p.d == 64 && kv_heads % 2 == 0 && rows <= head_rows ? 2 : 1;
+  // Two heads to a workgroup, as long as their rows are one block and K and V outgrow the
+  // last-level cache: their rows of 64 codes share lines of 128 bytes, and their scales one
+  // (us of two and one, blocks of 1 and of 16: 32 requests of 20000 keys 156, 200; 135, 148; 16 84, 106;
+  // 72, 80; 8 49, 47; 43, 42; 64 of 4000 69, 76; 58, 56; 1 of 4096, 16 tokens, 32, 27).  Never
+  // where nothing is cut: the workgroups are few (1 request of 1600 keys 30, 21)
+  constexpr double kPairBytes = 192 << 20;
+  const double bytes = 2. * p.d * n_requests * kv_heads * max_len;
+  p.heads = !p.whole && bytes > kPairBytes && p.d == 64 && kv_heads % 2 == 0 && rows <= head_rows ? 2 : 1;
   p.block_rows = static_cast<int32_t>(p.heads == 2 ? head_rows / group * 2 * group : 16 * kWaves * p.sub);
   return p;
 }

@@ -545,7 +545,10 @@ def test_is_tree_attention_of_the_same_values(device):
 
 
 # ---------------------------------------------------------------------------
-# Two heads to a workgroup: cut batches of 64 dims and an even number of KV heads
+# Two heads to a workgroup: cut batches of 64 dims and an even number of KV heads,
+# by their bounds larger than the last-level cache
+
+LARGE = 10 ** 7
 
 PAIRS = [
     # q heads, kv heads, head_dim, q dtype, format, page, block, old, new, bound on the new tokens
@@ -569,11 +572,11 @@ def test_pairs_of_heads(device, case, kind):
     seen, mask = c.masks(kind)
     sinks = torch.randn(shape[0], generator=torch.Generator().manual_seed(case)).to(device) if case % 2 else None
     for most_new in (most, c.max_new):
-        out = _run(c, mask=mask, sinks=sinks, max_len=5000, max_new=most_new, out_dtype=F32 if kind == "any" else None)
+        out = _run(c, mask=mask, sinks=sinks, max_len=LARGE, max_new=most_new, out_dtype=F32 if kind == "any" else None)
         _check(c, out, c.visible(seen), sinks=sinks)
     starts = np.concatenate([c.rng.integers(0, o + 1, n) for o, n in zip(shape[-2], shape[-1])])
     full = np.concatenate((starts, np.zeros(c.capacity - c.total, np.int64)))
-    _check(c, _run(c, mask=mask, starts=full, first=5, max_len=5000), c.visible(seen, starts, 5))
+    _check(c, _run(c, mask=mask, starts=full, first=5, max_len=LARGE), c.visible(seen, starts, 5))
 
 
 @pytest.mark.parametrize("form", list(FORMATS))
@@ -581,12 +584,12 @@ def test_what_one_head_of_a_pair_holds_stays_its_own(device, form):
     """NaN codes and scales of one head, in keys that are seen, make its rows NaN and no others."""
     c = Cache8(device, 1200, [900, 40], [3, 5], q_heads=12, kv_heads=4, head_dim=64, dtype=BF16, form=form, block=4, page=16)
     seen, mask = c.masks("tree")
-    plain = _run(c, mask=mask, max_len=5000)
+    plain = _run(c, mask=mask, max_len=LARGE)
     for head in range(4):
         parts = [[codes.clone(), scales.clone()] for codes, scales in c.parts]
         parts[1][0].view(torch.uint8)[:, head] = 0x7f
         parts[0][1][:, head] = float("nan")
-        out = _run(c, mask=mask, parts=parts, max_len=5000)
+        out = _run(c, mask=mask, parts=parts, max_len=LARGE)
         others = [h for h in range(12) if h // 3 != head]
         assert torch.equal(out[: c.total, others], plain[: c.total, others])
         assert torch.isnan(out[: c.total, 3 * head: 3 * head + 3].float()).all()
@@ -602,18 +605,19 @@ def test_strides_of_pairs(device, block):
     outer = [p[1].T.contiguous().T for p in c.parts]
     beside = torch.stack([p[1] for p in c.parts], -1)
     seen, mask = c.masks("tree")
-    plain = _run(c, mask=mask, max_len=5000)
+    plain = _run(c, mask=mask, max_len=LARGE)
     _check(c, plain, c.visible(seen))
     for parts in ([[both[:, :, i], outer[i]] for i in (0, 1)],
                   [[wide[..., 16:80].view(both.dtype), beside[..., 0]], [c.parts[1][0], beside[..., 1]]]):
-        assert torch.equal(_run(c, mask=mask, parts=parts, max_len=5000), plain)
+        assert torch.equal(_run(c, mask=mask, parts=parts, max_len=LARGE), plain)
 
 
+@pytest.mark.parametrize("bound", [5000, LARGE])
 @pytest.mark.parametrize("hk,d", [(4, 64), (3, 64), (2, 128)])
-def test_cut_batches_are_the_same_every_time(device, hk, d):
+def test_cut_batches_are_the_same_every_time(device, hk, d, bound):
     """Whatever an earlier call left in the workspace; with more blocks of rows and
     requests than a wave has lanes, and in a draining batch."""
-    need = kv8.attention_kv8_workspace_bytes(70 * 9 + 300, 70, 4 * hk, hk, d, 5000, 300)
+    need = kv8.attention_kv8_workspace_bytes(70 * 9 + 300, 70, 4 * hk, hk, d, bound, 300)
     ws = torch.full((need,), 255, dtype=torch.uint8, device=device)
     for requests, long in ((70, 300), (40, 300), (9, 9), (1, 2)):
         print(f"kv8 attention, {requests} requests cut, {hk} heads of {d}", flush=True)
@@ -622,8 +626,8 @@ def test_cut_batches_are_the_same_every_time(device, hk, d):
         new[-1] = long
         c = Cache8(device, 1220 + requests, old, new, q_heads=4 * hk, kv_heads=hk, head_dim=d, dtype=BF16)
         seen, mask = c.masks("chain")
-        first = _run(c, mask=mask, workspace=ws, max_len=5000)
+        first = _run(c, mask=mask, workspace=ws, max_len=bound)
         _check(c, first, c.visible(seen))
         for fill in (0, 170):
             ws.fill_(fill)
-            assert torch.equal(_run(c, mask=mask, workspace=ws, max_len=5000), first)
+            assert torch.equal(_run(c, mask=mask, workspace=ws, max_len=bound), first)
