@@ -39,6 +39,8 @@ reference repository root):
                 reference rejects page sizes other than 1
                 (``context_reposition.py:153-154``), so this module is the
                 extension's specification, pinned to ``occurrence`` at page size 1.
+``kv8``         a cache held in 8 bits (none in the reference): codes, scales, the
+                runs of a call, rows appended and moved.
 
 How each function is pinned (golden vectors / closed forms / brute force /
 invariants) is stated in its module docstring.  The RoPE tables are not part
