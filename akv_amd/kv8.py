@@ -25,9 +25,10 @@ only (``akv/system/sglang/kernels/ops/attention/context_reposition.py:149-152``)
 import torch
 
 from . import _lib
-from .ops import _KV_DTYPES, _on_device, current_stream_handle
+from .ops import _KV_DTYPES, _on_device, _raw_device, current_stream_handle
 
 _INDEX = {torch.int32: _lib.AKV_I32, torch.int64: _lib.AKV_I64}
+_POINTERS = (torch.int64, torch.uint64)
 _FORMATS = {torch.float8_e4m3fn: _lib.AKV_E4M3, torch.float8_e5m2: _lib.AKV_E5M2}
 
 
@@ -41,14 +42,22 @@ def _cache(k_buffer, v_buffer, k_scales, v_scales, scale_block, at):
         raise ValueError("K/V must be matching float8_e4m3fn or float8_e5m2 [slots, kv_heads, head_dim] buffers")
     if type(scale_block) is not int or not 0 < scale_block <= 64 or scale_block & (scale_block - 1):
         raise ValueError("scale_block must be a power of two up to 64")
-    blocks = -(-shape[0] // scale_block)
-    for s in (k_scales, v_scales):
-        if s.dtype != torch.float32 or s.ndim != 2 or s.shape[0] < blocks or s.shape[1] != shape[1]:
-            raise ValueError("k_scales / v_scales must be f32 [slots / scale_block, kv_heads]")
+    k_blocks, v_blocks = k_scales.shape, v_scales.shape
+    if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32 or len(k_blocks) != 2 or len(v_blocks) != 2 \
+            or min(k_blocks[0], v_blocks[0]) * scale_block < shape[0] or not k_blocks[1] == v_blocks[1] == shape[1]:
+        raise ValueError("k_scales / v_scales must be f32 [slots / scale_block, kv_heads]")
     if at < 0 or not (k_buffer.get_device() == v_buffer.get_device() == k_scales.get_device()
                       == v_scales.get_device() == at):
         raise ValueError("the 8-bit cache's tensors must be on one GPU")
     return form, shape, k_stride, v_stride, k_scales.stride(), v_scales.stride()
+
+
+def _launch(call, device, args):
+    """``call(*args)`` with ``device`` current."""
+    if _raw_device() == device.index:
+        return call(*args)
+    with _on_device(device):
+        return call(*args)
 
 
 def append_kv8(k, v, slot_map, k_buffer, v_buffer, k_scales, v_scales, *, scale_block=1, positions=None,
@@ -82,8 +91,7 @@ def append_kv8(k, v, slot_map, k_buffer, v_buffer, k_scales, v_scales, *, scale_
     if pool[1] != hk or pool[2] != d:
         raise ValueError("the cache must have k's heads and head_dim")
     slots_t = _INDEX.get(slot_map.dtype)
-    if slots_t is None or slot_map.ndim != 1 or slot_map.numel() != n or slot_map.get_device() != at \
-            or not slot_map.is_contiguous():
+    if slots_t is None or slot_map.shape != (n,) or slot_map.get_device() != at or not slot_map.is_contiguous():
         raise ValueError("slot_map must be a contiguous int32/int64 [tokens] tensor on k's device")
     q_args, out_args, hq = (None, 0, 0), (None, 0, 0), 0
     if cos_sin_cache is None:
@@ -92,39 +100,38 @@ def append_kv8(k, v, slot_map, k_buffer, v_buffer, k_scales, v_scales, *, scale_
         rope = (None, _lib.AKV_I32, None, _lib.AKV_F32, 0, 0)
         rotary_dim = 0
     else:
-        table, table_t = cos_sin_cache.stride(), _KV_DTYPES.get(cos_sin_cache.dtype)
+        table, table_t, rope_shape = cos_sin_cache.stride(), _KV_DTYPES.get(cos_sin_cache.dtype), cos_sin_cache.shape
         if rotary_dim is None:
             rotary_dim = d
-        if type(rotary_dim) is not int or not 0 < rotary_dim <= d or rotary_dim % 2 or cos_sin_cache.ndim != 2 \
-                or cos_sin_cache.shape[1] != rotary_dim or table[1] != 1 or table_t is None \
+        if type(rotary_dim) is not int or not 0 < rotary_dim <= d or rotary_dim % 2 or len(rope_shape) != 2 \
+                or rope_shape[1] != rotary_dim or table[1] != 1 or table_t is None \
                 or cos_sin_cache.get_device() != at:
             raise ValueError("the rotation needs a native cos/sin cache matching rotary_dim")
         positions_t = None if positions is None else _INDEX.get(positions.dtype)
-        if positions_t is None or positions.ndim != 1 or positions.numel() != n or positions.get_device() != at \
+        if positions_t is None or positions.shape != (n,) or positions.get_device() != at \
                 or not positions.is_contiguous():
             raise ValueError("positions must be a contiguous int32/int64 [tokens] tensor on k's device")
-        rope = (positions.data_ptr(), positions_t, cos_sin_cache.data_ptr(), table_t, table[0], cos_sin_cache.shape[0])
+        rope = (positions.data_ptr(), positions_t, cos_sin_cache.data_ptr(), table_t, table[0], rope_shape[0])
         if (q is None) != (q_out is None):
             raise ValueError("q and q_out go together")
         if q is not None:
-            q_stride, out_stride = q.stride(), q_out.stride()
-            if q.ndim != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype != dtype or q.get_device() != at \
-                    or q_stride[2] != 1 or q_out.shape != q.shape or q_out.dtype != dtype \
+            q_shape, q_stride, out_stride = q.shape, q.stride(), q_out.stride()
+            if len(q_shape) != 3 or q_shape[0] != n or q_shape[2] != d or q.dtype != dtype or q.get_device() != at \
+                    or q_stride[2] != 1 or q_out.shape != q_shape or q_out.dtype != dtype \
                     or q_out.get_device() != at or out_stride[2] != 1:
                 raise ValueError("q and q_out must be [tokens, q_heads, head_dim] rows of k's dtype and device")
-            hq = q.shape[1]
-            q_args, out_args = (q.data_ptr(), *q_stride[:2]), (q_out.data_ptr(), *out_stride[:2])
+            hq = q_shape[1]
+            q_args, out_args = (q.data_ptr(), q_stride[0], q_stride[1]), (q_out.data_ptr(), out_stride[0], out_stride[1])
     if n == 0:
         return
     device = k.device
-    with _on_device(device):
-        rc = _lib.calls().akv_kv8_append(
-            *q_args, k.data_ptr(), k_stride[0], k_stride[1], v.data_ptr(), v_stride[0], v_stride[1],
-            _KV_DTYPES[dtype], n, hq, hk, d, rotary_dim, 1 if is_neox_style else 0, *rope, *out_args,
-            slot_map.data_ptr(), slots_t, k_buffer.data_ptr(), v_buffer.data_ptr(), form, pool[0], kb[0], kb[1], vb[0],
-            vb[1], k_scales.data_ptr(), v_scales.data_ptr(), scale_block, ks[0], ks[1], vs[0], vs[1],
-            current_stream_handle(device),
-        )
+    rc = _launch(_lib.calls().akv_kv8_append, device, (
+        *q_args, k.data_ptr(), k_stride[0], k_stride[1], v.data_ptr(), v_stride[0], v_stride[1],
+        _KV_DTYPES[dtype], n, hq, hk, d, rotary_dim, 1 if is_neox_style else 0, *rope, *out_args,
+        slot_map.data_ptr(), slots_t, k_buffer.data_ptr(), v_buffer.data_ptr(), form, pool[0], kb[0], kb[1], vb[0],
+        vb[1], k_scales.data_ptr(), v_scales.data_ptr(), scale_block, ks[0], ks[1], vs[0], vs[1],
+        current_stream_handle(device),
+    ))
     if rc:
         _lib.check(rc, "akv_kv8_append")
 
@@ -151,21 +158,21 @@ def reposition_kv8_layers(k_data_ptrs, v_data_ptrs, k_scale_ptrs, v_scale_ptrs, 
     tables = (k_data_ptrs, v_data_ptrs, k_scale_ptrs, v_scale_ptrs)
     layers = k_data_ptrs.numel()
     for t in tables:
-        if t.ndim != 1 or t.numel() != layers or t.dtype not in (torch.uint64, torch.int64) or not t.is_contiguous() \
-                or t.get_device() != at:
+        if t.shape != (layers,) or t.dtype not in _POINTERS or not t.is_contiguous() or t.get_device() != at:
             raise ValueError("Reposition requires contiguous 64-bit layer pointer tables on the KV device")
     count = source_slots.numel()
     for t in (source_slots, destination_slots):
-        if t.ndim != 1 or t.numel() != count or t.dtype != torch.int32 or not t.is_contiguous() or t.get_device() != at:
+        if t.shape != (count,) or t.dtype != torch.int32 or not t.is_contiguous() or t.get_device() != at:
             raise ValueError("Reposition requires contiguous int32 slot vectors on the KV device")
-    if position_pairs.shape != (count, 2) or position_pairs.dtype != torch.int32 or position_pairs.stride(1) != 1 \
+    pair_stride, rope_shape = position_pairs.stride(), cos_sin_cache.shape
+    if position_pairs.shape != (count, 2) or position_pairs.dtype != torch.int32 or pair_stride[1] != 1 \
             or position_pairs.get_device() != at:
         raise ValueError("Reposition requires int32 [N, 2] positions on the KV device")
     if rotary_dim is None:
         rotary_dim = pool[2]
     table, table_t = cos_sin_cache.stride(), _KV_DTYPES.get(cos_sin_cache.dtype)
-    if type(rotary_dim) is not int or not 0 < rotary_dim <= pool[2] or rotary_dim % 2 or cos_sin_cache.ndim != 2 \
-            or cos_sin_cache.shape[1] != rotary_dim or table[1] != 1 or table_t is None \
+    if type(rotary_dim) is not int or not 0 < rotary_dim <= pool[2] or rotary_dim % 2 or len(rope_shape) != 2 \
+            or rope_shape[1] != rotary_dim or table[1] != 1 or table_t is None \
             or cos_sin_cache.get_device() != at:
         raise ValueError("Reposition requires a native cos/sin cache matching rotary_dim")
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1 or status.get_device() != at):
@@ -173,14 +180,13 @@ def reposition_kv8_layers(k_data_ptrs, v_data_ptrs, k_scale_ptrs, v_scale_ptrs, 
     if count == 0 or layers == 0:
         return
     device = k_layout.device
-    with _on_device(device):
-        rc = _lib.calls().akv_kv8_reposition(
-            *(t.data_ptr() for t in tables), layers, form, pool[1], pool[2], rotary_dim, pool[0], kb[0], kb[1], vb[0],
-            vb[1], scale_block, ks[0], ks[1], vs[0], vs[1], source_slots.data_ptr(), destination_slots.data_ptr(),
-            position_pairs.data_ptr(), position_pairs.stride(0), count, cos_sin_cache.data_ptr(), table_t, table[0],
-            cos_sin_cache.shape[0], 1 if is_neox_style else 0, 1 if skip_unmapped else 0,
-            None if status is None else status.data_ptr(), current_stream_handle(device),
-        )
+    rc = _launch(_lib.calls().akv_kv8_reposition, device, (
+        k_data_ptrs.data_ptr(), v_data_ptrs.data_ptr(), k_scale_ptrs.data_ptr(), v_scale_ptrs.data_ptr(), layers, form,
+        pool[1], pool[2], rotary_dim, pool[0], kb[0], kb[1], vb[0], vb[1], scale_block, ks[0], ks[1], vs[0], vs[1],
+        source_slots.data_ptr(), destination_slots.data_ptr(), position_pairs.data_ptr(), pair_stride[0], count,
+        cos_sin_cache.data_ptr(), table_t, table[0], rope_shape[0], 1 if is_neox_style else 0, 1 if skip_unmapped else 0,
+        None if status is None else status.data_ptr(), current_stream_handle(device),
+    ))
     if rc:
         _lib.check(rc, "akv_kv8_reposition")
 
@@ -272,17 +278,16 @@ def attention_kv8(q, k_buffer, v_buffer, k_scales, v_scales, qo_indptr, kv_indpt
         workspace = torch.empty(max(16, need), dtype=torch.uint8, device=device)
     elif workspace.get_device() != at or not workspace.is_contiguous():
         raise ValueError("the workspace must be contiguous, on q's device")
-    with _on_device(device):
-        rc = lib.akv_kv8_attention(
-            q_ptr, q_stride[0], q_stride[1], _KV_DTYPES[dtype], k_buffer.data_ptr(), v_buffer.data_ptr(), form, kb[0],
-            kb[1], vb[0], vb[1], pool[0], k_scales.data_ptr(), v_scales.data_ptr(), scale_block, ks[0], ks[1], vs[0],
-            vs[1], n, n_requests, hq, hk, d, qo_indptr.data_ptr(), kv_indptr.data_ptr(), indptr_t,
-            kv_indices.data_ptr(), stride, width, int(page_size), *mask_args,
-            None if key_starts is None else key_starts.data_ptr(), first_keys,
-            None if sinks is None else sinks.data_ptr(), float(scale), out_ptr, _KV_DTYPES[out_dtype], out_stride[0],
-            out_stride[1], int(max_len), int(max_new), workspace.data_ptr(), workspace.nbytes,
-            None if status is None else status.data_ptr(), current_stream_handle(device),
-        )
+    rc = _launch(lib.akv_kv8_attention, device, (
+        q_ptr, q_stride[0], q_stride[1], _KV_DTYPES[dtype], k_buffer.data_ptr(), v_buffer.data_ptr(), form, kb[0],
+        kb[1], vb[0], vb[1], pool[0], k_scales.data_ptr(), v_scales.data_ptr(), scale_block, ks[0], ks[1], vs[0],
+        vs[1], n, n_requests, hq, hk, d, qo_indptr.data_ptr(), kv_indptr.data_ptr(), indptr_t,
+        kv_indices.data_ptr(), stride, width, int(page_size), *mask_args,
+        None if key_starts is None else key_starts.data_ptr(), first_keys,
+        None if sinks is None else sinks.data_ptr(), float(scale), out_ptr, _KV_DTYPES[out_dtype], out_stride[0],
+        out_stride[1], int(max_len), int(max_new), workspace.data_ptr(), workspace.nbytes,
+        None if status is None else status.data_ptr(), current_stream_handle(device),
+    ))
     if rc:
         _lib.check(rc, "akv_kv8_attention")
     return out
