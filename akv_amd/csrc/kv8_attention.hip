@@ -562,7 +562,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
 #pragma unroll
       for (int dt = 0; dt < kDTiles; ++dt) v[dt] = v_tile(t, kk, dt);
       __builtin_amdgcn_sched_barrier(0);
+      // Products before the other wave's vector instructions, which have time while they
+      // run (12 requests of up to 20000 keys 149 -> 142 us, 512 tokens over 16000 244 -> 237).
+      __builtin_amdgcn_s_setprio(1);
       scores(k, sc);
+      __builtin_amdgcn_s_setprio(0);
       ks[0] *= a.scale_log2;
       ks[1] *= a.scale_log2;
       Weights p[SUB];
@@ -585,10 +589,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
         huge |= sum[s] > 0.25f * kHuge;
       }
       if (__builtin_amdgcn_ballot_w64(huge)) return false;
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int s = 0; s < SUB; ++s) l[s] = sum[s];
 #pragma unroll
       for (int dt = 0; dt < kDTiles; ++dt) add_values(v[dt], dt, p);
+      __builtin_amdgcn_s_setprio(0);
       return true;
     };
     // any 32 keys; v0: the first one's number
