@@ -34,7 +34,7 @@
 // 5.9 of what is really read; in blocks of 16 134 us.  For many rows by the vector
 // instructions: a part of 32 keys and 64 rows takes 198 of them (32 exponentials, 32
 // scalings before and 32 behind them, 32 sums, 48 conversions) beside 32 products, and they are issued 67%
-// of the time: 512 tokens of 64 heads over 16000 keys 227 us, 0.6 PFLOP/s.  Few keys are
+// of the time: 512 tokens of 64 heads over 16000 keys 223 us, 0.6 PFLOP/s.  Few keys are
 // bound by the launches and the chain list - slot - code - product: one request of 4096
 // keys 18 us, of which the merge is 4.  A prologue of 6 us and the pieces' results (64 KB
 // of 128 rows of 128 dims) make what is left of 12 requests of up to 20000 keys.
