@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
   // groups of rows that a head's `left` rows from a block's first on make
   auto groups_of = [&](int left) -> int {
     int groups = kHeadWaves;
-    while (groups > 1 && kHeadWaves / groups < kParts && left <= (groups >> 1) * kGroupRows) groups >>= 1;
+    while (groups > 1 && left <= (groups >> 1) * kGroupRows) groups >>= 1;
     return groups;
   };
   // One wave's view of the batch.  A request costs its tiles, by what the waves have to do
