@@ -303,7 +303,8 @@ __device__ __forceinline__ void rescale(const Stand<LANES>& at, int first, uint8
 
 // One run: the rows that the call brings to one block of a head, from its offset
 // `first` on (uniform).  value(it, i, z, unit) loads the lane's part of the run's row
-// i = it * rows + r, z in units of `unit`, and says whether it is to be written; `block` is
+// i = it * rows + r, z in units of `unit`, and says whether it is to be written (the same for
+// all lanes of a row; where no row of a head is, neither is its scale); `block` is
 // the block's first row at this lane's head, off[it] how far behind it the lane's part of
 // the round's row lies (place: its chunks).  ITERS: rounds of rows that stay
 // in registers (0: any number of rounds, loaded twice).  UNITS: units other than 1.
@@ -314,9 +315,9 @@ __device__ __forceinline__ void write_run(const Stand<LANES>& at, bool in, int l
   float z[N][16], unit[N];
   bool live[N];
   const float before = in && first ? load_scale(scale) : 0.f;
-  float top = 0.f;
+  float top = -1.f;  // below 0: no row is written
   auto settle = [&](bool finite_only) KV8_INLINE {
-    top = 0.f;
+    top = -1.f;
     if constexpr (ITERS > 0) {
 #pragma unroll
       for (int it = 0; it < N; ++it)
@@ -367,7 +368,7 @@ __device__ __forceinline__ void write_run(const Stand<LANES>& at, bool in, int l
       if (in && i < len && value(it, i, z[0], unit[0])) write(z[0], unit[0], block + off[0] + it * at.rows * stride);
     }
   }
-  if (!in) return;
+  if (!in || top < 0.f) return;  // (what the block holds keeps its scale)
   if (first && s != before) rescale<E5>(at, first, block, stride, before, s);
   if (at.u == 0 && at.r == 0) store_scale(scale, s);
 }

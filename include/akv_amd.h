@@ -936,8 +936,10 @@ int akv_kv8_append(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  * two are equal), and are stored as above.  Sources lie outside the blocks that the call writes.  The four
  * pointer tables are DEVICE arrays of n_layers base addresses of buffers and scales
  * that share the given strides.  An entry whose dst is outside [0, pool_slots)
- * (or, with skip_unmapped, 0) is passed over; one whose src is, is not written.  A
- * position outside [0, rope_rows) gives a NaN K row unless both are equal.
+ * (or, with skip_unmapped, 0) is passed over; one whose src is, is not written, nor is
+ * its block's scale where the call brings the block no other row (where it does, the
+ * slot holds nothing any more).  A position outside [0, rope_rows) gives a NaN K row
+ * unless both are equal.
  * status as in akv_reposition_kv_layers_gated.
  */
 int akv_kv8_reposition(const uint64_t* k_ptrs, const uint64_t* v_ptrs,

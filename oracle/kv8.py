@@ -96,7 +96,7 @@ def runs(slots, block, total):
 def store(codes, scales, rows, slots, block, form, live=None, units=1.0):
     """Rows ``[N, heads, D]`` in units ``[N, heads, 1]`` into ``codes`` ``[slots,
     heads, D]`` (the codes' values) and ``scales`` ``[blocks, heads]``, in place.
-    ``live``: rows that are written."""
+    ``live``: rows that are written (a run without any leaves its block's scale as it is)."""
     rows, real = np.asarray(rows), np.asarray(rows).dtype.type
     units = np.broadcast_to(np.asarray(units, dtype=real), (*rows.shape[:2], 1))
     for t, n in runs(slots, block, len(codes)):
@@ -104,6 +104,8 @@ def store(codes, scales, rows, slots, block, form, live=None, units=1.0):
         here = np.arange(t, t + n)
         if live is not None:
             here = here[np.asarray(live)[t: t + n]]
+            if not len(here):
+                continue
         x, unit = rows[here], units[here]
         with np.errstate(over="ignore", invalid="ignore"):
             y = x * unit

@@ -1,0 +1,45 @@
+"""Rows of an 8-bit cache where a call has little to write: destinations without a source."""
+
+import numpy as np
+import pytest
+import torch
+
+from akv_amd import kv8, rope
+from tests.kv8 import layer
+
+pytestmark = pytest.mark.gpu
+
+
+def _pointers(caches):
+    """The Reposition's tables of addresses: K, V, their scales."""
+    return [torch.tensor([c[i][j].data_ptr() for c in caches], dtype=torch.int64, device=caches[0][0][0].device)
+            for j in (0, 1) for i in (0, 1)]
+
+
+def _i32(x, device):
+    return torch.from_numpy(np.ascontiguousarray(x, dtype=np.int32)).to(device)
+
+
+@pytest.mark.parametrize("rotary", [64, 20])
+@pytest.mark.parametrize("skip,source", [(False, -1), (False, 320), (True, 0), (True, -1)])
+@pytest.mark.parametrize("block", [1, 4, 16, 64])
+def test_destinations_without_a_source_keep_codes_and_scale(device, block, skip, source, rotary):
+    """Whole blocks, a block's first slots, slots behind rows: what they hold is the
+    values that they held, in every layer, beside a row that does move."""
+    dst, moved = np.concatenate((np.arange(64, 131), [197, 198, 256])), 256
+    src = np.full(len(dst), source)
+    src[-1] = 7
+    pairs = np.stack((np.arange(len(dst)) + 9, np.arange(len(dst))), 1)
+    caches = [layer(device, 80 + i, 320, 2, 64, "e4m3", block) for i in range(3)]
+    before = [[[t.clone() for t in part] for part in cache] for cache in caches]
+    table = rope.make_table("plain", rotary, 600, base=10000.0, dtype=torch.float32, device=device)
+    (k, ks), (v, vs) = caches[0]
+    kv8.reposition_kv8_layers(*_pointers(caches), k, v, ks, vs, _i32(src, device), _i32(dst, device), _i32(pairs, device),
+                              table, scale_block=block, rotary_dim=rotary, skip_unmapped=skip)
+    slots = np.delete(np.arange(320), moved)
+    blocks = np.delete(np.arange(320 // block), moved // block)
+    for cache, held in zip(caches, before):
+        for (codes, scales), (c0, s0) in zip(cache, held):
+            codes, c0 = codes.view(torch.uint8), c0.view(torch.uint8)
+            assert not torch.equal(codes[moved], c0[moved])
+            assert torch.equal(codes[slots], c0[slots]) and torch.equal(scales[blocks], s0[blocks])

@@ -104,3 +104,19 @@ def test_fp32_rows_are_the_64_bit_rows(form, neox):
     np.testing.assert_allclose(want[moved][..., one], z[moved].real, atol=1e-12)
     np.testing.assert_allclose(want[moved][..., two], z[moved].imag, atol=1e-12)
     np.testing.assert_array_equal(want[~moved], raw[~moved])
+
+
+@pytest.mark.parametrize("form", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("block", [1, 4])
+def test_runs_without_a_live_row_leave_the_block(form, block):
+    """A slot behind rows, a block's first ones, a whole block; of one with a live row the others' codes stay."""
+    rng = np.random.default_rng(block)
+    codes, scales = oracle.rounded(rng.standard_normal((24, 2, 16)) * 40, form), np.full((24 // block, 2), 0.25)
+    slots = np.array([5, 8, 9, 12, 13, 14, 15, 16, 17])
+    live = np.array([0, 0, 0, 0, 0, 0, 0, 0, 1], dtype=bool)
+    before = codes.copy(), scales.copy()
+    oracle.store(codes, scales, np.full((9, 2, 16), 3.0), slots, block, form, live)
+    at = 17 // block
+    np.testing.assert_array_equal(np.delete(codes, 17, 0), np.delete(before[0], 17, 0))
+    np.testing.assert_array_equal(np.delete(scales, at, 0), np.delete(before[1], at, 0))
+    np.testing.assert_array_equal(codes[17] * scales[at][:, None], np.full((2, 16), 3.0))
