@@ -344,10 +344,19 @@ __device__ __forceinline__ void write_run(const Stand<LANES>& at, bool in, int l
   settle(false);
   if (__builtin_amdgcn_ballot_w64(!(top < INFINITY))) settle(true);
   const float s = first ? grown<E5>(top, before) : fitting<E5>(top);
-  // 1 / s: of a power of two by its bits; behind other rows s may be any number
+  // 1 / s: of a power of two by its bits; behind other rows s may be any number, also one
+  // whose inverse is past fp32's range: then 2^-24 / s, of values times 2^24
   float inverse = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, s));
-  if (first) inverse = 1.f / s;
+  bool tiny = false;
+  if (first) {
+    tiny = s < 0x1p-126f;
+    inverse = 1.f / (tiny ? s * 0x1p24f : s);
+  }
   auto write = [&](float (&x)[16], float by, uint8_t* row) KV8_INLINE {
+    if (tiny) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] *= 0x1p24f;
+    }
     float f = inverse;
     if (UNITS) {
       f *= by;

@@ -897,7 +897,8 @@ int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  *     scale that is not positive and finite scales nothing: those codes become 0.  One
  *     below 2^-100 that is too small gives way to the first rule's.)
  * and each value y becomes round(y / s), to nearest, ties to even (y times 1 / s in
- * fp32, which is exact unless s0 is no power of two); values that are not finite
+ * fp32, which is exact unless s0 is no power of two; below 2^-126 both by way of
+ * 2^24); values that are not finite
  * become the format's NaN or infinity (e4m3: NaN).
  *
  * akv_kv8_append: K rows k[t], rotated by row positions[t] of cos_sin as in

@@ -120,9 +120,10 @@ def store(codes, scales, rows, slots, block, form, live=None, units=1.0):
             changed = after != before
             codes[lower] = np.where(changed[None, :, None], rounded(codes[lower] * ratio[None, :, None], form), codes[lower])
         with np.errstate(over="ignore", invalid="ignore"):
-            by = unit * (real(1) / after.astype(real))[None, :, None]
+            lift = np.where(after < 2.0 ** -126, 2.0 ** 24, 1.0).astype(real)  # (1 / s has no fp32 value)
+            by = unit * (real(1) / (after.astype(real) * lift))[None, :, None]
             by = np.where((by == np.inf) & (unit < np.inf), np.finfo(real).max, by)  # (a row of zeros)
-            codes[np.asarray(slots)[here]] = rounded(x * by, form)
+            codes[np.asarray(slots)[here]] = rounded(x * lift[None, :, None] * by, form)
 
 
 def moved_rows(codes, scales, src, pairs, table, block, rotary_dim, neox, real, rotates):

@@ -1,11 +1,12 @@
-"""Rows of an 8-bit cache where a call has little to write: destinations without a source."""
+"""Rows of an 8-bit cache where a call has little to write or tiny units: destinations
+without a source, blocks whose scale lies at the end of fp32's range."""
 
 import numpy as np
 import pytest
 import torch
 
 from akv_amd import kv8, rope
-from tests.kv8 import layer
+from tests.kv8 import layer, values
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +44,30 @@ def test_destinations_without_a_source_keep_codes_and_scale(device, block, skip,
             codes, c0 = codes.view(torch.uint8), c0.view(torch.uint8)
             assert not torch.equal(codes[moved], c0[moved])
             assert torch.equal(codes[slots], c0[slots]) and torch.equal(scales[blocks], s0[blocks])
+
+
+@pytest.mark.parametrize("form", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("scale", [2.0 ** -149, 3 * 2.0 ** -149, 2.0 ** -130, 2.0 ** -127, 2.0 ** -126, 2.0 ** -101])
+def test_rows_behind_the_smallest_scales(device, form, scale):
+    """Rows that a block's tiny scale holds, zeros among them, are their codes in its
+    units, appended or moved there."""
+    hk, d, block = 2, 64, 4
+    units = torch.arange(-8, 8).repeat(4).float()  # whole numbers up to 8 are codes
+    rows = torch.stack((units, torch.zeros(d), units.flip(0)))[:, None].expand(3, hk, d)
+    cache = layer(device, 90, 16, hk, d, form, block)
+    for codes, scales in cache:
+        scales[1:] = scale
+        codes[12:15] = rows.to(device).to(codes.dtype)  # (the source of the move)
+    (kc, ks), (vc, vs) = cache
+    held = [t.view(torch.uint8)[:5].clone() for t in (kc, vc)]
+    x = (rows.double() * scale).float().to(device)
+    assert torch.equal(x.double().cpu(), rows.double() * scale)
+    table = rope.make_table("plain", d, 10, base=10000.0, dtype=torch.float32, device=device)
+    kv8.append_kv8(x, x, torch.arange(5, 8, device=device), kc, vc, ks, vs, scale_block=block)
+    kv8.reposition_kv8_layers(*_pointers([cache]), kc, vc, ks, vs, _i32([12, 13, 14], device), _i32([9, 10, 11], device),
+                              _i32([[3, 3]] * 3, device), table, scale_block=block)
+    for (codes, scales), before in zip(cache, held):
+        assert (scales[1:] == scale).all()
+        assert torch.equal(codes.view(torch.uint8)[:5], before)
+        for at in (5, 9):
+            np.testing.assert_array_equal(values(codes[at: at + 3]), rows.double().numpy())

@@ -120,3 +120,16 @@ def test_runs_without_a_live_row_leave_the_block(form, block):
     np.testing.assert_array_equal(np.delete(codes, 17, 0), np.delete(before[0], 17, 0))
     np.testing.assert_array_equal(np.delete(scales, at, 0), np.delete(before[1], at, 0))
     np.testing.assert_array_equal(codes[17] * scales[at][:, None], np.full((2, 16), 3.0))
+
+
+@pytest.mark.parametrize("form", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("real", [np.float32, np.float64])
+def test_rows_behind_the_smallest_scales(form, real):
+    """Multiples of a scale that holds them are those codes, also where 1 / scale is past fp32's range."""
+    units = np.array([0.0, 1.0, -7.0, 8.0]).repeat(4)[None, None]
+    for scale in (2.0 ** -149, 3 * 2.0 ** -149, 2.0 ** -130, 2.0 ** -126):
+        for unit in (1.0, scale):
+            codes, scales = np.zeros((4, 1, 16)), np.full((1, 1), scale)
+            oracle.store(codes, scales, (units * (scale / unit)).astype(real), [2], 4, form, units=unit)
+            np.testing.assert_array_equal(codes[2:3], units)
+            assert scales[0, 0] == scale
