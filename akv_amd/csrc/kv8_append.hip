@@ -244,6 +244,8 @@ extern "C" int akv_kv8_append(const void* q, int64_t q_stride_t, int64_t q_strid
   AppendArgs a{};
   a.c = Cache{kp_stride_slot, kp_stride_head, vp_stride_slot, vp_stride_head, ks_stride_block, ks_stride_head,
               vs_stride_block, vs_stride_head, pool_slots, kv_heads, head_dim, log2_of(scale_block)};
+  rc = check_apart(who, a.c);
+  if (rc) return rc;
   a.rope = Rope{cos_sin, rope_stride, rope_rows, rotary_dim, cos_sin_dtype, is_neox != 0};
   a.q = q;
   a.k = k;

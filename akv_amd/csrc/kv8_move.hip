@@ -376,6 +376,8 @@ extern "C" int akv_kv8_reposition(const uint64_t* k_ptrs, const uint64_t* v_ptrs
   MoveArgs a{};
   a.c = Cache{k_stride_slot, k_stride_head, v_stride_slot, v_stride_head, ks_stride_block, ks_stride_head,
               vs_stride_block, vs_stride_head, pool_slots, n_heads, head_dim, log2_of(scale_block)};
+  rc = check_apart(who, a.c);
+  if (rc) return rc;
   a.rope = Rope{cos_sin, rope_stride, rope_rows, rotary_dim, cos_sin_dtype, is_neox != 0};
   a.k_ptrs = k_ptrs;
   a.v_ptrs = v_ptrs;

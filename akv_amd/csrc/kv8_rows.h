@@ -20,6 +20,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "row_chunks.h"
 
@@ -431,6 +432,16 @@ int check_cache(const char* who, int32_t format, int32_t heads, int32_t head_dim
   if (scale_block < 1 || scale_block > kMostBlock || (scale_block & (scale_block - 1)))
     return fail(AKV_EINVAL, "%s: scale_block %d (powers of two up to %d)", who, scale_block, kMostBlock);
   if (slots < 0) return fail(AKV_EINVAL, "%s: negative size", who);
+  return AKV_OK;
+}
+
+// Rows and scales that a call writes lie apart: two waves write any two of them.
+int check_apart(const char* who, const Cache& c) {
+  const bool heads = c.heads > 1, slots = c.slots > 1, blocks = c.slots > 1ll << c.log2_block;
+  auto close = [](int64_t one, int64_t two, int64_t to) { return std::abs(one) < to || std::abs(two) < to; };
+  if ((heads && close(c.k_sh, c.v_sh, c.head_dim)) || (slots && close(c.k_ss, c.v_ss, c.head_dim)) ||
+      (heads && close(c.ks_sh, c.vs_sh, 1)) || (blocks && close(c.ks_sb, c.vs_sb, 1)))
+    return fail(AKV_EINVAL, "%s: rows or scales of the cache overlap", who);
   return AKV_OK;
 }
 

@@ -74,7 +74,9 @@ def append_kv8(k, v, slot_map, k_buffer, v_buffer, k_scales, v_scales, *, scale_
     as it is (rows that ``qk_norm_rope`` left in ``k_out``).
 
     A block's tokens follow one another in a call, their slots distinct and
-    ascending by 1, and blocks are filled in order.  A block begun by a call gets, per head, the
+    ascending by 1, and blocks are filled in order (the list is not checked: a block that is
+    come to twice has no defined content).  Scales that blocks or heads share
+    (stride 0) are refused, here and by the Reposition.  A block begun by a call gets, per head, the
     smallest power of two s >= 2^-100 that holds its rows (magnitude <= 448 s, or
     57344 s in e5m2) as its scale; behind earlier rows its scale is
     doubled as often as the new rows need, and the earlier codes are rounded

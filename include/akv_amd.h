@@ -884,11 +884,14 @@ int akv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  * scale_block slots (a power of two up to 64; block s / scale_block) and head, for K
  * and for V; a value is code * scale.  head_dim is a multiple of 16 up to 128.
  * Strides of codes and scales are in elements, the dims of a row are adjacent.
+ * One scale for several blocks or heads (a stride of 0) can be read, but the writers
+ * refuse strides at which rows or scales overlap.
  *
  * The writers fill blocks in ascending order of their slots: the rows that a call
  * brings to a block follow one another in its list, slots ascending by 1, slots are
  * distinct, and the slots of the block below the first of them hold earlier rows
- * (what lies above the last of them holds nothing any more).  With A the largest
+ * (what lies above the last of them holds nothing any more).  No call checks its list:
+ * rows that come to a block in two runs leave its scale and codes undefined.  With A the largest
  * finite magnitude of these rows in a head, the block's scale becomes
  *   first row at the block's first slot: the smallest power of two s >= 2^-100
  *     with A <= F s;
