@@ -71,3 +71,27 @@ def test_rows_behind_the_smallest_scales(device, form, scale):
         assert torch.equal(codes.view(torch.uint8)[:5], before)
         for at in (5, 9):
             np.testing.assert_array_equal(values(codes[at: at + 3]), rows.double().numpy())
+
+
+@pytest.mark.parametrize("form", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("block", [1, 4, 16, 64])
+@pytest.mark.parametrize("d,rotary", [(64, 64), (128, 128), (80, 40), (64, 20)])
+def test_a_table_at_any_address(device, d, rotary, block, form):
+    """Rows of a table an odd number of elements apart, from an odd one on: the same
+    codes and scales, bit for bit, whatever its type."""
+    dst = np.concatenate((np.arange(128, 195), [256]))
+    pairs = np.random.default_rng(block).integers(0, 600, (len(dst), 2))
+    pairs[::7, 1] = pairs[::7, 0]
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        table = rope.make_table("plain", rotary, 600, base=10000.0, dtype=dtype, device=device)
+        wide = torch.full((600, rotary + 9), 7.0, dtype=dtype, device=device)
+        wide[:, 3: 3 + rotary] = table
+        found = []
+        for one in (table, wide[:, 3: 3 + rotary]):
+            caches = [layer(device, 95 + i, 320, 3, d, form, block) for i in range(2)]
+            (k, ks), (v, vs) = caches[0]
+            kv8.reposition_kv8_layers(*_pointers(caches), k, v, ks, vs, _i32(np.arange(len(dst)), device),
+                                      _i32(dst, device), _i32(pairs, device), one, scale_block=block, rotary_dim=rotary)
+            found.append([(codes.view(torch.uint8), scales) for cache in caches for codes, scales in cache])
+        for (c0, s0), (c1, s1) in zip(*found):
+            assert torch.equal(c0, c1) and torch.equal(s0, s1)
