@@ -99,8 +99,12 @@ def store(codes, scales, rows, slots, block, form, live=None, units=1.0):
     ``live``: rows that are written (a run without any leaves its block's scale as it is)."""
     rows, real = np.asarray(rows), np.asarray(rows).dtype.type
     units = np.broadcast_to(np.asarray(units, dtype=real), (*rows.shape[:2], 1))
+    begun = set()
     for t, n in runs(slots, block, len(codes)):
         at, first = slots[t] // block, slots[t] % block
+        if at in begun:
+            raise ValueError("a block's rows follow one another in a call")
+        begun.add(at)
         here = np.arange(t, t + n)
         if live is not None:
             here = here[np.asarray(live)[t: t + n]]

@@ -133,3 +133,12 @@ def test_rows_behind_the_smallest_scales(form, real):
             oracle.store(codes, scales, (units * (scale / unit)).astype(real), [2], 4, form, units=unit)
             np.testing.assert_array_equal(codes[2:3], units)
             assert scales[0, 0] == scale
+
+
+@pytest.mark.parametrize("slots", [[4, 6], [4, -1, 5], [5, 4], [0, 4, 1]])
+def test_lists_that_come_to_a_block_twice(slots):
+    """What such a call leaves is undefined: the oracle says so, and no test compares with it."""
+    rows = np.ones((len(slots), 1, 16))
+    with pytest.raises(ValueError):
+        oracle.store(np.zeros((8, 1, 16)), np.ones((2, 1)), rows, np.array(slots), 4, "e4m3")
+    oracle.store(np.zeros((8, 1, 16)), np.ones((8, 1)), rows, np.array(slots), 1, "e4m3")
