@@ -149,13 +149,14 @@ def reposition_kv8_layers(k_data_ptrs, v_data_ptrs, k_scale_ptrs, v_scale_ptrs, 
     part turned in fp32 from ``position_pairs[t, 0]`` to ``[t, 1]`` (nothing is
     done where they are equal), and stored at its destination as ``append_kv8``
     stores rows: a block's destinations follow one another in the lists, ascending by
-    1, and sources lie outside the blocks that the call writes.  With
-    ``scale_block`` 1 a value that only moves keeps its code and scale (a row of zeros:
-    the least scale).  Slots
-    outside the pool are passed over (with ``skip_unmapped`` 0, too): without a source a destination
-    and its scale stay as they are (but for a block that other rows of the call come to: the slot
-    holds nothing any more).  A position outside the table gives a NaN K row.  ``status``: as
-    for ``reposition_kv_layers_gated``.
+    1, and sources lie outside the blocks that the call writes.  With ``scale_block`` 1 a
+    row that only moves keeps its values exactly, its scale a power of two as
+    ``append_kv8`` leaves it: the least that holds the row (half as large where rounding
+    took the row there; for zeros the least of all); rows under other scales are rounded
+    again.  Slots outside the pool are passed over (with ``skip_unmapped`` 0, too): without
+    a source a destination and its scale stay as they are, but in a block that other
+    rows of the call come to its slot holds nothing any more.  A position outside the
+    table gives a NaN K row.  ``status``: as for ``reposition_kv_layers_gated``.
     """
     at = k_layout.get_device()
     form, pool, kb, vb, ks, vs = _cache(k_layout, v_layout, k_scale_layout, v_scale_layout, scale_block, at)

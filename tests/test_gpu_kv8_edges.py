@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from akv_amd import kv8, rope
-from tests.kv8 import layer, values
+from tests.drafts import f64
+from tests.kv8 import LARGEST, layer, values
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +96,24 @@ def test_a_table_at_any_address(device, d, rotary, block, form):
             found.append([(codes.view(torch.uint8), scales) for cache in caches for codes, scales in cache])
         for (c0, s0), (c1, s1) in zip(*found):
             assert torch.equal(c0, c1) and torch.equal(s0, s1)
+
+
+@pytest.mark.parametrize("form", ["e4m3", "e5m2"])
+def test_appended_values_that_only_move_are_the_same(device, form):
+    """A scale for each token; among the rows some whose largest value was rounded down
+    to what half their scale holds."""
+    n, hk, d, most = 40, 2, 64, LARGEST[form]
+    gen = torch.Generator().manual_seed(9)
+    rows = torch.randn((n, 2 * hk, d), generator=gen) * torch.exp2(torch.randint(-20, 20, (n, 2 * hk, 1), generator=gen).float())
+    rows[::3] *= most / 2 * 1.005 / rows[::3].abs().amax(-1, keepdim=True)
+    cache = layer(device, 91, 2 * n, hk, d, form, 1)
+    (kc, ks), (vc, vs) = cache
+    rows = rows.to(device)
+    kv8.append_kv8(rows[:, :hk], rows[:, hk:], torch.arange(n, device=device), kc, vc, ks, vs)
+    held = [values(c[:n]) * f64(s[:n])[..., None] for c, s in cache]
+    table = rope.make_table("plain", d, 50, base=10000.0, dtype=torch.float32, device=device)
+    at = torch.arange(n, dtype=torch.int32, device=device)
+    kv8.reposition_kv8_layers(*_pointers([cache]), kc, vc, ks, vs, at, at + n, torch.stack((at, at), 1), table)
+    for (c, s), want in zip(cache, held):
+        assert torch.equal(s[n::3], s[:n:3] / 2)
+        np.testing.assert_array_equal(values(c[n:]) * f64(s[n:])[..., None], want)
