@@ -38,6 +38,13 @@
 // bound by the launches and the chain list - slot - code - product: one request of 4096
 // keys 18 us, of which the merge is 4.  A prologue of 6 us and the pieces' results (64 KB
 // of 128 rows of 128 dims) make what is left of 12 requests of up to 20000 keys.
+// The instances of the most rows do not fit 256 registers: 24 are spilled (64 dims, 4 subtiles;
+// pairs of heads 36), 19 (128 dims, 2 subtiles), with fp16 queries 54, 68 and 27; written
+// once a workgroup and read once a piece, around its tiles, never among them.
+//
+// What it does badly: a window over new tokens takes a mask, and with a mask every block of
+// rows visits all of the request's new keys and those from its lowest start on, masked (a
+// window of 128, 64 heads of 64: chunks of 128 tokens 33 us, of 512 74, of 4096 1318).
 //
 // Lane layouts (verified on gfx950): v_mfma_f32_16x16x32 -- lane l supplies
 // A[l%16][k(l,i)], B[k(l,i)][l%16] for i < 8 and holds D[4(l/16)+i][l%16];
@@ -60,9 +67,13 @@ typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 constexpr int kKeys = 128, kBuffers = 2;
 
 // What a piece costs beside its tiles, in keys (64 to 512: all within 3%), and the least a
-// workgroup is given: 128 keys as long as there is a CU for each, else 256 (us with 128, with
-// 256, one token, 8 heads of 64: 1 request of 2000 keys 16.0, 17.1, of 4096 16.2, 17.2, of 8192
-// 18.3, 17.1; of 128: 17.1, 18.5; 17.6, 18.8; 22.4, 19.7).
+// stretch is given, in what as many keys cost a request whose rows one wave has: 128 as long as
+// there is a CU for each, else 256 (us with 128, with 256, one token, 8 heads of 64: 1 request
+// of 2000 keys 16.0, 17.1, of 4096 16.2, 17.2, of 8192 18.3, 17.1; of 128: 17.1, 18.5; 17.6, 18.8;
+// 22.4, 19.7).  More waves' rows make a tile dearer, and a piece's own cost holds no key, so
+// in small batches stretches come without a tile and leave pieces of zeros for the merge: one
+// request of 2000 keys 16 of 128 stretches, with four waves' rows 128 of 256; of 4096 16 and 8
+// of 256; of 60000 none.
 constexpr int kPieceCost = 256;
 constexpr int least_share(int log2_groups) { return log2_groups > 8 ? 256 : 128; }
 
@@ -221,6 +232,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const Kv8Arg
   } else {
     // all work on a line: blocks of rows, KV heads, requests (fastest).  The
     // workgroups take equal stretches of it; a cut falls among a request's tiles.
+    // (Every wave adds up the longest request's blocks of rows over all requests: a
+    // prompt of 8192 tokens among 63 requests of one, 64 heads of 64, takes 1405 us, the two
+    // apart 1263 and 30.)
     int32_t most = 0;
     for (int i = lane; i < a.n_requests; i += 64) most = max(most, cost_of(i, 0).rows);
     blocks = (uniform(__ockl_wfred_max_i32(most)) + R - 1) / R;
@@ -879,6 +893,9 @@ struct Launch {
   int32_t row_blocks, block_rows;
 };
 
+// By the bounds alone, not by the batch's lengths, which the host does not know: a graph
+// captured for the longest context cuts its short requests too.
+//
 // Short requests are not cut: a workgroup has a request and head whole, and nothing is
 // merged.  Up to kWholeBytes of K a request always, up to kFullBytes where they are
 // kFullGroups (us whole and cut, one token a request of one length, 8 heads of 64: 1 request

@@ -44,7 +44,11 @@ enum Fate : int32_t { kTurned, kAtItsPlace, kUnknown, kLeft };
 // Bound by HBM: 19.9k scattered tokens of 36 layers, 8 heads of 64: 1.57 GB in 381 us, 4.1
 // TB/s; 16.4k of 32 layers, 8 heads of 128, in blocks and pages of 16: 2.17 GB in 483 us, 4.5 TB/s
 // (a copy: 5.16).  In blocks of 32 and 64, a wave's rounds held as codes and decoded three times,
-// 649 and 739 us (with the values kept in registers, a wave a SIMD, 1530 and 973).  The arithmetic hides behind it (without any of it 441 and 532 us in an
+// 649 and 659-739 us (with the values kept in registers, a wave a SIMD, 1530 and 973; 52 to 71 registers
+// of the eight rounds' are spilled): one wave has all of a block and head.  Blocks of 2, 4 and 8: 740,
+// 600, 546, since a workgroup has one block, of which few rows fill its waves, behind the whole chain of
+// loads; where that chain is all, 16.4k tokens of a layer's 2 heads of 64, 49, 28 and 17 us, blocks of 1 9.8.
+// The arithmetic hides behind it (without any of it 441 and 532 us in an
 // earlier order).  What is missing in the first are the scales: 32 bytes a token and
 // layer, alone in their lines; with none of them stored a raw copy of these rows takes 307 us,
 // with them 460.
