@@ -8,6 +8,7 @@ import torch
 from akv_amd import kv8, rope
 from tests.drafts import f64
 from tests.kv8 import LARGEST, layer, values
+from tests.test_gpu_kv8_rows import _move
 
 pytestmark = pytest.mark.gpu
 
@@ -117,3 +118,20 @@ def test_appended_values_that_only_move_are_the_same(device, form):
     for (c, s), want in zip(cache, held):
         assert torch.equal(s[n::3], s[:n:3] / 2)
         np.testing.assert_array_equal(values(c[n:]) * f64(s[n:])[..., None], want)
+
+
+@pytest.mark.parametrize("form", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("heads,d,rotary,block", [(3, 64, 64, 2), (2, 64, 64, 4), (5, 128, 128, 16), (1, 80, 40, 16),
+                                                  (2, 64, 20, 8), (2, 96, 96, 32), (4, 128, 64, 64)])
+def test_reposition_behind_rows(device, heads, d, rotary, block, form):
+    """Runs that begin inside a block, whose scale grows for some heads and holds for
+    others; one that fills its block, one of a single row, one that goes on into a fresh block."""
+    first, last = 64 * 3 + 1, 64 * 5 + block + block // 2 + 1
+    dst = np.concatenate((np.arange(first, 64 * 3 + block), [64 * 4 + block - 1], np.arange(64 * 5 + 1, last)))
+    rng = np.random.default_rng(block)
+    src = rng.permutation(64 * 3)[: len(dst)]
+    pairs = rng.integers(0, 600, (len(dst), 2))
+    pairs[::3, 1] = pairs[::3, 0]
+    for neox in (True, False):
+        print(f"move behind rows {heads} {d} {rotary} {block} {form} neox {neox}", flush=True)
+        _move(device, 100 + block, src, dst, pairs, 64 * 7, heads=heads, d=d, rotary=rotary, neox=neox, form=form, block=block)
