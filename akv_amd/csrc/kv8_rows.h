@@ -316,18 +316,18 @@ __device__ __forceinline__ void write_run(const Stand<LANES>& at, bool in, int l
   float z[N][16], unit[N];
   bool live[N];
   const float before = in && first ? load_scale(scale) : 0.f;
-  float top = -1.f;  // below 0: no row is written
+  float top = -1.f;  // below 0: no row is written (one of a unit that is no number counts as 0)
   auto settle = [&](bool finite_only) KV8_INLINE {
     top = -1.f;
     if constexpr (ITERS > 0) {
 #pragma unroll
       for (int it = 0; it < N; ++it)
-        if (live[it]) top = __builtin_fmaxf(top, largest_of(z[it], unit[it], finite_only));
+        if (live[it]) top = __builtin_fmaxf(__builtin_fmaxf(top, 0.f), largest_of(z[it], unit[it], finite_only));
     } else {
       for (int it = 0; it * at.rows < len; ++it) {
         const int i = it * at.rows + at.r;
         if (in && i < len && value(it, i, z[0], unit[0]))
-          top = __builtin_fmaxf(top, largest_of(z[0], unit[0], finite_only));
+          top = __builtin_fmaxf(__builtin_fmaxf(top, 0.f), largest_of(z[0], unit[0], finite_only));
       }
     }
     top = group_max<LANES>(top, at.span);

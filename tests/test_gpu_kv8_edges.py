@@ -6,9 +6,10 @@ import pytest
 import torch
 
 from akv_amd import kv8, rope
+from oracle import kv8 as oracle
 from tests.drafts import f64
-from tests.kv8 import LARGEST, layer, values
-from tests.test_gpu_kv8_rows import _move
+from tests.kv8 import LARGEST, layer, same, values
+from tests.test_gpu_kv8_rows import _move, _want
 
 pytestmark = pytest.mark.gpu
 
@@ -135,3 +136,29 @@ def test_reposition_behind_rows(device, heads, d, rotary, block, form):
     for neox in (True, False):
         print(f"move behind rows {heads} {d} {rotary} {block} {form} neox {neox}", flush=True)
         _move(device, 100 + block, src, dst, pairs, 64 * 7, heads=heads, d=d, rotary=rotary, neox=neox, form=form, block=block)
+
+
+@pytest.mark.parametrize("form", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("rotary", [64, 20])
+@pytest.mark.parametrize("block", [1, 4, 16])
+def test_sources_under_scales_that_are_no_numbers(device, block, rotary, form):
+    """NaN and infinite scales, codes of zero and others under them, to fresh blocks and behind
+    rows: NaN (or infinite) codes, and the scale of the rows that are finite."""
+    cache = layer(device, 97, 192, 2, 64, form, block)
+    for codes, scales in cache:
+        scales[: 32 // block] = float("nan")
+        scales[32 // block: 64 // block] = float("inf")
+        codes.view(torch.uint8)[:48:2] = 0
+    dst = np.concatenate((np.arange(128, 128 + 2 * block), np.arange(160 + (block > 1), 160 + max(block, 2))))
+    src = np.concatenate((np.arange(16, 16 + block), np.arange(47, 47 + len(dst) - block)))
+    pairs = np.stack((np.arange(len(dst)) + 9, np.arange(len(dst))), 1)
+    table = rope.make_table("plain", rotary, 600, base=10000.0, dtype=torch.float32, device=device)
+    with np.errstate(all="ignore"):
+        rows, units = zip(*(oracle.moved_rows(values(c), f64(s), src, pairs, table.cpu().numpy(), block, rotary, True,
+                                              np.float32, i == 0) for i, (c, s) in enumerate(cache)))
+        want = _want(cache, rows, dst, block, form, None, units)
+    (k, ks), (v, vs) = cache
+    kv8.reposition_kv8_layers(*_pointers([cache]), k, v, ks, vs, _i32(src, device), _i32(dst, device),
+                              _i32(pairs, device), table, scale_block=block, rotary_dim=rotary)
+    for got, w in zip(cache, want):
+        same(got, w)
