@@ -437,7 +437,7 @@ int check_cache(const char* who, int32_t format, int32_t heads, int32_t head_dim
 
 // Rows and scales that a call writes lie apart: two waves write any two of them.
 int check_apart(const char* who, const Cache& c) {
-  const bool heads = c.heads > 1, slots = c.slots > 1, blocks = c.slots > 1ll << c.log2_block;
+  const bool heads = c.slots > 0 && c.heads > 1, slots = c.slots > 1, blocks = c.slots > 1ll << c.log2_block;
   auto close = [](int64_t one, int64_t two, int64_t to) { return std::abs(one) < to || std::abs(two) < to; };
   if ((heads && close(c.k_sh, c.v_sh, c.head_dim)) || (slots && close(c.k_ss, c.v_ss, c.head_dim)) ||
       (heads && close(c.ks_sh, c.vs_sh, 1)) || (blocks && close(c.ks_sb, c.vs_sb, 1)))

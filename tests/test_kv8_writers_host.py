@@ -29,6 +29,14 @@ def test_strides_of_one_say_nothing(name):
         assert "batch too large" in _lib.last_error()
 
 
+def test_a_pool_of_nothing_has_no_strides():
+    strides = {name: 0 for name in ("k_stride_slot", "k_stride_head", "v_stride_slot", "v_stride_head", "ks_stride_block",
+                                    "ks_stride_head", "vs_stride_block", "vs_stride_head")}
+    pool = dict(k_pool=None, v_pool=None, k_scales=None, v_scales=None)
+    assert _call(APPEND, pool_slots=0, q_heads=0, **pool, **strides) == 0
+    assert _call(MOVE, pool_slots=0, **strides) == 0
+
+
 def test_scales_of_a_layer_can_be_read():
     """One scale for all blocks and heads is no reason to refuse the attention."""
     assert _call(READ, ks_stride_block=0, ks_stride_head=0, vs_stride_block=0, vs_stride_head=0, workspace_bytes=0) \
